@@ -320,6 +320,50 @@ int pg_sample_tokens(const float* logits, const float* noise, float temperature,
 int pg_commit_topk(int64_t* ids, const int64_t* pred, const float* conf, int B, int S, double keep_percent,
                    int fill_all, int mask_id, int pad_id, int cls_id, int sep_id, int32_t* counts, void* stream);
 
+/* ------------------------------------------------------------------ operators over rows of logits of any vocabulary
+ * logits: T rows of V <= 2^24 entries (dtype PG_F32 or PG_BF16), row t at logits + t*ld elements; any alignment of the element
+ * type.  Entries of a row are ordered by value, ties by the lower index; NaN counts as -inf, -0 as +0.  Workspaces: the
+ * *_workspace_bytes functions (may be 0; then NULL will do); a workspace serves one call at a time.
+ *
+ * pg_top_logits: a teacher's record of each row, for pg_distill_*: the first k <= min(V, 1024) entries (values [T][k] in the
+ * activation type, ids [T][k], in order) and rest[t] = log sum over the other entries of exp(x / temperature) (-inf if there is
+ * none above -inf), summed over those entries themselves: no digits are lost where the first k hold nearly all. */
+int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k);
+int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k, float temperature, void* values, int32_t* ids,
+                  float* rest, void* workspace, int64_t workspace_bytes, void* stream);
+/* pg_sample_tokens over any vocabulary with truncation (generate.py / models.py:24-27 sample the whole softmax).  With
+ * w_v = exp((x_v - max) / temperature), the row keeps its first min(k, n_p, n_m) entries: n_p = those before which less than
+ * top_p of the first k entries' mass lies, n_m = those with w >= min_p.  pred = argmax w_v / noise_v over them (ties: lowest
+ * index; noise ~ Exp(1), row t at noise + t*ld_noise), conf = w_pred / their mass.  top_k 0, top_p 1, min_p 0 switch a filter
+ * off; temperature 0 takes the first entry (conf 1).  A row without an entry above -inf: pred -1, conf 0.  temps / ks / ps / mins
+ * (nullable): settings per row; there out-of-range values mean: temperature <= 0 or NaN 0, k <= 0 off, top_p >= 1 or NaN off,
+ * top_p <= 0 the first entry, min_p <= 0 or NaN off, min_p > 1 as 1. */
+int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V);
+int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
+                       float temperature, int top_k, float top_p, float min_p, const float* temps, const int32_t* ks,
+                       const float* ps, const float* mins, int64_t* pred, float* conf, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+/* Distillation of a student's rows from a teacher's records (values, ids [T][k], k <= 1024; an entry with an id outside 0..V-1
+ * or a value of -inf or NaN is absent).  With t = softmax of values / temperature (and of rest, when given, for the event "any
+ * other token"), s = softmax(logits / temperature):
+ *   loss[t] = weight temperature^2 [ sum_e t_e log(t_e / s_id(e)) + t_rest log(t_rest / s_rest) ].
+ * An id that occurs twice counts as two entries and once in the set that s_rest leaves out.  weights [T] (NULL = 1): a row with
+ * weight 0 is not read and gives loss 0 and gradient 0, and so does a row with no entry or with no logit above -inf.
+ * pg_distill_fwd leaves pg_distill_stash_floats() floats per row for pg_distill_bwd, which writes
+ * dlogits = dloss[t] d loss[t] / d logits (activation type, every entry of every row; dloss NULL = 1);
+ * pg_distill_loss_grad is both in one call, for updates that know the weights beforehand. */
+int64_t pg_distill_stash_floats(void);
+int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k);
+int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
+                   const float* rest, const float* weights, float temperature, float* loss, float* stash, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+int pg_distill_bwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
+                   const float* weights, float temperature, const float* dloss, const float* stash, void* dlogits,
+                   int64_t ld_dlogits, void* stream);
+int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
+                         const float* rest, const float* weights, float temperature, float* loss, void* dlogits,
+                         int64_t ld_dlogits, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ critic head (models.py:76-84,104-105)
  * All fp32.  x is the CLS row of the last hidden state: row b at hidden + b*row_stride
  * (activation dtype).  `stash` holds the three post-ReLU activations and the input copy:

@@ -1,0 +1,524 @@
+// Operators over rows of vocabulary logits: a teacher's top entries with the log-mass of the rest, distillation from such
+// records (loss, gradient, both in one call), and sampling under temperature / top-k / top-p / min-p from given noise.
+//
+// Entries of a row are ordered by value, ties by the lower index: one 64-bit key per entry, (value bits made monotone) << 32 |
+// ~index, is unique, so "the first n entries of a row" is always "the entries whose key is at least B" for one key B.
+// NaN counts as -inf, -0 as +0.
+#include "../../include/protgen_hip.h"
+#include "pg_common.h"
+#include <float.h>
+#include <math.h>
+
+namespace {
+
+constexpr int MAX_K = 1024;
+constexpr int MAX_VOCAB = 1 << 24;  // 2^24 weights of at most 2^40 each fit the 64-bit fixed-point sums
+constexpr double LOG2E = 1.4426950408889634074;
+constexpr double LN2 = 0.69314718055994530942;
+
+__device__ __forceinline__ uint32_t value_key(float x) {
+  x = x + 0.0f;  // -0 -> +0
+  if (x != x) x = -INFINITY;
+  const uint32_t b = __float_as_uint(x);
+  return b ^ (((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ uint64_t entry_key(float x, uint32_t i) { return ((uint64_t)value_key(x) << 32) | (uint32_t)~i; }
+
+// f(index, value) over the n elements at p: elements up to the first 16-byte boundary and behind the last whole 16 bytes one by
+// one, the rest in 16-byte loads.
+template <typename T, int NT, typename F> __device__ __forceinline__ void each(const T* p, int n, F f) {
+  constexpr int E = 16 / (int)sizeof(T);
+  int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
+  if (head > n) head = n;
+  if ((int)threadIdx.x < head) f((int)threadIdx.x, to_f32<T>(p[threadIdx.x]));
+  const int nv = (n - head) / E;
+  for (int v = threadIdx.x; v < nv; v += NT) {
+    float o[E];
+    VecIO<T, E>::load(p + head + v * E, o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(head + v * E + e, o[e]);
+  }
+  for (int i = head + nv * E + threadIdx.x; i < n; i += NT) f(i, to_f32<T>(p[i]));
+}
+
+template <int NT, typename T, typename Op> __device__ __forceinline__ T block_all(T v, T* lds, Op op) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+  if (NT == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = lds[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) v = op(v, lds[w]);
+  return v;
+}
+template <int NT> __device__ __forceinline__ double block_sum(double v, double* lds) {
+  return block_all<NT>(v, lds, [](double a, double b) { return a + b; });
+}
+template <int NT> __device__ __forceinline__ float block_max(float v, float* lds) {
+  return block_all<NT>(v, lds, [](float a, float b) { return fmaxf(a, b); });
+}
+
+// A sum of exponentials held as m, s: sum = s * 2^(m c).  m starts at the lowest finite value, so that neither an empty sum nor
+// entries of -inf ever form inf - inf.
+struct ExpSum { float m, s; };
+__device__ __forceinline__ void exp_sum_add(ExpSum& a, float x, float c) {
+  if (x > a.m) {
+    a.s *= __builtin_amdgcn_exp2f((a.m - x) * c);
+    a.m = x;
+  }
+  a.s += __builtin_amdgcn_exp2f((x - a.m) * c);
+}
+__device__ __forceinline__ ExpSum exp_sum_join(ExpSum a, ExpSum b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + b.s * __builtin_amdgcn_exp2f((b.m - m) * c)};
+}
+template <int NT> __device__ __forceinline__ ExpSum block_exp_sum(ExpSum a, float c, float* lds) {
+  const float m = block_max<NT>(a.m, lds);
+  const float s = block_all<NT>(a.s * __builtin_amdgcn_exp2f((a.m - m) * c), lds, [](float x, float y) { return x + y; });
+  return {m, s};
+}
+
+// 2^t in 64 bits for t <= 0: 2^t = 2^n 2^f, |f| <= 1/2, the Taylor series of 2^f to degree 10 (remainder below 3e-13).
+__device__ __forceinline__ double exp2_f64(double t) {
+  if (!(t > -1000.0)) return 0.0;
+  const double n = rint(t), f = (t - n) * LN2;
+  double p = 1.0 / 3628800.0;
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+
+// ------------------------------------------------------------------ radix selection of one row by a whole workgroup
+// Five digits of the entry key from the top: 11 + 11 + 10 bits of the value, 12 + 12 of the index (the 8 bits between are ones
+// for every index below 2^24).  Each pass counts (and weighs) the entries that share the digits found so far.
+constexpr int SEL_BINS = 4096;
+struct SelLds {
+  uint32_t count[SEL_BINS];
+  uint64_t mass[SEL_BINS];
+  uint64_t wave_mass[16];
+  uint32_t wave_count[16];
+  uint64_t key, above_mass, bin_mass;
+  uint32_t above, bin_count;
+};
+__device__ __constant__ const int SEL_SHIFT[5] = {53, 42, 32, 12, 0};
+__device__ __constant__ const int SEL_BITS[5] = {11, 11, 10, 12, 12};
+
+constexpr double MASS_ONE = 1099511627776.0;  // 2^40: weights are at most 1
+
+// The largest key B such that the entries with key >= B number at least `need` (BY_MASS: weigh at least `need`) among the
+// entries with key >= floor_key; returns their mass through *mass (BY_MASS).  weight(x) in (0, 1].
+template <typename T, int NT, bool BY_MASS, typename W>
+__device__ uint64_t select_key(const T* row, int V, uint64_t floor_key, uint64_t need, W weight, SelLds& s) {
+  uint64_t prefix = 0, mask = 0;
+  for (int d = 0; d < 5; ++d) {
+    const int shift = SEL_SHIFT[d], bins = 1 << SEL_BITS[d];
+    __syncthreads();
+    for (int i = threadIdx.x; i < bins; i += NT) {
+      s.count[i] = 0;
+      if (BY_MASS) s.mass[i] = 0;
+    }
+    __syncthreads();
+    each<T, NT>(row, V, [&](int i, float x) {
+      const uint64_t k = entry_key(x, i);
+      if (k < floor_key || (k & mask) != prefix) return;
+      const int b = (int)(k >> shift) & (bins - 1);
+      atomicAdd(&s.count[b], 1u);
+      if (BY_MASS) atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)(weight(x) * MASS_ONE));
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) {  // walk the bins from the top
+      uint64_t left = need;
+      int b = bins - 1, last = -1;
+      for (; b >= 0; --b) {
+        if (!s.count[b]) continue;
+        const uint64_t have = BY_MASS ? s.mass[b] : s.count[b];
+        last = b;
+        if (have >= left) break;
+        left -= have;
+      }
+      if (b < 0) b = last, left = BY_MASS ? s.mass[b] : s.count[b];  // (fewer than `need`: everything)
+      s.key = (uint64_t)b;
+      s.above_mass = left;
+      s.bin_count = s.count[b];
+      s.bin_mass = BY_MASS ? s.mass[b] : s.count[b];
+    }
+    __syncthreads();
+    prefix |= s.key << shift;
+    mask |= (uint64_t)(bins - 1) << shift;
+    if (d == 2) {  // the bits between value and index
+      prefix |= 0xff000000ull;
+      mask |= 0xff000000ull;
+    }
+    need = s.above_mass;
+    if (s.bin_count == 1 || (!BY_MASS && need == s.bin_count)) break;  // the whole bin is in
+  }
+  // the digits not looked at are zero: every entry of the last bin is at least this key
+  return prefix > floor_key ? prefix : floor_key;
+}
+
+// ------------------------------------------------------------------ top entries
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, float tau,
+                                                 T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest) {
+  __shared__ SelLds sel;
+  __shared__ uint64_t list[MAX_K];
+  __shared__ uint32_t n_list;
+  __shared__ float red[16];
+  const int64_t t = blockIdx.x;
+  const T* row = logits + t * ld;
+  const float c = (float)(LOG2E / (double)tau);
+  const uint64_t B = select_key<T, NT, false>(row, V, 0, K, [](float) { return 0.0; }, sel);
+  int P = 1;
+  while (P < K) P <<= 1;
+  __syncthreads();
+  if (threadIdx.x == 0) n_list = 0;
+  for (int i = threadIdx.x; i < P; i += NT) list[i] = 0;
+  __syncthreads();
+  ExpSum es = {-FLT_MAX, 0.f};
+  float top_rest = -INFINITY;
+  each<T, NT>(row, V, [&](int i, float x) {
+    const uint64_t k = entry_key(x, i);
+    if (k >= B) {
+      list[atomicAdd(&n_list, 1u)] = k;
+    } else {
+      const float v = key_value((uint32_t)(k >> 32));
+      top_rest = fmaxf(top_rest, v);
+      exp_sum_add(es, v, c);
+    }
+  });
+  es = block_exp_sum<NT>(es, c, red);
+  top_rest = block_max<NT>(top_rest, red);
+  // bitonic sort, largest first
+  for (int size = 2; size <= P; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < P / 2; i += NT) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const bool down = (a & size) == 0;
+        const uint64_t x = list[a], y = list[b];
+        if ((x < y) == down) { list[a] = y; list[b] = x; }
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < K; i += NT) {
+    values[t * K + i] = from_f32<T>(key_value((uint32_t)(list[i] >> 32)));
+    ids[t * K + i] = (int32_t)~(uint32_t)list[i];
+  }
+  if (threadIdx.x == 0)
+    rest[t] = top_rest == INFINITY ? INFINITY : es.s > 0.f ? (float)((double)es.m / tau + log((double)es.s)) : -INFINITY;
+}
+
+// ------------------------------------------------------------------ sampling
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld,
+                                                             const float* __restrict__ noise, int64_t ld_noise, int V,
+                                                             float temperature, int top_k, float top_p, float min_p,
+                                                             const float* __restrict__ temps, const int32_t* __restrict__ ks,
+                                                             const float* __restrict__ ps, const float* __restrict__ mins,
+                                                             int64_t* __restrict__ pred, float* __restrict__ conf) {
+  __shared__ SelLds sel;
+  __shared__ double redd[16];
+  __shared__ uint64_t redk[16];
+  const int64_t t = blockIdx.x;
+  const T* row = logits + t * ld;
+  const float* q = noise + t * ld_noise;
+  const float temp = temps ? temps[t] : temperature;
+  int k = ks ? ks[t] : top_k;
+  const float p = ps ? ps[t] : top_p, least = mins ? mins[t] : min_p;
+  uint64_t kmax = 0;
+  each<T, NT>(row, V, [&](int i, float x) { const uint64_t e = entry_key(x, i); kmax = e > kmax ? e : kmax; });
+  kmax = block_all<NT>(kmax, redk, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+  const float m = key_value((uint32_t)(kmax >> 32));
+  const int64_t arg = (int64_t)(uint32_t)~(uint32_t)kmax;
+  if (m == -INFINITY || !(temp > 0.f)) {
+    if (threadIdx.x == 0) {
+      pred[t] = m == -INFINITY ? -1 : arg;
+      conf[t] = m == -INFINITY ? 0.f : 1.f;
+    }
+    return;
+  }
+  const double scale = LOG2E / (double)temp;
+  auto weight = [&](float x) { return x == m ? 1.0 : exp2_f64(((double)x - (double)m) * scale); };
+  uint64_t B = 0;
+  if (k > 0 && k < V) B = select_key<T, NT, false>(row, V, 0, k, weight, sel);
+  if (p < 1.f) {
+    double mass = 0;
+    each<T, NT>(row, V, [&](int i, float x) { if (entry_key(x, i) >= B) mass += (double)(uint64_t)(weight(x) * MASS_ONE); });
+    mass = block_sum<NT>(mass, redd);
+    const double want = ceil((double)p * mass);
+    B = select_key<T, NT, true>(row, V, B, want < 1.0 ? 1 : (uint64_t)want, weight, sel);
+  }
+  const double floor_x = least > 0.f ? (double)m + (double)temp * log(least < 1.f ? (double)least : 1.0) : -INFINITY;
+  double best = -1.0, total = 0.0;
+  uint64_t at = ~0ull;
+  each<T, NT>(row, V, [&](int i, float x) {
+    if (entry_key(x, i) < B || !(x > -INFINITY) || !((double)x >= floor_x || x == m)) return;
+    const double w = weight(x);
+    total += w;
+    const double r = w > 0.0 ? w / (double)q[i] : 0.0;
+    if (r > best || (r == best && (uint64_t)i < at)) { best = r; at = i; }
+  });
+  total = block_sum<NT>(total, redd);
+  const double top = block_all<NT>(best, redd, [](double a, double b) { return a > b ? a : b; });
+  at = block_all<NT>(best == top ? at : (uint64_t)~0ull, redk, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  if (threadIdx.x == 0) {
+    const int64_t i = at == ~0ull ? arg : (int64_t)at;
+    pred[t] = i;
+    conf[t] = (float)(weight(to_f32<T>(row[i])) / total);
+  }
+}
+
+// ------------------------------------------------------------------ distillation
+// Per row kept between forward and backward, all fp32: with c = log2(e)/tau,
+//   student probability of entry v:  exp2((x_v - [0]) c) [1]
+//   gradient (before tau, weight and upstream) of an entry outside the teacher's list:  [3] exp2((x_v - [2]) c)
+//   teacher probability of entry e:  exp2((v_e - [4]) c) [5]
+//   [6]: 1 if the row counts
+constexpr int STASH = 8;
+
+struct DistillArgs {
+  const void* values; const int32_t* ids; const float* rest; const float* weights;
+  int K; float tau;
+};
+
+template <typename T> __device__ __forceinline__ bool valid_entry(const T* values, const int32_t* ids, int e, int V) {
+  return (uint32_t)ids[e] < (uint32_t)V && to_f32<T>(values[e]) > -INFINITY;
+}
+
+// Is entry e the first of its id in the list?  (A list from pg_top_logits has no id twice.)
+template <typename T> __device__ __forceinline__ bool first_of_id(const T* values, const int32_t* ids, int e, int V) {
+  for (int j = 0; j < e; ++j)
+    if (ids[j] == ids[e] && valid_entry(values, ids, j, V)) return false;
+  return true;
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_fwd_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
+                                                         float* __restrict__ loss, float* __restrict__ stash) {
+  extern __shared__ uint32_t member[];  // one bit per entry of the vocabulary: in the teacher's list
+  __shared__ float red[16];
+  const int64_t t = blockIdx.x;
+  float* st = stash + t * STASH;
+  const float w = a.weights ? a.weights[t] : 1.f;
+  const T* row = logits + t * ld;
+  const T* values = (const T*)a.values + t * a.K;
+  const int32_t* ids = a.ids + t * a.K;
+  const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
+  const bool tail = a.rest != nullptr;
+  if (w == 0.f) {
+    if (threadIdx.x < STASH) st[threadIdx.x] = 0.f;
+    if (threadIdx.x == 0) loss[t] = 0.f;
+    return;
+  }
+  if (tail) {
+    for (int i = threadIdx.x; i < (V + 31) / 32; i += NT) member[i] = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.K; e += NT)
+      if (valid_entry(values, ids, e, V)) atomicOr(&member[ids[e] >> 5], 1u << (ids[e] & 31));
+    __syncthreads();
+  }
+  ExpSum o = {-FLT_MAX, 0.f};  // entries outside the list (tail) or all
+  each<T, NT>(row, V, [&](int i, float x) {
+    if (!tail || !((member[i >> 5] >> (i & 31)) & 1)) exp_sum_add(o, x, c);
+  });
+  // (a NaN never becomes the maximum, but makes the sum NaN)
+  o = block_exp_sum<NT>(o, c, red);
+  ExpSum all = o;
+  ExpSum te = {-FLT_MAX, 0.f};
+  if (tail) {
+    ExpSum in = {-FLT_MAX, 0.f};
+    for (int e = threadIdx.x; e < a.K; e += NT)
+      if (valid_entry(values, ids, e, V) && first_of_id(values, ids, e, V)) exp_sum_add(in, to_f32<T>(row[ids[e]]), c);
+    all = exp_sum_join(o, block_exp_sum<NT>(in, c, red), c);
+  }
+  for (int e = threadIdx.x; e < a.K; e += NT)
+    if (valid_entry(values, ids, e, V)) exp_sum_add(te, to_f32<T>(values[e]), c);
+  te = block_exp_sum<NT>(te, c, red);
+  const float rest = tail ? a.rest[t] : -INFINITY;  // in units of x / tau
+  const bool has_rest = rest > -INFINITY;
+  float tr = 0.f, log_tr = 0.f;
+  const bool entries = te.s > 0.f;
+  if (has_rest) {
+    const ExpSum r = {rest * a.tau, 1.f};
+    const ExpSum both = entries ? exp_sum_join(te, r, c) : r;
+    te = both;
+    tr = __builtin_amdgcn_exp2f((r.m - te.m) * c) / te.s;
+    log_tr = (r.m - te.m) * inv_tau - logf(te.s);
+  }
+  const bool live = entries && all.s != 0.f;
+  float part = 0.f;
+  const float shift = logf(all.s) - logf(te.s);
+  if (live)
+    for (int e = threadIdx.x; e < a.K; e += NT)
+      if (valid_entry(values, ids, e, V)) {
+        const float v = to_f32<T>(values[e]), pe = __builtin_amdgcn_exp2f((v - te.m) * c) / te.s;
+        if (pe > 0.f) part += pe * (((v - te.m) - (to_f32<T>(row[ids[e]]) - all.m)) * inv_tau + shift);
+      }
+  part = block_all<NT>(part, red, [](float x, float y) { return x + y; });
+  if (threadIdx.x == 0) {
+    float coef = 0.f;
+    if (live) {
+      if (tr > 0.f) part += tr * (log_tr - ((o.m - all.m) * inv_tau + logf(o.s) - logf(all.s)));
+      const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
+      coef = o.s != 0.f ? (sr - tr) / o.s : 0.f;
+    }
+    loss[t] = live ? w * a.tau * a.tau * part : 0.f;
+    st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
+    st[2] = o.m; st[3] = coef;
+    st[4] = te.m; st[5] = live ? 1.f / te.s : 0.f;
+    st[6] = live ? 1.f : 0.f; st[7] = 0.f;
+  }
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
+                                                         const float* __restrict__ upstream, const float* __restrict__ stash,
+                                                         T* __restrict__ grad, int64_t ld_grad) {
+  const int64_t t = blockIdx.x;
+  const float* st = stash + t * STASH;
+  const T* row = logits + t * ld;
+  T* out = grad + t * ld_grad;
+  const T* values = (const T*)a.values + t * a.K;
+  const int32_t* ids = a.ids + t * a.K;
+  const float c = (float)(LOG2E / (double)a.tau);
+  if (st[6] == 0.f) {
+    for (int i = threadIdx.x; i < V; i += NT) out[i] = from_f32<T>(0.f);
+    return;
+  }
+  const float f = (a.weights ? a.weights[t] : 1.f) * a.tau * (upstream ? upstream[t] : 1.f);
+  const float mo = st[2], co = st[3] * f;
+  each<T, NT>(row, V, [&](int i, float x) { out[i] = from_f32<T>(__builtin_amdgcn_exp2f((x - mo) * c) * co); });
+  __threadfence_block();
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.K; e += NT) {
+    if (!valid_entry(values, ids, e, V) || !first_of_id(values, ids, e, V)) continue;
+    float te = 0.f;
+    for (int j = e; j < a.K; ++j)
+      if (ids[j] == ids[e] && valid_entry(values, ids, j, V)) te += __builtin_amdgcn_exp2f((to_f32<T>(values[j]) - st[4]) * c) * st[5];
+    const float s = __builtin_amdgcn_exp2f((to_f32<T>(row[ids[e]]) - st[0]) * c) * st[1];
+    out[ids[e]] = from_f32<T>((s - te) * f);
+  }
+}
+
+int check_launch() { return hipGetLastError() == hipSuccess ? PG_OK : PG_ERR_LAUNCH; }
+
+int check_rows(int dtype, const void* logits, int64_t ld, int T, int V) {
+  if (!logits || T <= 0 || V <= 0 || ld < 0 || (dtype != PG_F32 && dtype != PG_BF16)) return PG_ERR_ARG;
+  return V > MAX_VOCAB ? PG_ERR_UNSUPPORTED : PG_OK;
+}
+int check_distill(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
+                  float tau) {
+  const int rc = check_rows(dtype, logits, ld, T, V);
+  if (rc != PG_OK) return rc;
+  if (!values || !ids || k <= 0 || !(tau > 0.f) || !(tau <= FLT_MAX)) return PG_ERR_ARG;
+  return k > MAX_K ? PG_ERR_UNSUPPORTED : PG_OK;
+}
+
+template <typename T>
+int distill_forward(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, float* stash, hipStream_t s) {
+  const size_t lds = a.rest ? (size_t)((V + 31) / 32) * 4 : 0;
+  if (lds > 128 * 1024) return PG_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, stash);
+  return check_launch();
+}
+
+}  // namespace
+
+extern "C" int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k) { return 0; }
+
+extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k, float temperature, void* values,
+                             int32_t* ids, float* rest, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_rows(dtype, logits, ld, T, V);
+  if (rc != PG_OK) return rc;
+  if (!values || !ids || !rest || k <= 0 || k > V || !(temperature > 0.f) || !(temperature <= FLT_MAX)) return PG_ERR_ARG;
+  if (k > MAX_K) return PG_ERR_UNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PG_F32)
+    hipLaunchKernelGGL((top_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, V, k, temperature,
+                       (float*)values, ids, rest);
+  else
+    hipLaunchKernelGGL((top_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, V, k, temperature,
+                       (bf16_t*)values, ids, rest);
+  return check_launch();
+}
+
+extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V) { return 0; }
+
+extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
+                                  float temperature, int top_k, float top_p, float min_p, const float* temps, const int32_t* ks,
+                                  const float* ps, const float* mins, int64_t* pred, float* conf, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  const int rc = check_rows(dtype, logits, ld, T, V);
+  if (rc != PG_OK) return rc;
+  if (!noise || ld_noise < 0 || !pred || !conf) return PG_ERR_ARG;
+  if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
+      (!mins && !(min_p >= 0.f && min_p <= 1.f)))
+    return PG_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PG_F32)
+    hipLaunchKernelGGL((sample_filtered_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, noise, ld_noise,
+                       V, temperature, top_k, top_p, min_p, temps, ks, ps, mins, pred, conf);
+  else
+    hipLaunchKernelGGL((sample_filtered_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, noise,
+                       ld_noise, V, temperature, top_k, top_p, min_p, temps, ks, ps, mins, pred, conf);
+  return check_launch();
+}
+
+extern "C" int64_t pg_distill_stash_floats(void) { return STASH; }
+extern "C" int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k) { return (int64_t)T * STASH * 4; }
+
+extern "C" int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids,
+                              int k, const float* rest, const float* weights, float temperature, float* loss, float* stash,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  const int rc = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
+  if (rc != PG_OK) return rc;
+  if (!loss || !stash) return PG_ERR_ARG;
+  const DistillArgs a = {values, ids, rest, weights, k, temperature};
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == PG_F32 ? distill_forward((const float*)logits, ld, T, V, a, loss, stash, s)
+                         : distill_forward((const bf16_t*)logits, ld, T, V, a, loss, stash, s);
+}
+
+extern "C" int pg_distill_bwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids,
+                              int k, const float* weights, float temperature, const float* dloss, const float* stash,
+                              void* dlogits, int64_t ld_dlogits, void* stream) {
+  const int rc = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
+  if (rc != PG_OK) return rc;
+  if (!stash || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
+  const DistillArgs a = {values, ids, nullptr, weights, k, temperature};
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PG_F32)
+    hipLaunchKernelGGL((distill_bwd_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, V, a, dloss, stash,
+                       (float*)dlogits, ld_dlogits);
+  else
+    hipLaunchKernelGGL((distill_bwd_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, V, a, dloss, stash,
+                       (bf16_t*)dlogits, ld_dlogits);
+  return check_launch();
+}
+
+extern "C" int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, int T, int V, const void* values,
+                                    const int32_t* ids, int k, const float* rest, const float* weights, float temperature,
+                                    float* loss, void* dlogits, int64_t ld_dlogits, void* workspace, int64_t workspace_bytes,
+                                    void* stream) {
+  const int bad = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
+  if (bad != PG_OK) return bad;
+  if (!loss || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
+  if (!workspace || workspace_bytes < pg_distill_workspace_bytes(dtype, T, V, k)) return PG_ERR_WORKSPACE;
+  float* stash = (float*)workspace;
+  const int rc = pg_distill_fwd(dtype, logits, ld, T, V, values, ids, k, rest, weights, temperature, loss, stash, nullptr, 0, stream);
+  if (rc != PG_OK) return rc;
+  return pg_distill_bwd(dtype, logits, ld, T, V, values, ids, k, weights, temperature, nullptr, stash, dlogits, ld_dlogits, stream);
+}

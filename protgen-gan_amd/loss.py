@@ -11,7 +11,9 @@ g = dS/dx and n_b = ||g_b * m||:
 Forward = encoder forward (primal stash) + first-order reverse to the input (adjoint
 stash).  Backward = one tangent-forward pass along v (tangent stash) + one reverse pass
 over the (primal, tangent) pair, which adds the parameter gradients straight into the
-flat gradient buffer.  Every pass is one C call into libprotgen_hip.so."""
+flat gradient buffer.  Every pass is one C call into libprotgen_hip.so.
+
+`distillation_loss` (no counterpart in the reference) trains a student generator from a teacher's top logits."""
 from __future__ import annotations
 
 import torch
@@ -133,3 +135,36 @@ def compute_gradient_penalty(critic, real_data, fake_data, real_mask, fake_mask,
     joint = (real_mask.to(real.device).bool() & fake_mask.to(real.device).bool()).to(torch.float32).contiguous()
     params = [p for p in critic.parameters() if p.requires_grad]
     return _GradientPenaltyFn.apply(critic, real, fake, joint, alpha, *params)
+
+
+class _DistillFn(torch.autograd.Function):
+    """Forward: row losses and eight numbers per row (pg_distill_fwd); backward: one pass that reads the logits again and writes
+    their gradient (pg_distill_bwd)."""
+
+    @staticmethod
+    def forward(ctx, logits, values, ids, rest, weights, temperature):
+        loss, stash = ops.distill_fwd(logits, values, ids, rest, weights, temperature)
+        ctx.save_for_backward(logits, values, ids, weights, stash)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, values, ids, weights, stash = ctx.saved_tensors
+        return (ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature),) + (None,) * 5
+
+
+def distillation_loss(student_logits, top_values, top_ids, rest=None, temperature=1.0, weights=None):
+    """Per-row distillation of student_logits [..., V] (fp32 or bf16) from a teacher's record (ops.top_logits at the same
+    temperature): with t = softmax of the record / temperature and s = softmax(student_logits / temperature),
+
+        loss = weights * temperature^2 * sum_e t_e log(t_e / s_e)          (fp32 [...])
+
+    over the record's entries e and, with `rest`, the event "any other token" (without it the teacher is renormalised over its
+    entries).  `weights` fp32 [...]: rows with weight 0 (padding, positions that are not scored) are not read and get no
+    gradient, whatever they hold.  Differentiable in student_logits, once; ids outside the vocabulary (-1) mark absent entries."""
+    for name, t in (("top_values", top_values), ("rest", rest), ("weights", weights)):
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{name} requires a gradient: the loss is differentiable in the student's logits only")
+    return _DistillFn.apply(student_logits, top_values, top_ids, rest, weights, float(temperature))

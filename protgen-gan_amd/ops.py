@@ -221,6 +221,178 @@ def sample_tokens(logits, noise, temperature: float, pred=None, conf=None):
     return pred, conf
 
 
+# ----------------------------------------------------------------------------- rows of logits
+def _rows(x, what="logits"):
+    """x [..., V] as (T, V, ld): rows of unit stride at a common distance, without a copy."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what}: expected [..., V] with V >= 1, got {tuple(x.shape)}")
+    if x.dim() != 2:
+        try:
+            x = x.view(-1, x.shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{what}: the leading dimensions of {tuple(x.shape)} have no common row stride; pass a contiguous tensor")
+    T, V = x.shape
+    if V > 1 and x.stride(1) != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    return T, V, (x.stride(0) if T > 1 else V)
+
+
+def _launch(x, name, args, nbytes=0):
+    """check(lib.name(*args[, workspace, bytes], stream)) on x's device and its current stream.  The workspace comes from the
+    caching allocator: calls on other streams, and captured graphs, have their own."""
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(x, name, args, nbytes)
+    if nbytes is not None:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        args += (ptr(ws), nbytes)
+    check(getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+
+
+def _same(device, **tensors):
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name} on {t.device}, logits on {device}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _positive(temperature):
+    temperature = float(temperature)
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return temperature
+
+
+def top_logits(logits, k: int, temperature: float = 1.0):
+    """A teacher's record of each row of logits [..., V] (fp32 or bf16), for distill_loss_grad and
+    loss.distillation_loss: (values [..., k], ids int32 [..., k], rest fp32 [...]), the k largest entries in order (ties: the
+    lower index first; NaN counts as -inf) and the log of the other entries' sum of exp(x / temperature)."""
+    dt = dt_code(logits.dtype)
+    T, V, ld = _rows(logits)
+    k, temperature = int(k), _positive(temperature)
+    if not 1 <= k <= min(V, TOP_LOGITS_MAX):
+        raise ValueError(f"k must lie in 1..min(V, {TOP_LOGITS_MAX}) = {min(V, TOP_LOGITS_MAX)}, got {k}")
+    _need_cuda(logits)
+    lead = logits.shape[:-1]
+    values = torch.empty(*lead, k, dtype=logits.dtype, device=logits.device)
+    ids = torch.empty(*lead, k, dtype=torch.int32, device=logits.device)
+    rest = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    if T:
+        _launch(logits, "pg_top_logits", (dt, logits.data_ptr(), ld, T, V, k, temperature, values.data_ptr(), ids.data_ptr(),
+                                          rest.data_ptr()), lib.pg_top_logits_workspace_bytes(dt, T, V, k))
+    return values, ids, rest
+
+
+TOP_LOGITS_MAX = 1024  # entries of a teacher's record
+
+
+def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, pred=None, conf=None):
+    """One token per row of logits [T, V] (fp32 or bf16, any V) from the softmax at `temperature`, cut to the first `top_k`
+    entries (0: all), of those to the smallest leading set that holds `top_p` of their mass, and to the entries of at least
+    `min_p` times the largest probability.  `noise` fp32 [T, V] ~ Exp(1): the token is the argmax of p / noise, as in
+    sample_tokens; only the kept entries' noise is read.  Every setting is a number or a tensor [T] on the device (fp32; top_k:
+    int32), read per row without a check.  temperature 0: the largest entry.  Returns (pred int64 [T], conf fp32 [T]), conf the
+    token's probability among the kept entries; a row with nothing above -inf gives (-1, 0)."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits: expected [T, V], got {tuple(logits.shape)}")
+    dt = dt_code(logits.dtype)
+    T, V, ld = _rows(logits)
+    dev = logits.device
+    _same(dev, noise=(noise, torch.float32, (T, V)))
+    ld_noise = _rows(noise, "noise")[2]
+    rows = {}
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(v) and v.dim():
+            _same(dev, **{name: (v, dtype, (T,))})
+            rows[name] = v.contiguous()
+    num = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
+    for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if name not in rows:
+            num[name] = int(v) if name == "top_k" else float(v)
+    if not 0.0 <= num["temperature"] < float("inf"):
+        raise ValueError(f"temperature must be finite and not negative, got {num['temperature']}")
+    if num["top_k"] < 0:
+        raise ValueError(f"top_k must not be negative, got {num['top_k']}")
+    if not 0.0 < num["top_p"] <= 1.0:
+        raise ValueError(f"top_p must lie in (0, 1], got {num['top_p']}")
+    if not 0.0 <= num["min_p"] <= 1.0:
+        raise ValueError(f"min_p must lie in [0, 1], got {num['min_p']}")
+    _need_cuda(logits)
+    if pred is None:
+        pred = torch.empty(T, dtype=torch.int64, device=dev)
+    if conf is None:
+        conf = torch.empty(T, dtype=torch.float32, device=dev)
+    _same(dev, pred=(pred, torch.int64, (T,)), conf=(conf, torch.float32, (T,)))
+    if not (pred.is_contiguous() and conf.is_contiguous()):
+        raise ValueError("pred and conf must be contiguous")
+    if T:
+        _launch(logits, "pg_sample_filtered",
+                (dt, logits.data_ptr(), ld, noise.data_ptr(), ld_noise, T, V, num["temperature"], min(num["top_k"], V), num["top_p"],
+                 num["min_p"], ptr(rows.get("temperature")), ptr(rows.get("top_k")), ptr(rows.get("top_p")),
+                 ptr(rows.get("min_p")), pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V))
+    return pred, conf
+
+
+def _distill_args(logits, values, ids, rest, weights, temperature):
+    dt = dt_code(logits.dtype)
+    T, V, ld = _rows(logits)
+    lead, k = logits.shape[:-1], values.shape[-1] if values.dim() else 0
+    if not 1 <= k <= TOP_LOGITS_MAX:
+        raise ValueError(f"values must hold 1..{TOP_LOGITS_MAX} entries per row, got {k}")
+    _same(logits.device, values=(values, logits.dtype, (*lead, k)), ids=(ids, torch.int32, (*lead, k)),
+          rest=(rest, torch.float32, lead), weights=(weights, torch.float32, lead))
+    temperature = _positive(temperature)
+    _need_cuda(logits)
+    values, ids = values.contiguous(), ids.contiguous()
+    rest = rest if rest is None else rest.contiguous()
+    weights = weights if weights is None else weights.contiguous()
+    return dt, T, V, ld, k, values, ids, rest, weights, temperature
+
+
+def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
+    """Row losses of loss.distillation_loss (fp32 [...]) and the stash distill_bwd needs."""
+    dt, T, V, ld, k, values, ids, rest, weights, temperature = _distill_args(logits, values, ids, rest, weights, temperature)
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    stash = torch.empty(T * lib.pg_distill_stash_floats(), dtype=torch.float32, device=logits.device)
+    if T:
+        _launch(logits, "pg_distill_fwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest),
+                                           ptr(weights), temperature, loss.data_ptr(), stash.data_ptr()),
+                lib.pg_distill_workspace_bytes(dt, T, V, k))
+    return loss, stash
+
+
+def distill_bwd(logits, values, ids, stash, dloss, weights=None, temperature=1.0):
+    """d sum(dloss * loss) / d logits, contiguous, in the logits' type.  `stash` from distill_fwd on the same arguments."""
+    dt, T, V, ld, k, values, ids, _, weights, temperature = _distill_args(logits, values, ids, None, weights, temperature)
+    _same(logits.device, dloss=(dloss, torch.float32, logits.shape[:-1]))
+    dloss = dloss.contiguous()
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if T:
+        _launch(logits, "pg_distill_bwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(weights),
+                                           temperature, dloss.data_ptr(), stash.data_ptr(), out.data_ptr(), V), None)
+    return out
+
+
+def distill_loss_grad(logits, values, ids, rest=None, temperature=1.0, weights=None):
+    """Row losses of loss.distillation_loss and d sum(losses) / d logits in one call (`weights` carries every factor of the
+    final loss, a mean's 1/n too): for updates scheduled by hand.  Returns (loss fp32 [...], dlogits in the logits' type)."""
+    dt, T, V, ld, k, values, ids, rest, weights, temperature = _distill_args(logits, values, ids, rest, weights, temperature)
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if T:
+        _launch(logits, "pg_distill_loss_grad",
+                (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest), ptr(weights), temperature,
+                 loss.data_ptr(), out.data_ptr(), V), lib.pg_distill_workspace_bytes(dt, T, V, k))
+    return loss, out
+
+
 def commit_topk(ids, pred, conf, keep_percent: float, fill_all: bool, mask_id=4, pad_id=0, cls_id=2, sep_id=3,
                 counts=None):
     B, S = ids.shape
