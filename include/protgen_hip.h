@@ -323,7 +323,8 @@ int pg_commit_topk(int64_t* ids, const int64_t* pred, const float* conf, int B, 
 /* ------------------------------------------------------------------ operators over rows of logits of any vocabulary
  * logits: T rows of V <= 2^24 entries (dtype PG_F32 or PG_BF16), row t at logits + t*ld elements; any alignment of the element
  * type.  Entries of a row are ordered by value, ties by the lower index; NaN counts as -inf, -0 as +0.  Workspaces: the
- * *_workspace_bytes functions (may be 0; then NULL will do); a workspace serves one call at a time.
+ * *_workspace_bytes functions (may be 0; then NULL will do); a workspace is 16-byte aligned and serves one
+ * call at a time.
  *
  * pg_top_logits: a teacher's record of each row, for pg_distill_*: the first k <= min(V, 1024) entries (values [T][k] in the
  * activation type, ids [T][k], in order) and rest[t] = log sum over the other entries of exp(x / temperature) (-inf if there is
@@ -349,7 +350,7 @@ int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* n
  *   loss[t] = weight temperature^2 [ sum_e t_e log(t_e / s_id(e)) + t_rest log(t_rest / s_rest) ].
  * An id that occurs twice counts as two entries and once in the set that s_rest leaves out.  weights [T] (NULL = 1): a row with
  * weight 0 is not read and gives loss 0 and gradient 0, and so does a row with no entry or with no logit above -inf.
- * pg_distill_fwd leaves pg_distill_stash_floats() floats per row for pg_distill_bwd, which writes
+ * pg_distill_fwd leaves pg_distill_stash_floats() floats per row (16-byte aligned) for pg_distill_bwd, which writes
  * dlogits = dloss[t] d loss[t] / d logits (activation type, every entry of every row; dloss NULL = 1);
  * pg_distill_loss_grad is both in one call, for updates that know the weights beforehand. */
 int64_t pg_distill_stash_floats(void);

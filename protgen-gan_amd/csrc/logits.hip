@@ -222,22 +222,37 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, i
 }
 
 // ------------------------------------------------------------------ sampling
+struct RowFilter {
+  float temperature, top_p, min_p;
+  int top_k;
+  // w >= min_p, as x >= max + temperature ln(min_p): no exponential's rounding decides it
+  __device__ __forceinline__ bool above_min_p(float x, float m) const {
+    if (!(min_p > 0.f) || x == m) return true;
+    return min_p < 1.f && (double)x >= (double)m + (double)temperature * log((double)min_p);
+  }
+};
+struct SampleArgs {
+  float temperature, top_p, min_p;
+  int top_k;
+  const float* temps; const int32_t* ks; const float* ps; const float* mins;
+  __device__ __forceinline__ RowFilter row(int64_t t) const {
+    return {temps ? temps[t] : temperature, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
+  }
+};
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld,
                                                              const float* __restrict__ noise, int64_t ld_noise, int V,
-                                                             float temperature, int top_k, float top_p, float min_p,
-                                                             const float* __restrict__ temps, const int32_t* __restrict__ ks,
-                                                             const float* __restrict__ ps, const float* __restrict__ mins,
-                                                             int64_t* __restrict__ pred, float* __restrict__ conf) {
+                                                             SampleArgs args, int64_t* __restrict__ pred,
+                                                             float* __restrict__ conf) {
   __shared__ SelLds sel;
   __shared__ double redd[16];
   __shared__ uint64_t redk[16];
   const int64_t t = blockIdx.x;
   const T* row = logits + t * ld;
   const float* q = noise + t * ld_noise;
-  const float temp = temps ? temps[t] : temperature;
-  int k = ks ? ks[t] : top_k;
-  const float p = ps ? ps[t] : top_p, least = mins ? mins[t] : min_p;
+  const RowFilter f = args.row(t);
+  const float temp = f.temperature, p = f.top_p;
+  const int k = f.top_k;
   uint64_t kmax = 0;
   each<T, NT>(row, V, [&](int i, float x) { const uint64_t e = entry_key(x, i); kmax = e > kmax ? e : kmax; });
   kmax = block_all<NT>(kmax, redk, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
@@ -261,11 +276,10 @@ __global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict
     const double want = ceil((double)p * mass);
     B = select_key<T, NT, true>(row, V, B, want < 1.0 ? 1 : (uint64_t)want, weight, sel);
   }
-  const double floor_x = least > 0.f ? (double)m + (double)temp * log(least < 1.f ? (double)least : 1.0) : -INFINITY;
   double best = -1.0, total = 0.0;
   uint64_t at = ~0ull;
   each<T, NT>(row, V, [&](int i, float x) {
-    if (entry_key(x, i) < B || !(x > -INFINITY) || !((double)x >= floor_x || x == m)) return;
+    if (entry_key(x, i) < B || !(x > -INFINITY) || !f.above_min_p(x, m)) return;
     const double w = weight(x);
     total += w;
     const double r = w > 0.0 ? w / (double)q[i] : 0.0;
@@ -413,6 +427,219 @@ __global__ __launch_bounds__(NT) void distill_bwd_kernel(const T* __restrict__ l
   }
 }
 
+
+// ------------------------------------------------------------------ vocabularies of at most 64 entries: G lanes a row
+// One lane per entry, G = 32 (two rows a wave) or 64.  The fill loop's 30-entry rows are 120 bytes: a workgroup per row costs
+// 5.5 ms at 32768 rows where one lane per entry takes some microseconds.  An entry's rank is the count of the entries
+// before it, read from LDS four at a time; sums run over the G lanes by DPP, in one fixed order.
+template <int G> struct Group {
+  template <int CTRL> static __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+  template <int STEP> static __device__ __forceinline__ int other(int v) {
+    if constexpr (STEP == 0) return dpp<0xB1>(v);   // lane ^ 1
+    if constexpr (STEP == 1) return dpp<0x4E>(v);   // lane ^ 2
+    if constexpr (STEP == 2) return dpp<0x141>(v);  // mirrored in 8: the other four
+    if constexpr (STEP == 3) return dpp<0x140>(v);  // mirrored in 16: the other eight
+    if constexpr (STEP == 4) return __builtin_amdgcn_ds_swizzle(v, 0x401F);  // lane ^ 16
+    if constexpr (STEP == 5) return __shfl_xor(v, 32, 64);
+  }
+  template <int STEP> static __device__ __forceinline__ float other(float v) { return __int_as_float(other<STEP>(__float_as_int(v))); }
+  template <int STEP> static __device__ __forceinline__ double other(double v) {
+    return __hiloint2double(other<STEP>(__double2hiint(v)), other<STEP>(__double2loint(v)));
+  }
+  template <typename T, typename Op> static __device__ __forceinline__ T all(T v, Op op) {
+    v = op(v, other<0>(v)); v = op(v, other<1>(v)); v = op(v, other<2>(v)); v = op(v, other<3>(v)); v = op(v, other<4>(v));
+    if constexpr (G == 64) v = op(v, other<5>(v));
+    return v;
+  }
+  static __device__ __forceinline__ float max(float v) { return all(v, [](float a, float b) { return fmaxf(a, b); }); }
+  static __device__ __forceinline__ int min(int v) { return all(v, [](int a, int b) { return a < b ? a : b; }); }
+  template <typename T> static __device__ __forceinline__ T sum(T v) { return all(v, [](T a, T b) { return a + b; }); }
+};
+
+// f(entry u's key, u) for the row's entries, keys in LDS (G per row, those past V zero: behind every entry)
+template <int G, typename F> __device__ __forceinline__ void each_key(const uint32_t* keys, int V, F f) {
+  for (int u = 0; u < V; u += 4) {
+    const uint4 k = *reinterpret_cast<const uint4*>(keys + u);
+    f(k.x, u); f(k.y, u + 1); f(k.z, u + 2); f(k.w, u + 3);
+  }
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ logits, int64_t ld, int rows, int V, int K, float tau,
+                                                        T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest) {
+  __shared__ __align__(16) uint32_t keys[256];
+  const int v = threadIdx.x & (G - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, t = t0 < rows ? t0 : rows - 1;
+  const float c = (float)(LOG2E / (double)tau);
+  const uint32_t key = v < V ? value_key(to_f32<T>(logits[t * ld + v])) : 0;
+  keys[threadIdx.x] = key;
+  __syncthreads();
+  int rank = 0;
+  each_key<G>(keys + (threadIdx.x & ~(G - 1)), V, [&](uint32_t k, int u) { rank += k > key || (k == key && u < v); });
+  const float x = key_value(key);
+  const bool left = v < V && rank >= K;
+  const float m = Group<G>::max(left ? x : -INFINITY);
+  const float sum = Group<G>::sum(left && x > -INFINITY ? __builtin_amdgcn_exp2f((x - m) * c) : 0.f);
+  if (t0 >= rows) return;
+  if (v < V && rank < K) {
+    values[t * K + rank] = from_f32<T>(x);
+    ids[t * K + rank] = v;
+  }
+  if (v == 0) rest[t] = m == -INFINITY || m == INFINITY ? m : (float)((double)m / tau + log((double)sum));
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
+                                                           int64_t ld_noise, int rows, int V, SampleArgs a,
+                                                           int64_t* __restrict__ pred, float* __restrict__ conf) {
+  __shared__ __align__(16) uint32_t keys[256];
+  __shared__ __align__(16) double weights[256];
+  const int v = threadIdx.x & (G - 1), first = threadIdx.x & ~(G - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, t = t0 < rows ? t0 : rows - 1;
+  const RowFilter f = a.row(t);
+  const uint32_t key = v < V ? value_key(to_f32<T>(logits[t * ld + v])) : 0;
+  const float q = v < V ? noise[t * ld_noise + v] : 1.f;
+  const float x = v < V ? key_value(key) : -INFINITY;
+  const float m = Group<G>::max(x);
+  const bool greedy = !(f.temperature > 0.f);
+  double w = 0.0;
+  if (v < V) w = x == m ? 1.0 : greedy ? 0.0 : exp2_f64(((double)x - (double)m) * (LOG2E / (double)f.temperature));
+  keys[threadIdx.x] = key;
+  weights[threadIdx.x] = w;
+  __syncthreads();
+  bool keep = v < V && x > -INFINITY && f.above_min_p(x, m);
+  if (f.top_p < 1.f) {
+    int rank = 0;
+    double before = 0.0;
+    const double* ws = weights + first;
+    each_key<G>(keys + first, V, [&](uint32_t k, int u) {
+      const bool b = k > key || (k == key && u < v);
+      rank += b;
+      before += b ? ws[u] : 0.0;
+    });
+    const bool in_k = f.top_k <= 0 || rank < f.top_k;
+    const double mass = Group<G>::sum(in_k ? w : 0.0);
+    keep = keep && in_k && (rank == 0 || before < (double)f.top_p * mass);
+  } else if (f.top_k > 0 && f.top_k < V) {
+    int rank = 0;
+    each_key<G>(keys + first, V, [&](uint32_t k, int u) { rank += k > key || (k == key && u < v); });
+    keep = keep && rank < f.top_k;
+  }
+  if (greedy) keep = keep && x == m;
+  const double total = Group<G>::sum(keep ? w : 0.0);
+  // the race: in fp32 (relative error below 2^-21) to find who can win, in 64 bits where more than one can
+  const float r = keep ? ((float)w > 0.f ? (float)w / q : 0.f) : -1.f;
+  const float top = Group<G>::max(greedy ? (keep ? 1.f : -1.f) : r);
+  bool win = keep && (greedy || r >= top * (1.f - 0x1p-18f));
+  const uint64_t ballot = __ballot(win), mine = G == 64 ? ballot : (threadIdx.x & 32) ? ballot >> 32 : ballot & 0xffffffffu;
+  if (!greedy && __popcll(mine) > 1) {
+    const double e = win ? (w > 0.0 ? w / (double)q : 0.0) : -1.0;
+    const double best = Group<G>::all(e, [](double p, double s) { return p > s ? p : s; });
+    win = win && e == best;
+  }
+  int at = Group<G>::min(win ? v : G);
+  if (at == G) at = Group<G>::min(keep && x == m ? v : G);  // (noise without a usable draw)
+  if (t0 >= rows) return;
+  if (m == -INFINITY) {
+    if (v == 0) pred[t] = -1, conf[t] = 0.f;
+  } else if (v == at) {
+    pred[t] = v;
+    conf[t] = greedy ? 1.f : (float)(w / total);
+  }
+}
+
+// Distillation, V and K <= G: the row, its entries and every sum in one group's registers; an entry's teacher probability reaches
+// its token's lane through LDS, added up over the list in order (an id that occurs twice adds twice).
+// LOSS: forward (loss, stash); GRAD: the gradient, from this pass's own numbers (LOSS) or from the stash.
+template <typename T, int G, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict__ logits, int64_t ld, int rows, int V, DistillArgs a,
+                                                            float* __restrict__ loss, float* __restrict__ stash,
+                                                            const float* __restrict__ upstream, T* __restrict__ grad,
+                                                            int64_t ld_grad) {
+  __shared__ float xs[256];
+  __shared__ __align__(16) int list_id[256];
+  __shared__ __align__(16) float list_p[256];
+  const int v = threadIdx.x & (G - 1), first = threadIdx.x & ~(G - 1);
+  const int64_t t0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, t = t0 < rows ? t0 : rows - 1;
+  const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
+  const float w = a.weights ? a.weights[t] : 1.f;
+  const bool on = w != 0.f;  // (a row of weight 0 is not read)
+  const float x = on && v < V ? to_f32<T>(logits[t * ld + v]) : -INFINITY;
+  int id = -1;
+  float val = -INFINITY;
+  if (on && v < a.K) {
+    id = a.ids[t * a.K + v];
+    val = to_f32<T>(((const T*)a.values)[t * a.K + v]);
+  }
+  const bool entry = (uint32_t)id < (uint32_t)V && val > -INFINITY;
+  float all_m, all_s, o_m, coef, te_m, te_inv, p, live;
+  xs[threadIdx.x] = x;
+  list_id[threadIdx.x] = entry ? id : -1;
+  if (LOSS) {
+    __syncthreads();
+    bool member = false;
+    for (int e = 0; e < a.K; ++e) member = member || list_id[first + e] == v;
+    const bool tail = a.rest != nullptr;
+    all_m = Group<G>::max(v < V ? x : -INFINITY);  // (NaN and +inf reach the sums)
+    all_m = all_m == -INFINITY ? 0.f : all_m;
+    const bool out = v < V && !(tail && member);
+    o_m = Group<G>::max(out ? x : -INFINITY);
+    o_m = o_m == -INFINITY ? 0.f : o_m;
+    const float o_s = Group<G>::sum(out ? __builtin_amdgcn_exp2f((x - o_m) * c) : 0.f);
+    const float in_s = Group<G>::sum(tail && member && v < V ? __builtin_amdgcn_exp2f((x - all_m) * c) : 0.f);
+    const float o_all = o_s * __builtin_amdgcn_exp2f((o_m - all_m) * c);
+    all_s = (o_s == 0.f ? 0.f : o_all) + in_s;
+    float rest = tail ? a.rest[t] : -INFINITY;
+    const bool has_rest = on && rest > -INFINITY;
+    te_m = Group<G>::max(entry ? val : -INFINITY);
+    const bool entries = te_m > -INFINITY;
+    const float rest_x = rest * a.tau;
+    if (has_rest) te_m = fmaxf(te_m, rest_x);
+    if (te_m == -INFINITY) te_m = 0.f;
+    float te_s = Group<G>::sum(entry ? __builtin_amdgcn_exp2f((val - te_m) * c) : 0.f);
+    const float rest_e = has_rest ? __builtin_amdgcn_exp2f((rest_x - te_m) * c) : 0.f;
+    te_s += rest_e;
+    const bool counts = entries && all_s != 0.f;  // (NaN counts)
+    te_inv = 1.f / te_s;
+    const float tr = rest_e * te_inv, log_all = logf(all_s), log_te = logf(te_s);
+    p = entry ? __builtin_amdgcn_exp2f((val - te_m) * c) * te_inv : 0.f;
+    float part = 0.f;
+    if (p > 0.f) part = p * (((val - te_m) - (xs[first + id] - all_m)) * inv_tau + (log_all - log_te));
+    part = Group<G>::sum(part);
+    if (tr > 0.f) part += tr * (((rest_x - te_m) * inv_tau - log_te) - ((o_m - all_m) * inv_tau + logf(o_s) - log_all));
+    coef = o_s != 0.f ? ((tail ? o_all / all_s : 1.f) - tr) / o_s : 0.f;
+    live = counts ? 1.f : 0.f;
+    if (v == 0 && t0 < rows) {
+      loss[t] = counts ? w * a.tau * a.tau * part : 0.f;
+      if (!GRAD) {
+        float* st = stash + t * STASH;
+        *reinterpret_cast<float4*>(st) = make_float4(all_m, counts ? 1.f / all_s : 0.f, o_m, counts ? coef : 0.f);
+        *reinterpret_cast<float4*>(st + 4) = make_float4(te_m, counts ? te_inv : 0.f, live, 0.f);
+      }
+    }
+    all_s = 1.f / all_s;
+  } else {
+    const float4 s0 = *reinterpret_cast<const float4*>(stash + t * STASH), s1 = *reinterpret_cast<const float4*>(stash + t * STASH + 4);
+    all_m = s0.x; all_s = s0.y; o_m = s0.z; coef = s0.w; te_m = s1.x; te_inv = s1.y; live = s1.z;
+    p = entry ? __builtin_amdgcn_exp2f((val - te_m) * c) * te_inv : 0.f;
+  }
+  if (!GRAD) return;
+  list_p[threadIdx.x] = p;
+  __syncthreads();
+  bool member = false;
+  float tv = 0.f;
+  for (int e = 0; e < a.K; ++e) {
+    const bool hit = list_id[first + e] == v;
+    member = member || hit;
+    tv += hit ? list_p[first + e] : 0.f;
+  }
+  const float f = w * a.tau * (upstream ? upstream[t] : 1.f);
+  float g = member ? __builtin_amdgcn_exp2f((x - all_m) * c) * all_s - tv : __builtin_amdgcn_exp2f((x - o_m) * c) * coef;
+  if (live == 0.f) g = 0.f;
+  else g *= f;
+  if (t0 < rows && v < V) grad[t * ld_grad + v] = from_f32<T>(g);
+}
+
 int check_launch() { return hipGetLastError() == hipSuccess ? PG_OK : PG_ERR_LAUNCH; }
 
 int check_rows(int dtype, const void* logits, int64_t ld, int T, int V) {
@@ -428,11 +655,66 @@ int check_distill(int dtype, const void* logits, int64_t ld, int T, int V, const
 }
 
 template <typename T>
+int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, int32_t* ids, float* rest, hipStream_t s) {
+  if (V <= 32)
+    hipLaunchKernelGGL((top_small_kernel<T, 32>), dim3((n + 7) / 8), dim3(256), 0, s, x, ld, n, V, k, tau, values, ids, rest);
+  else if (V <= 64)
+    hipLaunchKernelGGL((top_small_kernel<T, 64>), dim3((n + 3) / 4), dim3(256), 0, s, x, ld, n, V, k, tau, values, ids, rest);
+  else
+    hipLaunchKernelGGL((top_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, V, k, tau, values, ids, rest);
+  return check_launch();
+}
+
+template <typename T>
+int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int V, const SampleArgs& a, int64_t* pred, float* conf,
+                hipStream_t s) {
+  if (V <= 32)
+    hipLaunchKernelGGL((sample_small_kernel<T, 32>), dim3((n + 7) / 8), dim3(256), 0, s, x, ld, q, ldq, n, V, a, pred, conf);
+  else if (V <= 64)
+    hipLaunchKernelGGL((sample_small_kernel<T, 64>), dim3((n + 3) / 4), dim3(256), 0, s, x, ld, q, ldq, n, V, a, pred, conf);
+  else
+    hipLaunchKernelGGL((sample_filtered_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, q, ldq, V, a, pred, conf);
+  return check_launch();
+}
+
+template <typename T, bool LOSS, bool GRAD>
+int distill_small(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, float* stash, const float* up, T* grad,
+                  int64_t ldg, hipStream_t s) {
+  if (V <= 32 && a.K <= 32)
+    hipLaunchKernelGGL((distill_small_kernel<T, 32, LOSS, GRAD>), dim3((n + 7) / 8), dim3(256), 0, s, x, ld, n, V, a, loss, stash,
+                       up, grad, ldg);
+  else
+    hipLaunchKernelGGL((distill_small_kernel<T, 64, LOSS, GRAD>), dim3((n + 3) / 4), dim3(256), 0, s, x, ld, n, V, a, loss, stash,
+                       up, grad, ldg);
+  return check_launch();
+}
+bool small_rows(int V, int k) { return V <= 64 && k <= 64; }
+
+template <typename T>
 int distill_forward(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, float* stash, hipStream_t s) {
+  if (small_rows(V, a.K))
+    return distill_small<T, true, false>(x, ld, n, V, a, loss, stash, nullptr, nullptr, 0, s);
   const size_t lds = a.rest ? (size_t)((V + 31) / 32) * 4 : 0;
   if (lds > 128 * 1024) return PG_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, stash);
   return check_launch();
+}
+
+template <typename T>
+int distill_backward(const T* x, int64_t ld, int n, int V, const DistillArgs& a, const float* up, const float* stash, T* grad,
+                     int64_t ldg, hipStream_t s) {
+  if (small_rows(V, a.K))
+    return distill_small<T, false, true>(x, ld, n, V, a, nullptr, const_cast<float*>(stash), up, grad, ldg, s);
+  hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, V, a, up, stash, grad, ldg);
+  return check_launch();
+}
+
+template <typename T>
+int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, T* grad, int64_t ldg, float* stash,
+                 hipStream_t s) {
+  if (small_rows(V, a.K)) return distill_small<T, true, true>(x, ld, n, V, a, loss, nullptr, nullptr, grad, ldg, s);
+  const int rc = distill_forward(x, ld, n, V, a, loss, stash, s);
+  return rc != PG_OK ? rc : distill_backward(x, ld, n, V, a, nullptr, stash, grad, ldg, s);
 }
 
 }  // namespace
@@ -445,14 +727,8 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
   if (rc != PG_OK) return rc;
   if (!values || !ids || !rest || k <= 0 || k > V || !(temperature > 0.f) || !(temperature <= FLT_MAX)) return PG_ERR_ARG;
   if (k > MAX_K) return PG_ERR_UNSUPPORTED;
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == PG_F32)
-    hipLaunchKernelGGL((top_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, V, k, temperature,
-                       (float*)values, ids, rest);
-  else
-    hipLaunchKernelGGL((top_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, V, k, temperature,
-                       (bf16_t*)values, ids, rest);
-  return check_launch();
+  return dtype == PG_F32 ? top_rows((const float*)logits, ld, T, V, k, temperature, (float*)values, ids, rest, (hipStream_t)stream)
+                         : top_rows((const bf16_t*)logits, ld, T, V, k, temperature, (bf16_t*)values, ids, rest, (hipStream_t)stream);
 }
 
 extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V) { return 0; }
@@ -467,14 +743,9 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
   if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
       (!mins && !(min_p >= 0.f && min_p <= 1.f)))
     return PG_ERR_ARG;
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == PG_F32)
-    hipLaunchKernelGGL((sample_filtered_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, noise, ld_noise,
-                       V, temperature, top_k, top_p, min_p, temps, ks, ps, mins, pred, conf);
-  else
-    hipLaunchKernelGGL((sample_filtered_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, noise,
-                       ld_noise, V, temperature, top_k, top_p, min_p, temps, ks, ps, mins, pred, conf);
-  return check_launch();
+  const SampleArgs a = {temperature, top_p, min_p, top_k, temps, ks, ps, mins};
+  return dtype == PG_F32 ? sample_rows((const float*)logits, ld, noise, ld_noise, T, V, a, pred, conf, (hipStream_t)stream)
+                         : sample_rows((const bf16_t*)logits, ld, noise, ld_noise, T, V, a, pred, conf, (hipStream_t)stream);
 }
 
 extern "C" int64_t pg_distill_stash_floats(void) { return STASH; }
@@ -486,6 +757,7 @@ extern "C" int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, 
   const int rc = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
   if (rc != PG_OK) return rc;
   if (!loss || !stash) return PG_ERR_ARG;
+  if ((uintptr_t)stash & 15) return PG_ERR_ALIGN;
   const DistillArgs a = {values, ids, rest, weights, k, temperature};
   hipStream_t s = (hipStream_t)stream;
   return dtype == PG_F32 ? distill_forward((const float*)logits, ld, T, V, a, loss, stash, s)
@@ -498,15 +770,12 @@ extern "C" int pg_distill_bwd(int dtype, const void* logits, int64_t ld, int T, 
   const int rc = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
   if (rc != PG_OK) return rc;
   if (!stash || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
+  if ((uintptr_t)stash & 15) return PG_ERR_ALIGN;
   const DistillArgs a = {values, ids, nullptr, weights, k, temperature};
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PG_F32)
-    hipLaunchKernelGGL((distill_bwd_kernel<float, 256>), dim3(T), dim3(256), 0, s, (const float*)logits, ld, V, a, dloss, stash,
-                       (float*)dlogits, ld_dlogits);
-  else
-    hipLaunchKernelGGL((distill_bwd_kernel<bf16_t, 256>), dim3(T), dim3(256), 0, s, (const bf16_t*)logits, ld, V, a, dloss, stash,
-                       (bf16_t*)dlogits, ld_dlogits);
-  return check_launch();
+  return dtype == PG_F32
+             ? distill_backward((const float*)logits, ld, T, V, a, dloss, stash, (float*)dlogits, ld_dlogits, s)
+             : distill_backward((const bf16_t*)logits, ld, T, V, a, dloss, stash, (bf16_t*)dlogits, ld_dlogits, s);
 }
 
 extern "C" int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, int T, int V, const void* values,
@@ -517,8 +786,10 @@ extern "C" int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, i
   if (bad != PG_OK) return bad;
   if (!loss || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
   if (!workspace || workspace_bytes < pg_distill_workspace_bytes(dtype, T, V, k)) return PG_ERR_WORKSPACE;
-  float* stash = (float*)workspace;
-  const int rc = pg_distill_fwd(dtype, logits, ld, T, V, values, ids, k, rest, weights, temperature, loss, stash, nullptr, 0, stream);
-  if (rc != PG_OK) return rc;
-  return pg_distill_bwd(dtype, logits, ld, T, V, values, ids, k, weights, temperature, nullptr, stash, dlogits, ld_dlogits, stream);
+  if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
+  const DistillArgs a = {values, ids, rest, weights, k, temperature};
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == PG_F32
+             ? distill_both((const float*)logits, ld, T, V, a, loss, (float*)dlogits, ld_dlogits, (float*)workspace, s)
+             : distill_both((const bf16_t*)logits, ld, T, V, a, loss, (bf16_t*)dlogits, ld_dlogits, (float*)workspace, s);
 }

@@ -270,6 +270,17 @@ def test_distill_odd_rows(pg, dtype, tail, V):
     check_distill(pg, x, v.to(DEV), i.to(DEV), r.to(DEV) if tail else None, 1.5, w.to(DEV))
 
 
+@pytest.mark.parametrize("V,k", [(5, 20), (30, 33), (30, 64), (30, 200), (64, 65), (70, 1024)])
+def test_distill_more_entries_than_tokens(pg, V, k):
+    """Records longer than the vocabulary: most entries absent or repeated."""
+    T = 9
+    g = torch.Generator().manual_seed(k)
+    x, v = rows(T, V, torch.float32, k), torch.randn(T, k, generator=g)
+    i = torch.randint(-2 * V, 2 * V, (T, k), generator=g).to(torch.int32)
+    check_distill(pg, x, v.to(DEV), i.to(DEV), torch.randn(T, generator=g).to(DEV), 1.0, None)
+    check_distill(pg, x, v.to(DEV), i.to(DEV), None, 1.0, None)
+
+
 def test_distill_rest_without_a_token(pg):
     """The teacher leaves mass to tokens the student's vocabulary does not have left: infinite loss, finite gradient."""
     x, v, i, r = record(pg, 4, 9, 9, torch.float32, 3, 1.0, True)

@@ -101,6 +101,7 @@ def test_c_abi_refusals(pg):
 
     def bwd(stash=p, out=p, ldo=8):
         return lib.pg_distill_bwd(0, p, 8, 2, 8, p, p, 3, None, 1.0, None, stash, out, ldo, None)
+    assert fwd(stash=p + 4) == -2 and bwd(stash=p + 4) == -2
     assert bwd(stash=None) == ARG and bwd(out=None) == ARG and bwd(ldo=7) == ARG
 
     def both(ws=p, n=0, ldo=8):
