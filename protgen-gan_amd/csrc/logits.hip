@@ -221,6 +221,333 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, i
     rest[t] = top_rest == INFINITY ? INFINITY : es.s > 0.f ? (float)((double)es.m / tau + log((double)es.s)) : -INFINITY;
 }
 
+// ------------------------------------------------------------------ the largest entries of a segment of a row, kept in registers
+// A row is cut into segments of NT * VPT 16-byte vectors; a workgroup loads one whole segment into registers (all its loads in
+// flight at once) and reads it once.  Each thread's vectors form four groups; the K-th largest of the NT * 4 group maxima is a
+// lower bound of the segment's K-th largest entry and not far below it (64 of 1024 maxima leave about 70 entries above the
+// bound), found by eight rounds of counting on the upper 16 bits of their keys.  Vectors with an entry above the bound go to
+// LDS, everything else into the sum of exponentials.  Where too many entries tie at the bound, the exact K-th key is found by
+// bisection over the segment instead.
+constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
+constexpr int MAX_SEG_K = 512;
+constexpr int MAX_CAP(int nt) { return nt == 64 ? 512 : 1088; }  // keys a segment may leave
+
+__device__ __forceinline__ void unpack(uint4 d, float (&o)[4]) {
+  o[0] = __uint_as_float(d.x); o[1] = __uint_as_float(d.y); o[2] = __uint_as_float(d.z); o[3] = __uint_as_float(d.w);
+}
+__device__ __forceinline__ void unpack(uint4 d, float (&o)[8]) {
+  o[0] = __uint_as_float(d.x << 16); o[1] = __uint_as_float(d.x & 0xffff0000u);
+  o[2] = __uint_as_float(d.y << 16); o[3] = __uint_as_float(d.y & 0xffff0000u);
+  o[4] = __uint_as_float(d.z << 16); o[5] = __uint_as_float(d.z & 0xffff0000u);
+  o[6] = __uint_as_float(d.w << 16); o[7] = __uint_as_float(d.w & 0xffff0000u);
+}
+template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E]) {  // (NaN: passed over)
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; ++e) m = fmaxf(m, o[e]);
+  return m;
+}
+// The exponentials of E entries of which vm is the largest, NaN as -inf, with one rescaling for all of them.
+template <int E> __device__ __forceinline__ void exp_sum_vec(ExpSum& a, const float (&o)[E], float vm, float c) {
+  const float m = fmaxf(a.m, vm);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((fmaxf(o[e], -INFINITY) - m) * c);
+  a.s = a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + s;
+  a.m = m;
+}
+__device__ __forceinline__ void exp_sum_one(ExpSum& a, float x, float c) {
+  const float o[1] = {x};
+  exp_sum_vec<1>(a, o, fmaxf(x, -INFINITY), c);
+}
+
+template <int NT> struct SegLds {
+  static constexpr int STAGE = NT == 64 ? 256 : 512;  // vectors that may hold an entry above the bound
+  static constexpr int LIST = NT == 64 ? 512 : 2048;  // keys (a power of two of at least MAX_CAP)
+  uint64_t list[LIST];
+  uint4 vec[STAGE];
+  int at[STAGE];
+  uint32_t n_vec, n;
+  int wave_count[2][3 * 16];
+  float red[16];
+};
+struct SegHead {      // what a segment leaves for the merge
+  uint64_t level;     // every entry of the segment with at least this key is in its list
+  float m, s;         // the sum over its other entries
+  uint32_t n, pad[3];
+};
+
+template <typename T, int NT, int VPT> struct Segment {
+  static constexpr int E = 16 / (int)sizeof(T), VECS = NT * VPT;
+  uint4 d[VPT];
+  float ends[2];     // this thread's entry of those before the first / behind the last whole vector
+  int end_at[2];     // their indexes, -1: none
+  int base, nv;
+
+  __device__ __forceinline__ int index(int j) const { return base + (j * NT + (int)threadIdx.x) * E; }
+  __device__ __forceinline__ bool has(int j) const { return j * NT + (int)threadIdx.x < nv; }
+  __device__ __forceinline__ void load(const T* row, int V, int seg, int nseg) {
+    int head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
+    if (head > V) head = V;
+    const int all = (V - head) / E, tail = head + all * E;
+    base = head + seg * VECS * E;
+    nv = all - seg * VECS;
+    nv = nv < 0 ? 0 : nv > VECS ? VECS : nv;
+    const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      d[j] = make_uint4(none, none, none, none);
+      if (has(j)) d[j] = *reinterpret_cast<const uint4*>(row + index(j));
+    }
+    end_at[0] = seg == 0 && (int)threadIdx.x < head ? (int)threadIdx.x : -1;
+    end_at[1] = seg == nseg - 1 && (int)threadIdx.x < V - tail ? tail + (int)threadIdx.x : -1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ends[i] = end_at[i] >= 0 ? to_f32<T>(row[end_at[i]]) : -INFINITY;
+  }
+  // Unpacked anew in every phase: kept from one to the next, the fp32 values of a bf16 segment would not fit the registers.
+  __device__ __forceinline__ void fresh() {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) asm volatile("" : "+v"(d[j].x), "+v"(d[j].y), "+v"(d[j].z), "+v"(d[j].w));
+  }
+  // f(value, index) over this thread's entries, read again from memory (a loop over the registers would have to be unrolled)
+  template <typename F> __device__ __forceinline__ void entries(const T* row, F f) const {
+#pragma unroll 1
+    for (int j = 0; j < VPT && has(j); ++j) {
+      float o[E];
+      unpack(*reinterpret_cast<const uint4*>(row + index(j)), o);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(o[e], index(j) + e);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (end_at[i] >= 0) f(ends[i], end_at[i]);
+  }
+};
+
+// Leaves the keys of the segment's largest entries in list (n of them, at most cap, in no order; at least K if it has as many),
+// the sum over its other entries in rest (per thread), and the level.  FINITE: entries of -inf are never listed.
+template <typename T, int NT, int VPT, bool FINITE>
+__device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, int K, int cap, float c, SegLds<NT>& l, uint64_t& level,
+                                       ExpSum& rest) {
+  constexpr int E = Segment<T, NT, VPT>::E, NW = NT / 64, STAGE = SegLds<NT>::STAGE, LIST = SegLds<NT>::LIST;
+  uint64_t* list = l.list;
+  float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    float o[E];
+    unpack(sg.d[j], o);
+    gm[j & 3] = fmaxf(gm[j & 3], vec_max<E>(o));
+  }
+  gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
+  uint32_t mk[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
+  if (threadIdx.x == 0) l.n_vec = 0, l.n = 0;
+  uint32_t bound = 0;
+  for (int b = 30; b >= 16; b -= 2) {  // two bits a round
+    int cnt[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint32_t trial = bound | ((uint32_t)(i + 1) << b);
+      cnt[i] = 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) cnt[i] += __popcll(__ballot(mk[g] >= trial));
+    }
+    if (NW > 1) {
+      int* w = l.wave_count[(b >> 1) & 1];
+      if ((threadIdx.x & 63) < 3) w[(threadIdx.x >> 6) * 3 + (threadIdx.x & 63)] = (threadIdx.x & 63) == 0 ? cnt[0] : (threadIdx.x & 63) == 1 ? cnt[1] : cnt[2];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        cnt[i] = 0;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) cnt[i] += w[k * 3 + i];
+      }
+    }
+    bound |= (cnt[2] >= K ? 3u : cnt[1] >= K ? 2u : cnt[0] >= K ? 1u : 0u) << b;
+  }
+  const float thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
+  rest = {-FLT_MAX, 0.f};
+  __syncthreads();
+  sg.fresh();
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    float o[E];
+    unpack(sg.d[j], o);
+    const float vm = vec_max<E>(o);
+    if (vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j)) {
+      const uint32_t p = atomicAdd(&l.n_vec, 1u);
+      if (p < STAGE) {
+        l.vec[p] = sg.d[j];
+        l.at[p] = sg.index(j);
+      }
+    } else {
+      exp_sum_vec<E>(rest, o, vm, c);
+    }
+  }
+  auto take = [&](float x, int i) {
+    x = fmaxf(x, -INFINITY);
+    if (x >= thr && (!FINITE || x > -INFINITY)) {
+      const uint32_t p = atomicAdd(&l.n, 1u);
+      if (p < LIST) list[p] = entry_key(x, i);
+    } else {
+      exp_sum_one(rest, x, c);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (sg.end_at[i] >= 0) take(sg.ends[i], sg.end_at[i]);
+  __syncthreads();
+  const int n_vec = l.n_vec;
+  for (int i = threadIdx.x; i < (n_vec < STAGE ? n_vec : STAGE); i += NT) {
+    float o[E];
+    unpack(l.vec[i], o);
+#pragma unroll
+    for (int e = 0; e < E; ++e) take(o[e], l.at[i] + e);
+  }
+  __syncthreads();
+  int n = l.n;
+  level = thr > -INFINITY ? (uint64_t)value_key(thr) << 32 : 0;
+  if (n_vec > STAGE || n > cap) {  // too many at the bound: the K-th key itself, bit by bit
+    auto count = [&](auto in) {
+      int k = 0;
+      sg.entries(row, [&](float x, int i) { k += in(x, i); });
+      return block_all<NT>(k, reinterpret_cast<int*>(l.red), [](int a, int b) { return a + b; });
+    };
+    uint32_t vk = 0;
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t trial = vk | (1u << b);
+      if (count([&](float x, int) { return value_key(x) >= trial; }) >= K) vk = trial;
+    }
+    const int above = count([&](float x, int) { return value_key(x) > vk; });
+    uint32_t low = 0;  // of the entries at the K-th value, the K - above lowest indexes: the largest bound on ~index that keeps them
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t trial = low | (1u << b);
+      if (count([&](float x, int i) { return value_key(x) == vk && (uint32_t)~i >= trial; }) >= K - above) low = trial;
+    }
+    level = ((uint64_t)vk << 32) | low;
+    rest = {-FLT_MAX, 0.f};
+    __syncthreads();
+    if (threadIdx.x == 0) l.n = 0;
+    __syncthreads();
+    sg.entries(row, [&](float x, int i) {
+      const uint64_t k = entry_key(x, i);
+      if (k >= level && (!FINITE || x > -INFINITY)) list[atomicAdd(&l.n, 1u)] = k;
+      else exp_sum_one(rest, x, c);
+    });
+    __syncthreads();
+    n = l.n;
+  }
+  return n;
+}
+
+// list[0..n) in LDS, largest first; at least P = the next power of two of room
+template <int NT> __device__ __forceinline__ void sort_keys(uint64_t* list, int n) {
+  int P = 1;
+  while (P < n) P <<= 1;
+  for (int i = n + threadIdx.x; i < P; i += NT) list[i] = 0;
+  for (int size = 2; size <= P; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < P / 2; i += NT) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const uint64_t x = list[a], y = list[b];
+        if ((x < y) == ((a & size) == 0)) { list[a] = y; list[b] = x; }
+      }
+    }
+  __syncthreads();
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float tau, float c, ExpSum rest, float* red, T* values,
+                                           int32_t* ids, float* rest_out) {
+  sort_keys<NT>(list, n);
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float x = key_value((uint32_t)(list[i] >> 32));
+    if (i < K) {
+      values[i] = from_f32<T>(x);
+      ids[i] = (int32_t)~(uint32_t)list[i];
+    } else {
+      exp_sum_one(rest, x, c);
+    }
+  }
+  rest = block_exp_sum<NT>(rest, c, red);
+  if (threadIdx.x == 0)
+    *rest_out = rest.m == INFINITY ? INFINITY : rest.s > 0.f ? (float)((double)rest.m / tau + log((double)rest.s)) : -INFINITY;
+}
+
+template <typename T, int NT, int VPT>
+__global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
+                                                         T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest_out,
+                                                         SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
+  __shared__ SegLds<NT> l;
+  const int64_t t = blockIdx.x;
+  const int seg = blockIdx.y, nseg = gridDim.y;
+  const float c = (float)(LOG2E / (double)tau);
+  Segment<T, NT, VPT> sg;
+  const T* row = logits + t * ld;
+  sg.load(row, V, seg, nseg);
+  uint64_t level;
+  ExpSum rest;
+  const int n = collect<T, NT, VPT, false>(sg, row, K, cap, c, l, level, rest);
+  if (nseg == 1) {
+    top_finish<T, NT>(l.list, n, K, tau, c, rest, l.red, values + t * K, ids + t * K, rest_out + t);
+    return;
+  }
+  rest = block_exp_sum<NT>(rest, c, l.red);
+  const int64_t at = t * nseg + seg;
+  for (int i = threadIdx.x; i < n; i += NT) lists[at * cap + i] = l.list[i];
+  if (threadIdx.x == 0) heads[at] = {level, rest.m, rest.s, (uint32_t)n, {0, 0, 0}};
+}
+
+// All segments' keys of row t into list; returns their number, the sums in rest (one segment per thread), and the row's level.
+template <int NT>
+__device__ __forceinline__ int gather_segments(const SegHead* heads, const uint64_t* lists, int64_t t, int nseg, int cap, uint64_t* list,
+                                               ExpSum& rest, uint64_t& level) {
+  rest = {-FLT_MAX, 0.f};
+  level = 0;
+  int n = 0;
+  for (int s = 0; s < nseg; ++s) {
+    const SegHead h = heads[t * nseg + s];
+    if (s % NT == (int)threadIdx.x) rest = rest.s == 0.f ? ExpSum{h.m, h.s} : rest;
+    level = h.level > level ? h.level : level;
+    for (int i = threadIdx.x; i < (int)h.n; i += NT) list[n + i] = lists[(t * nseg + s) * cap + i];
+    n += h.n;
+  }
+  return n;
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void top_merge_kernel(int nseg, int K, int cap, float tau, T* __restrict__ values,
+                                                       int32_t* __restrict__ ids, float* __restrict__ rest_out,
+                                                       const SegHead* __restrict__ heads, const uint64_t* __restrict__ lists) {
+  __shared__ uint64_t list[MERGE];
+  __shared__ float red[16];
+  const int64_t t = blockIdx.x;
+  ExpSum rest;
+  uint64_t level;
+  const int n = gather_segments<NT>(heads, lists, t, nseg, cap, list, rest, level);
+  top_finish<T, NT>(list, n, K, tau, (float)(LOG2E / (double)tau), rest, red, values + t * K, ids + t * K, rest_out + t);
+}
+
+// How a call is cut: threads and vectors per thread of a segment, segments per row, keys a segment may leave.
+struct Cut { int nt, vpt, nseg, cap; };
+Cut cut_rows(int dtype, int T, int V, int K) {
+  if (K > MAX_SEG_K || V <= 64) return {0, 0, 0, 0};
+  const int vecs = V / (dtype == PG_F32 ? 4 : 8);
+  const int shapes[3][2] = {{64, 4}, {256, 4}, {256, 16}};
+  for (int i = K <= 128 ? 0 : 1; i < 3; ++i) {
+    const int per = shapes[i][0] * shapes[i][1], nseg = vecs <= per ? 1 : (vecs + per - 1) / per;
+    if (nseg > 1 && i < 2) {
+      // few rows: small segments, to spread them over the chip; many: the next larger ones
+      if (i == 0 || (int64_t)T * nseg > 1024) continue;
+    }
+    const int most = MAX_CAP(shapes[i][0]), cap = MERGE / nseg < most ? MERGE / nseg : most;
+    if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap};
+  }
+  return {0, 0, 0, 0};
+}
+
 // ------------------------------------------------------------------ sampling
 struct RowFilter {
   float temperature, top_p, min_p;
@@ -655,7 +982,22 @@ int check_distill(int dtype, const void* logits, int64_t ld, int T, int V, const
 }
 
 template <typename T>
-int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, int32_t* ids, float* rest, hipStream_t s) {
+int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, int32_t* ids, float* rest, void* ws, hipStream_t s) {
+  const Cut cut = cut_rows(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V, k);
+  if (cut.nt) {
+    SegHead* heads = (SegHead*)ws;
+    uint64_t* lists = (uint64_t*)(heads + (int64_t)n * cut.nseg);
+    const dim3 grid(n, cut.nseg);
+    if (cut.nt == 64)
+      hipLaunchKernelGGL((top_segment_kernel<T, 64, 4>), grid, dim3(64), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
+    else if (cut.vpt == 4)
+      hipLaunchKernelGGL((top_segment_kernel<T, 256, 4>), grid, dim3(256), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
+    else
+      hipLaunchKernelGGL((top_segment_kernel<T, 256, 16>), grid, dim3(256), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
+    if (cut.nseg > 1)
+      hipLaunchKernelGGL((top_merge_kernel<T, 256>), dim3(n), dim3(256), 0, s, cut.nseg, k, cut.cap, tau, values, ids, rest, heads, lists);
+    return check_launch();
+  }
   if (V <= 32)
     hipLaunchKernelGGL((top_small_kernel<T, 32>), dim3((n + 7) / 8), dim3(256), 0, s, x, ld, n, V, k, tau, values, ids, rest);
   else if (V <= 64)
@@ -719,7 +1061,10 @@ int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, flo
 
 }  // namespace
 
-extern "C" int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k) { return 0; }
+extern "C" int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k) {
+  const Cut cut = cut_rows(dtype, T, V, k);
+  return cut.nseg > 1 ? (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8) : 0;
+}
 
 extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k, float temperature, void* values,
                              int32_t* ids, float* rest, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -727,8 +1072,11 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
   if (rc != PG_OK) return rc;
   if (!values || !ids || !rest || k <= 0 || k > V || !(temperature > 0.f) || !(temperature <= FLT_MAX)) return PG_ERR_ARG;
   if (k > MAX_K) return PG_ERR_UNSUPPORTED;
-  return dtype == PG_F32 ? top_rows((const float*)logits, ld, T, V, k, temperature, (float*)values, ids, rest, (hipStream_t)stream)
-                         : top_rows((const bf16_t*)logits, ld, T, V, k, temperature, (bf16_t*)values, ids, rest, (hipStream_t)stream);
+  const int64_t need = pg_top_logits_workspace_bytes(dtype, T, V, k);
+  if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
+  return dtype == PG_F32 ? top_rows((const float*)logits, ld, T, V, k, temperature, (float*)values, ids, rest, workspace, (hipStream_t)stream)
+                         : top_rows((const bf16_t*)logits, ld, T, V, k, temperature, (bf16_t*)values, ids, rest, workspace, (hipStream_t)stream);
 }
 
 extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V) { return 0; }
