@@ -339,7 +339,7 @@ int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k
  * off; temperature 0 takes the first entry (conf 1).  A row without an entry above -inf: pred -1, conf 0.  temps / ks / ps / mins
  * (nullable): settings per row; there out-of-range values mean: temperature <= 0 or NaN 0, k <= 0 off, top_p >= 1 or NaN off,
  * top_p <= 0 the first entry, min_p <= 0 or NaN off, min_p > 1 as 1. */
-int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V);
+int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, int top_k /* 0: none, or per row */);
 int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
                        float temperature, int top_k, float top_p, float min_p, const float* temps, const int32_t* ks,
                        const float* ps, const float* mins, int64_t* pred, float* conf, void* workspace, int64_t workspace_bytes,

@@ -101,132 +101,12 @@ __device__ __forceinline__ double exp2_f64(double t) {
   return ldexp(p, (int)n);
 }
 
-// ------------------------------------------------------------------ radix selection of one row by a whole workgroup
-// Five digits of the entry key from the top: 11 + 11 + 10 bits of the value, 12 + 12 of the index (the 8 bits between are ones
-// for every index below 2^24).  Each pass counts (and weighs) the entries that share the digits found so far.
-constexpr int SEL_BINS = 4096;
-struct SelLds {
-  uint32_t count[SEL_BINS];
-  uint64_t mass[SEL_BINS];
-  uint64_t wave_mass[16];
-  uint32_t wave_count[16];
-  uint64_t key, above_mass, bin_mass;
-  uint32_t above, bin_count;
-};
-__device__ __constant__ const int SEL_SHIFT[5] = {53, 42, 32, 12, 0};
-__device__ __constant__ const int SEL_BITS[5] = {11, 11, 10, 12, 12};
-
-constexpr double MASS_ONE = 1099511627776.0;  // 2^40: weights are at most 1
-
-// The largest key B such that the entries with key >= B number at least `need` (BY_MASS: weigh at least `need`) among the
-// entries with key >= floor_key; returns their mass through *mass (BY_MASS).  weight(x) in (0, 1].
-template <typename T, int NT, bool BY_MASS, typename W>
-__device__ uint64_t select_key(const T* row, int V, uint64_t floor_key, uint64_t need, W weight, SelLds& s) {
-  uint64_t prefix = 0, mask = 0;
-  for (int d = 0; d < 5; ++d) {
-    const int shift = SEL_SHIFT[d], bins = 1 << SEL_BITS[d];
-    __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += NT) {
-      s.count[i] = 0;
-      if (BY_MASS) s.mass[i] = 0;
-    }
-    __syncthreads();
-    each<T, NT>(row, V, [&](int i, float x) {
-      const uint64_t k = entry_key(x, i);
-      if (k < floor_key || (k & mask) != prefix) return;
-      const int b = (int)(k >> shift) & (bins - 1);
-      atomicAdd(&s.count[b], 1u);
-      if (BY_MASS) atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)(weight(x) * MASS_ONE));
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) {  // walk the bins from the top
-      uint64_t left = need;
-      int b = bins - 1, last = -1;
-      for (; b >= 0; --b) {
-        if (!s.count[b]) continue;
-        const uint64_t have = BY_MASS ? s.mass[b] : s.count[b];
-        last = b;
-        if (have >= left) break;
-        left -= have;
-      }
-      if (b < 0) b = last, left = BY_MASS ? s.mass[b] : s.count[b];  // (fewer than `need`: everything)
-      s.key = (uint64_t)b;
-      s.above_mass = left;
-      s.bin_count = s.count[b];
-      s.bin_mass = BY_MASS ? s.mass[b] : s.count[b];
-    }
-    __syncthreads();
-    prefix |= s.key << shift;
-    mask |= (uint64_t)(bins - 1) << shift;
-    if (d == 2) {  // the bits between value and index
-      prefix |= 0xff000000ull;
-      mask |= 0xff000000ull;
-    }
-    need = s.above_mass;
-    if (s.bin_count == 1 || (!BY_MASS && need == s.bin_count)) break;  // the whole bin is in
-  }
-  // the digits not looked at are zero: every entry of the last bin is at least this key
-  return prefix > floor_key ? prefix : floor_key;
-}
-
-// ------------------------------------------------------------------ top entries
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, float tau,
-                                                 T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest) {
-  __shared__ SelLds sel;
-  __shared__ uint64_t list[MAX_K];
-  __shared__ uint32_t n_list;
-  __shared__ float red[16];
-  const int64_t t = blockIdx.x;
-  const T* row = logits + t * ld;
-  const float c = (float)(LOG2E / (double)tau);
-  const uint64_t B = select_key<T, NT, false>(row, V, 0, K, [](float) { return 0.0; }, sel);
-  int P = 1;
-  while (P < K) P <<= 1;
-  __syncthreads();
-  if (threadIdx.x == 0) n_list = 0;
-  for (int i = threadIdx.x; i < P; i += NT) list[i] = 0;
-  __syncthreads();
-  ExpSum es = {-FLT_MAX, 0.f};
-  float top_rest = -INFINITY;
-  each<T, NT>(row, V, [&](int i, float x) {
-    const uint64_t k = entry_key(x, i);
-    if (k >= B) {
-      list[atomicAdd(&n_list, 1u)] = k;
-    } else {
-      const float v = key_value((uint32_t)(k >> 32));
-      top_rest = fmaxf(top_rest, v);
-      exp_sum_add(es, v, c);
-    }
-  });
-  es = block_exp_sum<NT>(es, c, red);
-  top_rest = block_max<NT>(top_rest, red);
-  // bitonic sort, largest first
-  for (int size = 2; size <= P; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < P / 2; i += NT) {
-        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
-        const bool down = (a & size) == 0;
-        const uint64_t x = list[a], y = list[b];
-        if ((x < y) == down) { list[a] = y; list[b] = x; }
-      }
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < K; i += NT) {
-    values[t * K + i] = from_f32<T>(key_value((uint32_t)(list[i] >> 32)));
-    ids[t * K + i] = (int32_t)~(uint32_t)list[i];
-  }
-  if (threadIdx.x == 0)
-    rest[t] = top_rest == INFINITY ? INFINITY : es.s > 0.f ? (float)((double)es.m / tau + log((double)es.s)) : -INFINITY;
-}
-
 // ------------------------------------------------------------------ the largest entries of a segment of a row, kept in registers
 // A row is cut into segments of NT * VPT 16-byte vectors; a workgroup loads one whole segment into registers (all its loads in
 // flight at once) and reads it once.  Each thread's vectors form four groups; the K-th largest of the NT * 4 group maxima is a
 // lower bound of the segment's K-th largest entry and not far below it (64 of 1024 maxima leave about 70 entries above the
 // bound), found by eight rounds of counting on the upper 16 bits of their keys.  Vectors with an entry above the bound go to
-// LDS, everything else into the sum of exponentials.  Where too many entries tie at the bound, the exact K-th key is found by
+// LDS, all others into the sum of exponentials.  Where too many entries tie at the bound, the exact K-th key is found by
 // bisection over the segment instead.
 constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
 constexpr int MAX_SEG_K = 512;
@@ -261,14 +141,47 @@ __device__ __forceinline__ void exp_sum_one(ExpSum& a, float x, float c) {
   exp_sum_vec<1>(a, o, fmaxf(x, -INFINITY), c);
 }
 
+// exp((x - m) / temperature) for x <= m in whole multiples of 2^-40: sums of these are the same in any order.
+__device__ __forceinline__ uint64_t fixed_weight(float x, float m, float c) {
+  return x == m ? 1ull << 40 : (uint64_t)(__builtin_amdgcn_exp2f((x - m) * c) * 0x1p40f);
+}
+
+// The largest multiple B of 2^lo with at least K of the workgroup's keys k[R] >= B (0: there are fewer), two bits a round.
+template <int NT, int R, typename Key> __device__ __forceinline__ Key kth_bound(const Key (&k)[R], int K, int hi, int lo, int (*counts)[48]) {
+  constexpr int NW = NT / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Key bound = 0;
+  for (int b = hi; b >= lo; b -= 2) {
+    int cnt[3] = {0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int g = 0; g < R; ++g) cnt[i] += __popcll(__ballot(k[g] >= (bound | ((Key)(i + 1) << b))));
+    if (NW > 1) {  // (two buffers: a round's counts are read while the next round's are written)
+      int* w = counts[(b >> 1) & 1];
+      if (lane < 3) w[wave * 3 + lane] = lane == 0 ? cnt[0] : lane == 1 ? cnt[1] : cnt[2];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        cnt[i] = 0;
+#pragma unroll
+        for (int j = 0; j < NW; ++j) cnt[i] += w[j * 3 + i];
+      }
+    }
+    bound |= (Key)(cnt[2] >= K ? 3 : cnt[1] >= K ? 2 : cnt[0] >= K ? 1 : 0) << b;
+  }
+  return bound;
+}
+
 template <int NT> struct SegLds {
+  uint64_t wave[16];
   static constexpr int STAGE = NT == 64 ? 256 : 512;  // vectors that may hold an entry above the bound
   static constexpr int LIST = NT == 64 ? 512 : 2048;  // keys (a power of two of at least MAX_CAP)
   uint64_t list[LIST];
   uint4 vec[STAGE];
   int at[STAGE];
   uint32_t n_vec, n;
-  int wave_count[2][3 * 16];
+  int counts[2][48];
   float red[16];
 };
 struct SegHead {      // what a segment leaves for the merge
@@ -329,7 +242,7 @@ template <typename T, int NT, int VPT> struct Segment {
 template <typename T, int NT, int VPT, bool FINITE>
 __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, int K, int cap, float c, SegLds<NT>& l, uint64_t& level,
                                        ExpSum& rest) {
-  constexpr int E = Segment<T, NT, VPT>::E, NW = NT / 64, STAGE = SegLds<NT>::STAGE, LIST = SegLds<NT>::LIST;
+  constexpr int E = Segment<T, NT, VPT>::E, STAGE = SegLds<NT>::STAGE, LIST = SegLds<NT>::LIST;
   uint64_t* list = l.list;
   float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -343,29 +256,7 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
 #pragma unroll
   for (int g = 0; g < 4; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
   if (threadIdx.x == 0) l.n_vec = 0, l.n = 0;
-  uint32_t bound = 0;
-  for (int b = 30; b >= 16; b -= 2) {  // two bits a round
-    int cnt[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const uint32_t trial = bound | ((uint32_t)(i + 1) << b);
-      cnt[i] = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) cnt[i] += __popcll(__ballot(mk[g] >= trial));
-    }
-    if (NW > 1) {
-      int* w = l.wave_count[(b >> 1) & 1];
-      if ((threadIdx.x & 63) < 3) w[(threadIdx.x >> 6) * 3 + (threadIdx.x & 63)] = (threadIdx.x & 63) == 0 ? cnt[0] : (threadIdx.x & 63) == 1 ? cnt[1] : cnt[2];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        cnt[i] = 0;
-#pragma unroll
-        for (int k = 0; k < NW; ++k) cnt[i] += w[k * 3 + i];
-      }
-    }
-    bound |= (cnt[2] >= K ? 3u : cnt[1] >= K ? 2u : cnt[0] >= K ? 1u : 0u) << b;
-  }
+  const uint32_t bound = kth_bound<NT>(mk, K, 30, 16, l.counts);
   const float thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
   rest = {-FLT_MAX, 0.f};
   __syncthreads();
@@ -387,23 +278,38 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
   }
   auto take = [&](float x, int i) {
     x = fmaxf(x, -INFINITY);
-    if (x >= thr && (!FINITE || x > -INFINITY)) {
+    const bool in = x >= thr && (!FINITE || x > -INFINITY);
+    if (in) {
       const uint32_t p = atomicAdd(&l.n, 1u);
       if (p < LIST) list[p] = entry_key(x, i);
-    } else {
-      exp_sum_one(rest, x, c);
     }
+    return in;
   };
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (sg.end_at[i] >= 0) take(sg.ends[i], sg.end_at[i]);
+    if (sg.end_at[i] >= 0 && !take(sg.ends[i], sg.end_at[i])) exp_sum_one(rest, sg.ends[i], c);
   __syncthreads();
-  const int n_vec = l.n_vec;
-  for (int i = threadIdx.x; i < (n_vec < STAGE ? n_vec : STAGE); i += NT) {
+  const int n_vec = l.n_vec, staged = n_vec < STAGE ? n_vec : STAGE;
+  float most = -INFINITY;  // the largest entry that a vector with a listed one brings along
+  for (int i = threadIdx.x; i < staged; i += NT) {
     float o[E];
     unpack(l.vec[i], o);
 #pragma unroll
-    for (int e = 0; e < E; ++e) take(o[e], l.at[i] + e);
+    for (int e = 0; e < E; ++e)
+      if (!take(o[e], l.at[i] + e)) most = fmaxf(most, o[e]);
+  }
+  most = block_max<NT>(most, l.red);
+  if (most > -INFINITY) {  // the staged vectors are in no fixed order: their sum is one of whole multiples of 2^-40 of the largest
+    uint64_t sum = 0;
+    for (int i = threadIdx.x; i < staged; i += NT) {
+      float o[E];
+      unpack(l.vec[i], o);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (o[e] < thr) sum += fixed_weight(o[e], most, c);
+    }
+    sum = block_all<NT>(sum, l.wave, [](uint64_t a, uint64_t b) { return a + b; });
+    if (threadIdx.x == 0) rest = exp_sum_join(rest, {most, (float)sum * 0x1p-40f}, c);
   }
   __syncthreads();
   int n = l.n;
@@ -500,34 +406,116 @@ __global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict_
   if (threadIdx.x == 0) heads[at] = {level, rest.m, rest.s, (uint32_t)n, {0, 0, 0}};
 }
 
-// All segments' keys of row t into list; returns their number, the sums in rest (one segment per thread), and the row's level.
-template <int NT>
-__device__ __forceinline__ int gather_segments(const SegHead* heads, const uint64_t* lists, int64_t t, int nseg, int cap, uint64_t* list,
-                                               ExpSum& rest, uint64_t& level) {
-  rest = {-FLT_MAX, 0.f};
-  level = 0;
-  int n = 0;
-  for (int s = 0; s < nseg; ++s) {
-    const SegHead h = heads[t * nseg + s];
-    if (s % NT == (int)threadIdx.x) rest = rest.s == 0.f ? ExpSum{h.m, h.s} : rest;
-    level = h.level > level ? h.level : level;
-    for (int i = threadIdx.x; i < (int)h.n; i += NT) list[n + i] = lists[(t * nseg + s) * cap + i];
-    n += h.n;
+// The segments' keys of one row, at most MERGE, R = MERGE / NT to a thread (0: none).
+constexpr int MAX_SEGS = 64;
+template <int NT> struct RowKeys {
+  static constexpr int R = MERGE / NT;
+  uint64_t k[R];
+  uint64_t level;  // complete down to here
+  ExpSum rest;     // this thread's share of the entries that no segment listed
+  int n;
+  __device__ __forceinline__ void load(const SegHead* heads, const uint64_t* lists, int64_t t, int nseg, int cap, uint32_t* ends) {
+    rest = {-FLT_MAX, 0.f};
+    const bool mine = (int)threadIdx.x < nseg;
+    SegHead h = {};
+    if (mine) {
+      h = heads[t * nseg + threadIdx.x];
+      rest = {h.m, h.s};
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {  // (nseg <= 64: one wave)
+      uint32_t end = mine ? h.n : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(end, o, 64);
+        if ((int)threadIdx.x >= o) end += up;
+      }
+      uint64_t lv = mine ? h.level : 0;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t v = __shfl_xor(lv, o, 64);
+        lv = v > lv ? v : lv;
+      }
+      ends[threadIdx.x] = end;
+      if (threadIdx.x == 0) {
+        ends[64] = (uint32_t)lv;
+        ends[65] = (uint32_t)(lv >> 32);
+      }
+    }
+    __syncthreads();
+    n = ends[nseg - 1];
+    level = ((uint64_t)ends[65] << 32) | ends[64];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = r * NT + threadIdx.x;
+      k[r] = 0;
+      if (i < n) {
+        int s = 0;
+        while ((int)ends[s] <= i) ++s;
+        k[r] = lists[(t * nseg + s) * cap + i - (s ? (int)ends[s - 1] : 0)];
+      }
+    }
   }
-  return n;
-}
+  // The keys that can be among the first K, unsorted, into list; the sum over the others joins rest.  More than `room` of them
+  // (ties at the bound): the exact K-th key as the bound.  The others come in no fixed order: their sum is one of whole multiples
+  // of 2^-40 of the largest.
+  template <typename L> __device__ __forceinline__ int first(int K, int room, uint64_t* list, float c, L& l) {
+    uint64_t bound = 0;
+    if (n > 2 * K) bound = kth_bound<NT>(k, K, 62, 48, l.counts);
+    for (int round = 0;; ++round) {
+      int m = 0;
+      uint64_t most = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        m += k[r] != 0 && k[r] >= bound;
+        if (k[r] < bound && k[r] > most) most = k[r];
+      }
+      m = block_all<NT>(m, reinterpret_cast<int*>(l.red), [](int a, int b) { return a + b; });
+      if (m > room && round == 0) {
+        bound = kth_bound<NT>(k, K, 62, 0, l.counts);
+        continue;
+      }
+      if (bound) {
+        most = block_all<NT>(most, l.wave, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        const float x0 = key_value((uint32_t)(most >> 32));
+        uint64_t sum = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (k[r] != 0 && k[r] < bound) sum += fixed_weight(key_value((uint32_t)(k[r] >> 32)), x0, c);
+        sum = block_all<NT>(sum, l.wave, [](uint64_t a, uint64_t b) { return a + b; });
+        if (threadIdx.x == 0 && most && x0 > -INFINITY) rest = exp_sum_join(rest, {x0, (float)sum * 0x1p-40f}, c);
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) l.n = 0;
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (k[r] != 0 && k[r] >= bound) list[atomicAdd(&l.n, 1u)] = k[r];
+      __syncthreads();
+      level = bound > level ? bound : level;
+      return m;
+    }
+  }
+};
+
+struct MergeLds {
+  uint64_t list[2 * MAX_SEG_K], wave[16];
+  float red[16];
+  uint32_t n, ends[66];
+  int counts[2][48];
+};
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void top_merge_kernel(int nseg, int K, int cap, float tau, T* __restrict__ values,
                                                        int32_t* __restrict__ ids, float* __restrict__ rest_out,
                                                        const SegHead* __restrict__ heads, const uint64_t* __restrict__ lists) {
-  __shared__ uint64_t list[MERGE];
-  __shared__ float red[16];
+  __shared__ MergeLds l;
   const int64_t t = blockIdx.x;
-  ExpSum rest;
-  uint64_t level;
-  const int n = gather_segments<NT>(heads, lists, t, nseg, cap, list, rest, level);
-  top_finish<T, NT>(list, n, K, tau, (float)(LOG2E / (double)tau), rest, red, values + t * K, ids + t * K, rest_out + t);
+  const float c = (float)(LOG2E / (double)tau);
+  RowKeys<NT> rk;
+  rk.load(heads, lists, t, nseg, cap, l.ends);
+  const int n = rk.first(K, 2 * MAX_SEG_K, l.list, c, l);
+  top_finish<T, NT>(l.list, n, K, tau, c, rk.rest, l.red, values + t * K, ids + t * K, rest_out + t);
 }
 
 // How a call is cut: threads and vectors per thread of a segment, segments per row, keys a segment may leave.
@@ -542,7 +530,10 @@ Cut cut_rows(int dtype, int T, int V, int K) {
       // few rows: small segments, to spread them over the chip; many: the next larger ones
       if (i == 0 || (int64_t)T * nseg > 1024) continue;
     }
-    const int most = MAX_CAP(shapes[i][0]), cap = MERGE / nseg < most ? MERGE / nseg : most;
+    if (nseg > MAX_SEGS) continue;
+    int cap = 2 * K + 64;
+    if (cap > MAX_CAP(shapes[i][0])) cap = MAX_CAP(shapes[i][0]);
+    if (cap > MERGE / nseg) cap = MERGE / nseg;
     if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap};
   }
   return {0, 0, 0, 0};
@@ -566,60 +557,286 @@ struct SampleArgs {
     return {temps ? temps[t] : temperature, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
   }
 };
+// ------------------------------------------------------------------ one row by a whole workgroup, any boundary
+constexpr int BINS = 2048, POOL = 2048;
+constexpr double MASS_ONE = 1099511627776.0;  // 2^40: weights are at most 1, their sums whole multiples of 2^-40 in any order
+// Six digits of an entry's key from the top: 11 + 11 + 10 bits of the value, 11 + 11 + 10 of ~index.
+__device__ __constant__ const int SEL_SHIFT[6] = {53, 42, 32, 21, 10, 0};
+__device__ __constant__ const int SEL_BITS[6] = {11, 11, 10, 11, 11, 10};
+
+template <int NT> struct RowLds {
+  union {
+    struct { uint64_t mass[BINS]; uint32_t count[BINS]; } h;
+    uint64_t list[POOL];
+  };
+  uint64_t wave[16];
+  uint64_t cut_before;
+  double redd[16];
+  float red[16];
+  int cut, counts[2][48];
+  uint32_t n, ends[66];
+};
+
+// The first i < n at which get(0) + ... + get(i) reaches need, and the sum before it; i = n, the sum of all, if none does.
+struct CutAt { int i; uint64_t before; };
+template <int NT, typename L, typename F> __device__ __forceinline__ CutAt find_cut(int n, uint64_t need, L& l, F get) {
+  const int per = (n + NT - 1) / NT, a = min((int)threadIdx.x * per, n), b = min(a + per, n);
+  uint64_t sum = 0;
+  for (int i = a; i < b; ++i) sum += get(i);
+  uint64_t upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t v = __shfl_up(upto, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) upto += v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x >> 6] = upto;
+  if (threadIdx.x == 0) l.cut = n;
+  __syncthreads();
+  uint64_t all = 0, off = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) off += l.wave[w];
+    all += l.wave[w];
+  }
+  upto += off;
+  uint64_t before = upto - sum;
+  if (before < need && upto >= need) {
+    int i = a;
+    for (uint64_t g; i < b && before + (g = get(i)) < need; ++i) before += g;
+    l.cut = i;
+    l.cut_before = before;
+  }
+  __syncthreads();
+  return l.cut < n ? CutAt{l.cut, l.cut_before} : CutAt{n, all};
+}
+
+// Entries of a row with key >= floor: the largest key B such that those >= B number `need` (BY_MASS: weigh at least the share
+// `part` of all of them).  First 2048 bins of equal width in m - x (an entry's bin never decreases with m - x, so bins are ranges
+// of the order), then the bin with the boundary is listed and sorted; one that does not fit the list (many equal values, entries
+// far below the largest) is divided by the key's bits first.
+template <typename T, int NT, bool BY_MASS, typename W>
+__device__ uint64_t boundary(const T* row, int V, float m, float bins_per_unit, uint64_t floor, int need_count, double part, W weight,
+                             RowLds<NT>& l) {
+  auto bin_of = [&](float x) {
+    x = fmaxf(x, -INFINITY);
+    const float d = (m - x) * bins_per_unit;
+    return d < (float)(BINS - 1) ? (int)d : x == m ? 0 : BINS - 1;
+  };
+  auto fixed = [&](float x) { return (uint64_t)(weight(x) * MASS_ONE); };
+  uint64_t need = need_count, prefix = 0, mask = 0;
+  int bin = -1, in_bin = 0;
+  for (int d = -1; d < 6; ++d) {
+    const int shift = d < 0 ? 0 : SEL_SHIFT[d], bins = d < 0 ? BINS : 1 << SEL_BITS[d];
+    __syncthreads();
+    for (int i = threadIdx.x; i < bins; i += NT) l.h.count[i] = 0, l.h.mass[i] = 0;
+    __syncthreads();
+    each<T, NT>(row, V, [&](int i, float x) {
+      const uint64_t k = entry_key(x, i);
+      if (k < floor) return;
+      int b = bin_of(x);
+      if (d >= 0) {
+        if (b != bin || (k & mask) != prefix) return;
+        b = bins - 1 - ((int)(k >> shift) & (bins - 1));
+      }
+      atomicAdd(&l.h.count[b], 1u);
+      if (BY_MASS) atomicAdd((unsigned long long*)&l.h.mass[b], (unsigned long long)fixed(x));
+    });
+    __syncthreads();
+    auto get = [&](int i) { return BY_MASS ? l.h.mass[i] : (uint64_t)l.h.count[i]; };
+    if (BY_MASS && d < 0) {
+      const CutAt all = find_cut<NT>(bins, ~0ull, l, get);
+      const double want = ceil(part * (double)all.before);
+      need = want < 1.0 ? 1 : (uint64_t)want < all.before ? (uint64_t)want : all.before;
+    }
+    const CutAt c = find_cut<NT>(bins, need, l, get);
+    const int b = c.i < bins ? c.i : bins - 1;  // (fewer than asked for: down to the last)
+    in_bin = l.h.count[b];
+    need = c.i < bins ? need - c.before : ~0ull;
+    if (d < 0) bin = b;
+    else {
+      prefix |= (uint64_t)(bins - 1 - b) << shift;
+      mask |= (uint64_t)(bins - 1) << shift;
+    }
+    if (in_bin <= POOL) break;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) l.n = 0;
+  __syncthreads();
+  each<T, NT>(row, V, [&](int i, float x) {
+    const uint64_t k = entry_key(x, i);
+    if (k >= floor && bin_of(x) == bin && (k & mask) == prefix) l.list[atomicAdd(&l.n, 1u)] = k;
+  });
+  __syncthreads();
+  const int n = l.n;
+  if (n == 0) return floor;
+  sort_keys<NT>(l.list, n);
+  const CutAt c = find_cut<NT>(n, need, l, [&](int i) { return BY_MASS ? fixed(key_value((uint32_t)(l.list[i] >> 32))) : (uint64_t)1; });
+  return l.list[c.i < n ? c.i : n - 1];
+}
+
+// The race over the entries that keep(x, key) admits, of the whole row: reads logits and, for those, noise.
+struct Race {
+  double best, total;
+  uint64_t at;
+  __device__ __forceinline__ void add(double w, float q, uint32_t i) {
+    total += w;
+    const double r = w > 0.0 ? w / (double)q : 0.0;
+    if (r > best || (r == best && i < at)) { best = r; at = i; }
+  }
+};
+
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void sample_filtered_kernel(const T* __restrict__ logits, int64_t ld,
-                                                             const float* __restrict__ noise, int64_t ld_noise, int V,
-                                                             SampleArgs args, int64_t* __restrict__ pred,
-                                                             float* __restrict__ conf) {
-  __shared__ SelLds sel;
-  __shared__ double redd[16];
-  __shared__ uint64_t redk[16];
+__global__ __launch_bounds__(NT) void sample_row_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
+                                                        int64_t ld_noise, int V, SampleArgs args, int nseg, int cap,
+                                                        const SegHead* __restrict__ heads, const uint64_t* __restrict__ lists,
+                                                        int64_t* __restrict__ pred, float* __restrict__ conf) {
+  __shared__ RowLds<NT> l;
   const int64_t t = blockIdx.x;
   const T* row = logits + t * ld;
   const float* q = noise + t * ld_noise;
   const RowFilter f = args.row(t);
-  const float temp = f.temperature, p = f.top_p;
-  const int k = f.top_k;
-  uint64_t kmax = 0;
-  each<T, NT>(row, V, [&](int i, float x) { const uint64_t e = entry_key(x, i); kmax = e > kmax ? e : kmax; });
-  kmax = block_all<NT>(kmax, redk, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-  const float m = key_value((uint32_t)(kmax >> 32));
-  const int64_t arg = (int64_t)(uint32_t)~(uint32_t)kmax;
-  if (m == -INFINITY || !(temp > 0.f)) {
-    if (threadIdx.x == 0) {
-      pred[t] = m == -INFINITY ? -1 : arg;
-      conf[t] = m == -INFINITY ? 0.f : 1.f;
+  const bool greedy = !(f.temperature > 0.f);
+  const double scale = LOG2E / (double)f.temperature;
+  uint64_t top;  // the row's first key
+  Race race = {-1.0, 0.0, ~0ull};
+  float m;
+  auto weight = [&](float x) { return x == m ? 1.0 : exp2_f64(((double)x - (double)m) * scale); };
+  bool done = false;
+  if (nseg) {
+    // from the segments' lists, if the end of the kept entries lies within them
+    RowKeys<NT> rk;
+    rk.load(heads, lists, t, nseg, cap, l.ends);
+    const float c = greedy ? 0.f : (float)scale;
+    const int want = f.top_k > 0 && f.top_k < POOL / 4 ? f.top_k : POOL / 8;
+    const int n = rk.first(want, POOL, l.list, c, l);
+    if (n == 0) {
+      if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
+      return;
     }
+    sort_keys<NT>(l.list, n);
+    top = l.list[0];
+    m = key_value((uint32_t)(top >> 32));
+    if (!greedy && m < INFINITY) {
+      const ExpSum out = block_exp_sum<NT>(rk.rest, c, l.red);
+      const double left = (double)out.s * (double)__builtin_amdgcn_exp2f((out.m - m) * c);  // the mass outside the list
+      const CutAt known = find_cut<NT>(n, ~0ull, l, [&](int i) { return (uint64_t)(l.list[i] >= rk.level); });
+      const int nv = (int)known.before;           // the list is complete that far
+      const bool whole = rk.level == 0;           // (every entry above -inf)
+      const int nk = f.top_k > 0 && f.top_k < V ? f.top_k : V;
+      const bool nk_in = nk <= nv || whole;
+      int keep = nk_in ? (nk < nv ? nk : nv) : V;
+      bool sure = true;
+      auto mass = [&](int i) { return (uint64_t)(weight(key_value((uint32_t)(l.list[i] >> 32))) * MASS_ONE); };
+      if (f.top_p < 1.f) {
+        if (nk_in || nk == V) {
+          const int among = nk_in ? keep : n;
+          const CutAt all = find_cut<NT>(among, ~0ull, l, mass);
+          // fp32 sums of up to 2^7 terms per thread and a tree: their relative error stays below 2^-15
+          const double rest = nk_in ? 0.0 : left * MASS_ONE, W = (double)all.before + rest, err = rest * 0x1p-15;
+          const double need = ceil((double)f.top_p * W);
+          const CutAt at = find_cut<NT>(nv, need < 1.0 ? 1 : (uint64_t)need, l, mass);
+          const double lo = need - err, hi = need + err;
+          if (at.i < nv) {
+            if (err > 0.0 && !((double)at.before < lo && (double)at.before + (double)mass(at.i) >= hi)) sure = false;
+            keep = keep < at.i + 1 ? keep : at.i + 1;
+          } else if (!nk_in && (double)at.before >= lo) {
+            sure = false;
+          }
+        } else {
+          sure = false;  // (the mass of the first k is not known)
+        }
+      }
+      if (f.min_p > 0.f) {
+        const CutAt above = find_cut<NT>(nv, ~0ull, l, [&](int i) { return (uint64_t)f.above_min_p(key_value((uint32_t)(l.list[i] >> 32)), m); });
+        const int na = (int)above.before;
+        if (na < nv || whole) keep = keep < na ? keep : na;
+      }
+      done = sure && keep <= nv;
+      if (done)
+        for (int i = threadIdx.x; i < keep; i += NT) {
+          const uint32_t at = ~(uint32_t)l.list[i];
+          race.add(weight(key_value((uint32_t)(l.list[i] >> 32))), q[at], at);
+        }
+    }
+  } else {
+    top = 0;
+    each<T, NT>(row, V, [&](int i, float x) { const uint64_t e = entry_key(x, i); top = e > top ? e : top; });
+    top = block_all<NT>(top, l.wave, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+    m = key_value((uint32_t)(top >> 32));
+    if (m == -INFINITY) {
+      if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
+      return;
+    }
+  }
+  const uint32_t arg = ~(uint32_t)top;
+  if (greedy) {
+    if (threadIdx.x == 0) pred[t] = arg, conf[t] = 1.f;
     return;
   }
-  const double scale = LOG2E / (double)temp;
-  auto weight = [&](float x) { return x == m ? 1.0 : exp2_f64(((double)x - (double)m) * scale); };
-  uint64_t B = 0;
-  if (k > 0 && k < V) B = select_key<T, NT, false>(row, V, 0, k, weight, sel);
-  if (p < 1.f) {
-    double mass = 0;
-    each<T, NT>(row, V, [&](int i, float x) { if (entry_key(x, i) >= B) mass += (double)(uint64_t)(weight(x) * MASS_ONE); });
-    mass = block_sum<NT>(mass, redd);
-    const double want = ceil((double)p * mass);
-    B = select_key<T, NT, true>(row, V, B, want < 1.0 ? 1 : (uint64_t)want, weight, sel);
+  if (!done) {
+    // from the whole row: the boundary key of each filter, then the race
+    const float span = fminf(40.f * f.temperature, 32.f), per = (float)BINS / span;
+    uint64_t B = 0;
+    if (f.top_k > 0 && f.top_k < V) B = boundary<T, NT, false>(row, V, m, per, 0, f.top_k, 0.0, weight, l);
+    if (f.top_p < 1.f) B = boundary<T, NT, true>(row, V, m, per, B, 0, (double)f.top_p, weight, l);
+    each<T, NT>(row, V, [&](int i, float x) {
+      if (x > -INFINITY && entry_key(x, i) >= B && f.above_min_p(x, m)) race.add(weight(x), q[i], i);
+    });
   }
-  double best = -1.0, total = 0.0;
-  uint64_t at = ~0ull;
-  each<T, NT>(row, V, [&](int i, float x) {
-    if (entry_key(x, i) < B || !(x > -INFINITY) || !f.above_min_p(x, m)) return;
-    const double w = weight(x);
-    total += w;
-    const double r = w > 0.0 ? w / (double)q[i] : 0.0;
-    if (r > best || (r == best && (uint64_t)i < at)) { best = r; at = i; }
-  });
-  total = block_sum<NT>(total, redd);
-  const double top = block_all<NT>(best, redd, [](double a, double b) { return a > b ? a : b; });
-  at = block_all<NT>(best == top ? at : (uint64_t)~0ull, redk, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  const double total = block_sum<NT>(race.total, l.redd);
+  const double best = block_all<NT>(race.best, l.redd, [](double a, double b) { return a > b ? a : b; });
+  const uint64_t at = block_all<NT>(race.best == best ? race.at : (uint64_t)~0ull, l.wave, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
   if (threadIdx.x == 0) {
-    const int64_t i = at == ~0ull ? arg : (int64_t)at;
+    const uint32_t i = at == ~0ull ? arg : (uint32_t)at;
     pred[t] = i;
     conf[t] = (float)(weight(to_f32<T>(row[i])) / total);
   }
+}
+
+template <typename T, int NT, int VPT>
+__global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
+                                                               int cap, SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
+  __shared__ SegLds<NT> l;
+  const int64_t t = blockIdx.x;
+  const int seg = blockIdx.y, nseg = gridDim.y;
+  const float temp = args.temps ? args.temps[t] : args.temperature;
+  const float c = temp > 0.f ? (float)(LOG2E / (double)temp) : 0.f;
+  const T* row = logits + t * ld;
+  Segment<T, NT, VPT> sg;
+  sg.load(row, V, seg, nseg);
+  uint64_t level;
+  ExpSum rest;
+  const int n = collect<T, NT, VPT, true>(sg, row, K, cap, c, l, level, rest);
+  rest = block_exp_sum<NT>(rest, c, l.red);
+  const int64_t at = t * nseg + seg;
+  for (int i = threadIdx.x; i < n; i += NT) lists[at * cap + i] = l.list[i];
+  if (threadIdx.x == 0) heads[at] = {level, rest.m, rest.s, (uint32_t)n, {0, 0, 0}};
+}
+
+// ------------------------------------------------------------------ top entries, any k and vocabulary
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, float tau,
+                                                 T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest) {
+  __shared__ RowLds<NT> l;
+  const int64_t t = blockIdx.x;
+  const T* row = logits + t * ld;
+  const float c = (float)(LOG2E / (double)tau);
+  float m = -INFINITY;
+  each<T, NT>(row, V, [&](int, float x) { m = fmaxf(m, x); });
+  m = block_max<NT>(m, l.red);
+  const uint64_t B = boundary<T, NT, false>(row, V, m, BINS / 32.f, 0, K, 0.0, [](float) { return 0.0; }, l);
+  __syncthreads();
+  if (threadIdx.x == 0) l.n = 0;
+  __syncthreads();
+  ExpSum out = {-FLT_MAX, 0.f};
+  each<T, NT>(row, V, [&](int i, float x) {
+    const uint64_t k = entry_key(x, i);
+    if (k >= B) l.list[atomicAdd(&l.n, 1u)] = k;
+    else exp_sum_one(out, x, c);
+  });
+  __syncthreads();
+  top_finish<T, NT>(l.list, K, K, tau, c, out, l.red, values + t * K, ids + t * K, rest + t);
 }
 
 // ------------------------------------------------------------------ distillation
@@ -1007,15 +1224,42 @@ int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, 
   return check_launch();
 }
 
+// The entries the segments look for: k itself where it is one number up to 512, else 128, the end of most nucleus and min-p
+// sets.  No segments where they could not end the kept set: no filter at all, or a larger k that only top_p or nothing can undercut.
+int sample_k(int top_k) { return top_k > 0 && top_k <= MAX_SEG_K ? (top_k < 16 ? 16 : top_k) : 128; }
+Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
+  const bool rows = a.temps || a.ks || a.ps || a.mins;
+  const bool by_k = a.top_k > 0 && a.top_k <= MAX_SEG_K && a.top_k < V, large_k = a.top_k > MAX_SEG_K && a.top_k < V;
+  const bool ends = by_k || (!large_k && a.top_p < 1.f) || a.min_p > 0.f || a.temperature == 0.f;
+  if (!rows && !ends) return {0, 0, 0, 0};
+  return cut_rows(dtype, T, V, sample_k(a.ks ? 0 : a.top_k));
+}
+
 template <typename T>
 int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int V, const SampleArgs& a, int64_t* pred, float* conf,
-                hipStream_t s) {
+                void* ws, hipStream_t s) {
   if (V <= 32)
     hipLaunchKernelGGL((sample_small_kernel<T, 32>), dim3((n + 7) / 8), dim3(256), 0, s, x, ld, q, ldq, n, V, a, pred, conf);
   else if (V <= 64)
     hipLaunchKernelGGL((sample_small_kernel<T, 64>), dim3((n + 3) / 4), dim3(256), 0, s, x, ld, q, ldq, n, V, a, pred, conf);
-  else
-    hipLaunchKernelGGL((sample_filtered_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, q, ldq, V, a, pred, conf);
+  else {
+    const Cut cut = sample_cut(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V, a);
+    SegHead* heads = (SegHead*)ws;
+    uint64_t* lists = (uint64_t*)(heads + (int64_t)n * cut.nseg);
+    const dim3 grid(n, cut.nseg);
+    const int K = sample_k(a.ks ? 0 : a.top_k);
+    if (cut.nt == 64)
+      hipLaunchKernelGGL((sample_segment_kernel<T, 64, 4>), grid, dim3(64), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
+    else if (cut.nt && cut.vpt == 4)
+      hipLaunchKernelGGL((sample_segment_kernel<T, 256, 4>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
+    else if (cut.nt)
+      hipLaunchKernelGGL((sample_segment_kernel<T, 256, 16>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
+    // one row per CU at most: the whole CU for a row
+    if (n <= 256)
+      hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3(n), dim3(1024), 0, s, x, ld, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
+    else
+      hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
+  }
   return check_launch();
 }
 
@@ -1079,7 +1323,10 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
                          : top_rows((const bf16_t*)logits, ld, T, V, k, temperature, (bf16_t*)values, ids, rest, workspace, (hipStream_t)stream);
 }
 
-extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V) { return 0; }
+extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, int top_k) {
+  const Cut cut = cut_rows(dtype, T, V, sample_k(top_k));
+  return (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8);
+}
 
 extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
                                   float temperature, int top_k, float top_p, float min_p, const float* temps, const int32_t* ks,
@@ -1091,9 +1338,12 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
   if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
       (!mins && !(min_p >= 0.f && min_p <= 1.f)))
     return PG_ERR_ARG;
+  const int64_t need = pg_sample_filtered_workspace_bytes(dtype, T, V, ks ? 0 : top_k);
+  if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
   const SampleArgs a = {temperature, top_p, min_p, top_k, temps, ks, ps, mins};
-  return dtype == PG_F32 ? sample_rows((const float*)logits, ld, noise, ld_noise, T, V, a, pred, conf, (hipStream_t)stream)
-                         : sample_rows((const bf16_t*)logits, ld, noise, ld_noise, T, V, a, pred, conf, (hipStream_t)stream);
+  return dtype == PG_F32 ? sample_rows((const float*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream)
+                         : sample_rows((const bf16_t*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream);
 }
 
 extern "C" int64_t pg_distill_stash_floats(void) { return STASH; }

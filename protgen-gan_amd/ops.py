@@ -336,7 +336,7 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         _launch(logits, "pg_sample_filtered",
                 (dt, logits.data_ptr(), ld, noise.data_ptr(), ld_noise, T, V, num["temperature"], min(num["top_k"], V), num["top_p"],
                  num["min_p"], ptr(rows.get("temperature")), ptr(rows.get("top_k")), ptr(rows.get("top_p")),
-                 ptr(rows.get("min_p")), pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V))
+                 ptr(rows.get("min_p")), pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V, min(num["top_k"], V)))
     return pred, conf
 
 
