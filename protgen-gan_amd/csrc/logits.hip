@@ -27,21 +27,40 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t entry_key(float x, uint32_t i) { return ((uint64_t)value_key(x) << 32) | (uint32_t)~i; }
 
+__device__ __forceinline__ void unpack(uint4 d, float (&o)[4]) {
+  o[0] = __uint_as_float(d.x); o[1] = __uint_as_float(d.y); o[2] = __uint_as_float(d.z); o[3] = __uint_as_float(d.w);
+}
+__device__ __forceinline__ void unpack(uint4 d, float (&o)[8]) {
+  o[0] = __uint_as_float(d.x << 16); o[1] = __uint_as_float(d.x & 0xffff0000u);
+  o[2] = __uint_as_float(d.y << 16); o[3] = __uint_as_float(d.y & 0xffff0000u);
+  o[4] = __uint_as_float(d.z << 16); o[5] = __uint_as_float(d.z & 0xffff0000u);
+  o[6] = __uint_as_float(d.w << 16); o[7] = __uint_as_float(d.w & 0xffff0000u);
+}
 // f(index, value) over the n elements at p: elements up to the first 16-byte boundary and behind the last whole 16 bytes one by
-// one, the rest in 16-byte loads.
+// one, the rest in 16-byte loads, four in flight per thread (with one, a pass over a row is sixteen memory latencies in a row).
 template <typename T, int NT, typename F> __device__ __forceinline__ void each(const T* p, int n, F f) {
   constexpr int E = 16 / (int)sizeof(T);
   int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
   if (head > n) head = n;
-  if ((int)threadIdx.x < head) f((int)threadIdx.x, to_f32<T>(p[threadIdx.x]));
-  const int nv = (n - head) / E;
-  for (int v = threadIdx.x; v < nv; v += NT) {
-    float o[E];
-    VecIO<T, E>::load(p + head + v * E, o);
+  const int nv = (n - head) / E, tail = head + nv * E;
+  const uint4* vec = reinterpret_cast<const uint4*>(p + head);
+  if ((int)threadIdx.x < nv) {
+    uint4 d[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) f(head + v * E + e, o[e]);
+    for (int u = 0; u < 4; ++u) d[u] = vec[min((int)threadIdx.x + u * NT, nv - 1)];
+#pragma unroll 1
+    for (int v = threadIdx.x; v < nv; v += NT) {
+      float o[E];
+      unpack(d[0], o);
+      d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
+      d[3] = vec[min(v + 4 * NT, nv - 1)];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(head + v * E + e, o[e]);
+    }
   }
-  for (int i = head + nv * E + threadIdx.x; i < n; i += NT) f(i, to_f32<T>(p[i]));
+#pragma unroll 1
+  for (int i = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head; i < n; i += i < head ? n : NT)
+    f(i, to_f32<T>(p[i]));
 }
 
 template <int NT, typename T, typename Op> __device__ __forceinline__ T block_all(T v, T* lds, Op op) {
@@ -83,20 +102,19 @@ template <int NT> __device__ __forceinline__ ExpSum block_exp_sum(ExpSum a, floa
   return {m, s};
 }
 
-// 2^t in 64 bits for t <= 0: 2^t = 2^n 2^f, |f| <= 1/2, the Taylor series of 2^f to degree 10 (remainder below 3e-13).
+// 2^t in 64 bits for t <= 0: 2^t = 2^n 2^f, |f| <= 1/2, the Taylor series of 2^f to degree 9 (remainder below 8e-12).
 __device__ __forceinline__ double exp2_f64(double t) {
-  if (!(t > -1000.0)) return 0.0;
-  const double n = rint(t), f = (t - n) * LN2;
-  double p = 1.0 / 3628800.0;
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
+  t = fmax(t, -1022.0);
+  const double n = rint(t), f = t - n;
+  double p = 1.01780860092396959520e-7;           // ln(2)^9 / 9!
+  p = fma(p, f, 1.32154867901443052734e-6);
+  p = fma(p, f, 1.52527338040598376946e-5);
+  p = fma(p, f, 1.54035303933816060656e-4);
+  p = fma(p, f, 1.33335581464284411157e-3);
+  p = fma(p, f, 9.61812910762847687873e-3);
+  p = fma(p, f, 5.55041086648215761801e-2);
+  p = fma(p, f, 2.40226506959100694072e-1);
+  p = fma(p, f, 6.93147180559945286227e-1);
   p = fma(p, f, 1.0);
   return ldexp(p, (int)n);
 }
@@ -112,15 +130,6 @@ constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
 constexpr int MAX_SEG_K = 512;
 constexpr int MAX_CAP(int nt) { return nt == 64 ? 512 : 1088; }  // keys a segment may leave
 
-__device__ __forceinline__ void unpack(uint4 d, float (&o)[4]) {
-  o[0] = __uint_as_float(d.x); o[1] = __uint_as_float(d.y); o[2] = __uint_as_float(d.z); o[3] = __uint_as_float(d.w);
-}
-__device__ __forceinline__ void unpack(uint4 d, float (&o)[8]) {
-  o[0] = __uint_as_float(d.x << 16); o[1] = __uint_as_float(d.x & 0xffff0000u);
-  o[2] = __uint_as_float(d.y << 16); o[3] = __uint_as_float(d.y & 0xffff0000u);
-  o[4] = __uint_as_float(d.z << 16); o[5] = __uint_as_float(d.z & 0xffff0000u);
-  o[6] = __uint_as_float(d.w << 16); o[7] = __uint_as_float(d.w & 0xffff0000u);
-}
 template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E]) {  // (NaN: passed over)
   float m = -INFINITY;
 #pragma unroll
@@ -146,29 +155,30 @@ __device__ __forceinline__ uint64_t fixed_weight(float x, float m, float c) {
   return x == m ? 1ull << 40 : (uint64_t)(__builtin_amdgcn_exp2f((x - m) * c) * 0x1p40f);
 }
 
-// The largest multiple B of 2^lo with at least K of the workgroup's keys k[R] >= B (0: there are fewer), two bits a round.
-template <int NT, int R, typename Key> __device__ __forceinline__ Key kth_bound(const Key (&k)[R], int K, int hi, int lo, int (*counts)[48]) {
+// The largest multiple B of 2^lo with at least K of the workgroup's keys k[r], r < used, at B or above (0: there are fewer), two
+// bits a round; a wave's three counts share a word.
+template <int NT, int R, typename Key>
+__device__ __forceinline__ Key kth_bound(const Key (&k)[R], int used, int K, int hi, int lo, uint64_t (*counts)[16]) {
   constexpr int NW = NT / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Key bound = 0;
   for (int b = hi; b >= lo; b -= 2) {
-    int cnt[3] = {0, 0, 0};
+    uint64_t cnt = 0;
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
+    for (int g = 0; g < R; ++g) {
+      if (g >= used) break;
 #pragma unroll
-      for (int g = 0; g < R; ++g) cnt[i] += __popcll(__ballot(k[g] >= (bound | ((Key)(i + 1) << b))));
-    if (NW > 1) {  // (two buffers: a round's counts are read while the next round's are written)
-      int* w = counts[(b >> 1) & 1];
-      if (lane < 3) w[wave * 3 + lane] = lane == 0 ? cnt[0] : lane == 1 ? cnt[1] : cnt[2];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        cnt[i] = 0;
-#pragma unroll
-        for (int j = 0; j < NW; ++j) cnt[i] += w[j * 3 + i];
-      }
+      for (int i = 0; i < 3; ++i) cnt += (uint64_t)__popcll(__ballot(k[g] >= (bound | ((Key)(i + 1) << b)))) << (20 * i);
     }
-    bound |= (Key)(cnt[2] >= K ? 3 : cnt[1] >= K ? 2 : cnt[0] >= K ? 1 : 0) << b;
+    if (NW > 1) {  // (two buffers: a round's counts are read while the next round's are written)
+      uint64_t* w = counts[(b >> 1) & 1];
+      if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = cnt;
+      __syncthreads();
+      cnt = 0;
+#pragma unroll
+      for (int j = 0; j < NW; ++j) cnt += w[j];
+    }
+    const int c1 = (int)cnt & 0xfffff, c2 = (int)(cnt >> 20) & 0xfffff, c3 = (int)(cnt >> 40);
+    bound |= (Key)(c3 >= K ? 3 : c2 >= K ? 2 : c1 >= K ? 1 : 0) << b;
   }
   return bound;
 }
@@ -177,11 +187,11 @@ template <int NT> struct SegLds {
   uint64_t wave[16];
   static constexpr int STAGE = NT == 64 ? 256 : 512;  // vectors that may hold an entry above the bound
   static constexpr int LIST = NT == 64 ? 512 : 2048;  // keys (a power of two of at least MAX_CAP)
-  uint64_t list[LIST];
+  __align__(16) uint64_t list[LIST];
   uint4 vec[STAGE];
   int at[STAGE];
   uint32_t n_vec, n;
-  int counts[2][48];
+  uint64_t counts[2][16];
   float red[16];
 };
 struct SegHead {      // what a segment leaves for the merge
@@ -256,7 +266,7 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
 #pragma unroll
   for (int g = 0; g < 4; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
   if (threadIdx.x == 0) l.n_vec = 0, l.n = 0;
-  const uint32_t bound = kth_bound<NT>(mk, K, 30, 16, l.counts);
+  const uint32_t bound = kth_bound<NT>(mk, 4, K, 30, 16, l.counts);
   const float thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
   rest = {-FLT_MAX, 0.f};
   __syncthreads();
@@ -349,6 +359,21 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
 
 // list[0..n) in LDS, largest first; at least P = the next power of two of room
 template <int NT> __device__ __forceinline__ void sort_keys(uint64_t* list, int n) {
+  if (n <= NT && n <= 512) {  // few: each key's rank by counting, two barriers instead of one per step of a network
+    const uint64_t mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+    if ((n & 1) && threadIdx.x == 0) list[n] = 0;
+    __syncthreads();
+    int rank = 0;
+    if ((int)threadIdx.x < n)
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
+        rank += (two.x > mine) + (two.y > mine);
+      }
+    __syncthreads();
+    if ((int)threadIdx.x < n) list[rank] = mine;
+    __syncthreads();
+    return;
+  }
   int P = 1;
   while (P < n) P <<= 1;
   for (int i = n + threadIdx.x; i < P; i += NT) list[i] = 0;
@@ -461,7 +486,13 @@ template <int NT> struct RowKeys {
   // of 2^-40 of the largest.
   template <typename L> __device__ __forceinline__ int first(int K, int room, uint64_t* list, float c, L& l) {
     uint64_t bound = 0;
-    if (n > 2 * K) bound = kth_bound<NT>(k, K, 62, 48, l.counts);
+    const int used = (n + NT - 1) / NT;
+    if (n > 2 * K) {  // by the upper half of the values' bits, nearly always enough
+      uint32_t hi[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) hi[r] = (uint32_t)(k[r] >> 32);
+      bound = (uint64_t)kth_bound<NT>(hi, used, K, 30, 16, l.counts) << 32;
+    }
     for (int round = 0;; ++round) {
       int m = 0;
       uint64_t most = 0;
@@ -472,7 +503,7 @@ template <int NT> struct RowKeys {
       }
       m = block_all<NT>(m, reinterpret_cast<int*>(l.red), [](int a, int b) { return a + b; });
       if (m > room && round == 0) {
-        bound = kth_bound<NT>(k, K, 62, 0, l.counts);
+        bound = kth_bound<NT>(k, used, K, 62, 0, l.counts);
         continue;
       }
       if (bound) {
@@ -499,10 +530,10 @@ template <int NT> struct RowKeys {
 };
 
 struct MergeLds {
-  uint64_t list[2 * MAX_SEG_K], wave[16];
+  __align__(16) uint64_t list[2 * MAX_SEG_K];
+  uint64_t wave[16], counts[2][16];
   float red[16];
   uint32_t n, ends[66];
-  int counts[2][48];
 };
 
 template <typename T, int NT>
@@ -564,16 +595,18 @@ constexpr double MASS_ONE = 1099511627776.0;  // 2^40: weights are at most 1, th
 __device__ __constant__ const int SEL_SHIFT[6] = {53, 42, 32, 21, 10, 0};
 __device__ __constant__ const int SEL_BITS[6] = {11, 11, 10, 11, 11, 10};
 
+struct PackedEntry { float x; int i; };
 template <int NT> struct RowLds {
+  __align__(16) uint64_t list[POOL];
   union {
-    struct { uint64_t mass[BINS]; uint32_t count[BINS]; } h;
-    uint64_t list[POOL];
+    uint64_t mass[BINS];
+    PackedEntry pack[NT / 64 * 512];
   };
-  uint64_t wave[16];
+  uint64_t wave[16], counts[2][16];
   uint64_t cut_before;
   double redd[16];
   float red[16];
-  int cut, counts[2][48];
+  int cut;
   uint32_t n, ends[66];
 };
 
@@ -611,187 +644,418 @@ template <int NT, typename L, typename F> __device__ __forceinline__ CutAt find_
   return l.cut < n ? CutAt{l.cut, l.cut_before} : CutAt{n, all};
 }
 
-// Entries of a row with key >= floor: the largest key B such that those >= B number `need` (BY_MASS: weigh at least the share
-// `part` of all of them).  First 2048 bins of equal width in m - x (an entry's bin never decreases with m - x, so bins are ranges
-// of the order), then the bin with the boundary is listed and sorted; one that does not fit the list (many equal values, entries
-// far below the largest) is divided by the key's bits first.
-template <typename T, int NT, bool BY_MASS, typename W>
-__device__ uint64_t boundary(const T* row, int V, float m, float bins_per_unit, uint64_t floor, int need_count, double part, W weight,
-                             RowLds<NT>& l) {
-  auto bin_of = [&](float x) {
-    x = fmaxf(x, -INFINITY);
-    const float d = (m - x) * bins_per_unit;
-    return d < (float)(BINS - 1) ? (int)d : x == m ? 0 : BINS - 1;
-  };
-  auto fixed = [&](float x) { return (uint64_t)(weight(x) * MASS_ONE); };
-  uint64_t need = need_count, prefix = 0, mask = 0;
-  int bin = -1, in_bin = 0;
-  for (int d = -1; d < 6; ++d) {
-    const int shift = d < 0 ? 0 : SEL_SHIFT[d], bins = d < 0 ? BINS : 1 << SEL_BITS[d];
-    __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += NT) l.h.count[i] = 0, l.h.mass[i] = 0;
-    __syncthreads();
-    each<T, NT>(row, V, [&](int i, float x) {
-      const uint64_t k = entry_key(x, i);
-      if (k < floor) return;
-      int b = bin_of(x);
-      if (d >= 0) {
-        if (b != bin || (k & mask) != prefix) return;
-        b = bins - 1 - ((int)(k >> shift) & (bins - 1));
-      }
-      atomicAdd(&l.h.count[b], 1u);
-      if (BY_MASS) atomicAdd((unsigned long long*)&l.h.mass[b], (unsigned long long)fixed(x));
-    });
-    __syncthreads();
-    auto get = [&](int i) { return BY_MASS ? l.h.mass[i] : (uint64_t)l.h.count[i]; };
-    if (BY_MASS && d < 0) {
-      const CutAt all = find_cut<NT>(bins, ~0ull, l, get);
-      const double want = ceil(part * (double)all.before);
-      need = want < 1.0 ? 1 : (uint64_t)want < all.before ? (uint64_t)want : all.before;
-    }
-    const CutAt c = find_cut<NT>(bins, need, l, get);
-    const int b = c.i < bins ? c.i : bins - 1;  // (fewer than asked for: down to the last)
-    in_bin = l.h.count[b];
-    need = c.i < bins ? need - c.before : ~0ull;
-    if (d < 0) bin = b;
-    else {
-      prefix |= (uint64_t)(bins - 1 - b) << shift;
-      mask |= (uint64_t)(bins - 1) << shift;
-    }
-    if (in_bin <= POOL) break;
+// Bins of equal width in m - x, m the largest entry: an entry's bin never decreases with m - x, so bins are ranges of the order.
+struct Bins {
+  float m, per;
+  __device__ __forceinline__ Bins(float largest, float per_unit) : m(fminf(largest, FLT_MAX)), per(per_unit) {}
+  __device__ __forceinline__ int of(float x) const { return (int)fminf((m - fminf(x, FLT_MAX)) * per, (float)(BINS - 1)); }
+};
+// Where a filter's kept entries end: at a key of bin `bin` whose digits under `mask` are `prefix`; n such entries are in the list,
+// sorted, of which the first `kept` are kept, down to key B.
+struct Border {
+  int bin, n, kept;
+  float lo, hi;  // the bin's values
+  uint64_t prefix, mask, B;
+};
+// The smallest value whose bin is at most b (b < 0: none, NaN), by bisection over the values' keys.
+__device__ __forceinline__ float lowest_of(const Bins& bins, int b) {
+  uint32_t lo = 0x007fffffu, hi = 0xff800000u;  // -inf .. +inf
+  if (b < 0) return NAN;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (bins.of(key_value(mid)) <= b) hi = mid;
+    else lo = mid + 1;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) l.n = 0;
-  __syncthreads();
-  each<T, NT>(row, V, [&](int i, float x) {
-    const uint64_t k = entry_key(x, i);
-    if (k >= floor && bin_of(x) == bin && (k & mask) == prefix) l.list[atomicAdd(&l.n, 1u)] = k;
-  });
-  __syncthreads();
-  const int n = l.n;
-  if (n == 0) return floor;
-  sort_keys<NT>(l.list, n);
-  const CutAt c = find_cut<NT>(n, need, l, [&](int i) { return BY_MASS ? fixed(key_value((uint32_t)(l.list[i] >> 32))) : (uint64_t)1; });
-  return l.list[c.i < n ? c.i : n - 1];
+  return key_value(lo);
 }
 
-// The race over the entries that keep(x, key) admits, of the whole row: reads logits and, for those, noise.
+__device__ __forceinline__ uint64_t fixed(double w) {  // w <= 1 in multiples of 2^-40
+  return (uint64_t)(__double_as_longlong(w + 4096.0) - 0x40b0000000000000ll);  // (in 4096..8192 one unit in the last place is 2^-40)
+}
+
+// The border after which `need_count` entries (by_mass: the share `part` of the mass) of those with key >= floor lie.  2048 bins are
+// counted (weighed) first; the border's bin is listed by gather(at) and sorted.  One that does not fit the list (many equal values,
+// entries far below the largest) is divided by the key's bits first.
+template <typename T, int NT, typename W, typename G>
+__device__ __forceinline__ Border border(const T* row, int V, Bins bins, uint64_t floor, bool by_mass, int need_count, double part, W weight,
+                                         RowLds<NT>& l, G gather) {
+  uint32_t* count = reinterpret_cast<uint32_t*>(l.mass);
+  const float floor_x = floor ? key_value((uint32_t)(floor >> 32)) : -INFINITY;
+  auto below = [&](float x, int i) { return x <= floor_x && (x < floor_x || entry_key(x, i) < floor); };
+  uint64_t need = need_count;
+  Border at = {0, 0, 0, INFINITY, -INFINITY, 0, 0, 0};
+#pragma unroll 1
+  for (int d = -1;; ++d) {
+    if (need_count >= 0) {
+      const int shift = d < 0 ? 0 : SEL_SHIFT[d], n_bins = d < 0 ? BINS : 1 << SEL_BITS[d];
+      __syncthreads();
+      for (int i = threadIdx.x; i < n_bins; i += NT) l.mass[i] = 0;
+      __syncthreads();
+      auto put = [&](int b, float x) {
+        if (by_mass) atomicAdd((unsigned long long*)&l.mass[b], (unsigned long long)fixed(weight(x)));
+        else atomicAdd(&count[b], 1u);
+      };
+      if (d < 0)
+        each<T, NT>(row, V, [&](int i, float x) {
+          x = fmaxf(x, -INFINITY);
+          if (!below(x, i)) put(bins.of(x), x);
+        });
+      else
+        for (int i = threadIdx.x; i < V; i += NT) {
+          const float x = fmaxf(to_f32<T>(row[i]), -INFINITY);
+          const uint64_t k = entry_key(x, i);
+          if (k >= floor && bins.of(x) == at.bin && (k & at.mask) == at.prefix) put(n_bins - 1 - ((int)(k >> shift) & (n_bins - 1)), x);
+        }
+      __syncthreads();
+      auto get = [&](int i) { return by_mass ? l.mass[i] : (uint64_t)count[i]; };
+      if (by_mass && d < 0) {
+        const double all = (double)find_cut<NT>(n_bins, ~0ull, l, get).before;
+        need = (uint64_t)fmin(fmax(ceil(part * all), 1.0), all);
+      }
+      const CutAt c = find_cut<NT>(n_bins, need, l, get);
+      const int b = min(c.i, n_bins - 1);  // (fewer than asked for: down to the last)
+      need = c.i < n_bins ? need - c.before : ~0ull;
+      if (d < 0) {
+        at.bin = b;
+        at.lo = lowest_of(bins, b);
+        const float next = lowest_of(bins, b - 1);
+        at.hi = b > 0 ? key_value(value_key(next) - 1) : INFINITY;
+      } else {
+        at.prefix |= (uint64_t)(n_bins - 1 - b) << shift;
+        at.mask |= (uint64_t)(n_bins - 1) << shift;
+      }
+    } else {
+      at.bin = BINS;  // (no border to look for: every entry above -inf is before it, lo > hi)
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) l.n = 0;
+    __syncthreads();
+    gather(at);
+    __syncthreads();
+    if (l.n <= POOL || d == 5) break;
+  }
+  at.n = l.n;
+  if (at.n == 0) return at;
+  sort_keys<NT>(l.list, at.n);
+  const CutAt c = find_cut<NT>(at.n, need, l, [&](int i) { return by_mass ? fixed(weight(key_value((uint32_t)(l.list[i] >> 32)))) : (uint64_t)1; });
+  at.kept = min(c.i + 1, at.n);
+  at.B = l.list[at.kept - 1];
+  return at;
+}
+
+// exp((x - m) / temperature) in 64 bits (scale = log2(e) / temperature); the largest entry has 1, an infinite one too.
+struct Weight {
+  float m;
+  double scale;
+  __device__ __forceinline__ double operator()(float x) const { return x == m ? 1.0 : exp2_f64(((double)x - (double)m) * scale); }
+};
+
+// The entries of the border's bin into the list.
+template <typename T, int NT>
+__device__ __forceinline__ void gather_bin(const T* row, int V, uint64_t floor, const Border& at, RowLds<NT>& l) {
+  each<T, NT>(row, V, [&](int i, float x) {
+    x = fmaxf(x, -INFINITY);
+    if (x < at.lo || x > at.hi) return;
+    const uint64_t k = entry_key(x, i);
+    if (k < floor || (k & at.mask) != at.prefix) return;
+    const uint32_t p = atomicAdd(&l.n, 1u);
+    if (p < POOL) l.list[p] = k;
+  });
+}
+
+// A thread's share of the race: the best w / noise, in 64 bits where an fp32 quotient (off by less than 2^-20) says it can win.
 struct Race {
-  double best, total;
-  uint64_t at;
-  __device__ __forceinline__ void add(double w, float q, uint32_t i) {
+  double best = -1.0, total = 0.0;
+  float screen = -1.f, x = 0.f;
+  uint64_t at = ~0ull;
+  __device__ __forceinline__ void add(double w, float value, float q, uint32_t i) {
     total += w;
-    const double r = w > 0.0 ? w / (double)q : 0.0;
-    if (r > best || (r == best && i < at)) { best = r; at = i; }
+    const float r = (float)w * __builtin_amdgcn_rcpf(q);
+    if (r < screen) return;
+    const double e = w > 0.0 ? w / (double)q : 0.0;
+    if (e > best || (e == best && i < at)) {
+      best = e;
+      at = i;
+      x = value;
+      screen = (float)e < FLT_MAX ? (float)e * (1.f - 0x1p-16f) : FLT_MAX;
+    }
   }
 };
 
+struct ListLds {
+  __align__(16) uint64_t list[POOL];
+  uint64_t mass[POOL];
+  uint64_t wave[16], counts[2][16];
+  double redd[16];
+  float red[16];
+  int cut;
+  uint32_t n, ends[66];
+};
+
+// Ends a row's race over the whole workgroup or its first wave: token and probability.
+template <int NT, typename L, typename W>
+__device__ __forceinline__ void finish(const Race& race, double kept_mass, uint32_t arg, W weight, L& l, int64_t* pred,
+                                       float* conf) {
+  const double best = block_all<NT>(race.best, l.redd, [](double a, double b) { return fmax(a, b); });
+  const uint64_t mine = race.best == best ? race.at : (uint64_t)~0ull;
+  const uint64_t at = block_all<NT>(mine, l.wave, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  if (at == ~0ull) {  // (noise without a usable draw)
+    if (threadIdx.x == 0) *pred = arg, *conf = (float)(1.0 / kept_mass);
+  } else if (mine == at) {
+    *pred = (int64_t)at;
+    *conf = (float)(weight(race.x) / kept_mass);
+  }
+}
+
+// From the segments' lists, if the end of the kept entries lies within them.  A row where it does not is left to
+// sample_row_kernel: pred = -2 - (index of its largest entry), conf = that entry.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void sample_row_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
-                                                        int64_t ld_noise, int V, SampleArgs args, int nseg, int cap,
-                                                        const SegHead* __restrict__ heads, const uint64_t* __restrict__ lists,
-                                                        int64_t* __restrict__ pred, float* __restrict__ conf) {
+__global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict__ noise, int64_t ld_noise, int V, SampleArgs args,
+                                                         int nseg, int cap, const SegHead* __restrict__ heads,
+                                                         const uint64_t* __restrict__ lists, int64_t* __restrict__ pred,
+                                                         float* __restrict__ conf) {
+  __shared__ ListLds l;
+  const int64_t t = blockIdx.x;
+  const float* q = noise + t * ld_noise;
+  const RowFilter f = args.row(t);
+  const bool greedy = !(f.temperature > 0.f);
+  const double scale = LOG2E / (double)f.temperature;
+  const float c = greedy ? 0.f : (float)scale;
+  RowKeys<NT> rk;
+  rk.load(heads, lists, t, nseg, cap, l.ends);
+  const int want = f.top_k > 0 && f.top_k < POOL / 4 ? f.top_k : 192;  // (what 256 threads sort by counting)
+  const int n = rk.first(want, POOL, l.list, c, l);
+  if (n == 0) {
+    if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
+    return;
+  }
+  sort_keys<NT>(l.list, n);
+  const float m = key_value((uint32_t)(l.list[0] >> 32));
+  const uint32_t arg = ~(uint32_t)l.list[0];
+  if (greedy) {
+    if (threadIdx.x == 0) pred[t] = arg, conf[t] = 1.f;
+    return;
+  }
+  const Weight weight = {m, scale};
+  // l.mass[i]: the weights of the entries 0..i; nv, na: entries down to which the list is complete / that min_p leaves
+  const int per = (n + NT - 1) / NT, a0 = min((int)threadIdx.x * per, n), a1 = min(a0 + per, n);
+  uint64_t sum = 0;
+  int both = 0;
+  for (int i = a0; i < a1; ++i) {
+    const uint64_t k = l.list[i];
+    const float x = key_value((uint32_t)(k >> 32));
+    sum += fixed(weight(x));
+    l.mass[i] = sum;
+    both += (k >= rk.level) + (f.above_min_p(x, m) << 16);
+  }
+  uint64_t upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t v = __shfl_up(upto, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) upto += v;
+  }
+  float out_m = rk.rest.m, out_s = rk.rest.s;  // (the segments' sums: in the first wave's lanes)
+  if (threadIdx.x < 64) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const ExpSum j = exp_sum_join({out_m, out_s}, {__shfl_xor(out_m, o, 64), __shfl_xor(out_s, o, 64)}, c);
+      out_m = j.m; out_s = j.s;
+    }
+    if (threadIdx.x == 0) l.red[0] = out_m, l.red[1] = out_s;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) both += __shfl_xor(both, o, 64);
+  if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x >> 6] = upto, l.counts[0][threadIdx.x >> 6] = (uint64_t)(uint32_t)both;
+  if (threadIdx.x == 0) l.cut = n;
+  __syncthreads();
+  uint64_t off = upto - sum;
+  int nv = 0, na = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) off += l.wave[w];
+    nv += (int)l.counts[0][w] & 0xffff;
+    na += (int)l.counts[0][w] >> 16;
+  }
+  for (int i = a0; i < a1; ++i) l.mass[i] += off;
+  const double left = (double)l.red[1] * (double)__builtin_amdgcn_exp2f((l.red[0] - m) * c);  // the mass outside the list
+  __syncthreads();
+  const bool whole = rk.level == 0;  // (every entry above -inf is in the list)
+  const int nk = f.top_k > 0 && f.top_k < V ? f.top_k : V;
+  const bool nk_in = nk <= nv || whole;
+  int keep = nk_in ? min(nk, nv) : V;
+  bool sure = true;
+  if (f.top_p < 1.f) {
+    if (nk_in || nk == V) {
+      // the mass outside: fp32 sums of up to 2^7 terms per thread and a tree, their relative error below 2^-15
+      const double rest = nk_in ? 0.0 : left * MASS_ONE, err = rest * 0x1p-15;
+      const double need = fmax(1.0, ceil((double)f.top_p * ((double)l.mass[(nk_in ? keep : n) - 1] + rest)));
+      for (int i = a0; i < a1; ++i)
+        if ((i == 0 || (double)l.mass[i - 1] < need) && (double)l.mass[i] >= need) l.cut = i;
+      __syncthreads();
+      const int at = l.cut;  // (n: beyond the list)
+      const double before = at > 0 ? (double)l.mass[min(at, nv) - 1] : 0.0;
+      if (at < nv) {
+        if (err > 0.0) sure = before < need - err && (double)l.mass[at] >= need + err;
+        keep = min(keep, at + 1);
+      } else if (!nk_in) {
+        sure = before < need - err;
+      }
+    } else {
+      sure = false;  // (the mass of the first k is not known)
+    }
+    if (m == INFINITY && !nk_in) sure = false;  // (infinite entries outside the list have no mass in it)
+  }
+  if (f.min_p > 0.f && (na < nv || whole)) keep = min(keep, na);
+  if (!sure || keep > nv) {
+    if (threadIdx.x == 0) pred[t] = -2 - (int64_t)arg, conf[t] = m;
+    return;
+  }
+  const double kept_mass = (double)l.mass[keep - 1] * 0x1p-40;
+  Race race;
+  for (int i = threadIdx.x; i < keep; i += NT) {
+    const uint32_t at = ~(uint32_t)l.list[i];
+    const float x = key_value((uint32_t)(l.list[i] >> 32));
+    race.add(weight(x), x, q[at], at);
+  }
+  if (keep <= 64) {  // the first wave's alone
+    if (threadIdx.x < 64) finish<64>(race, kept_mass, arg, weight, l, pred + t, conf + t);
+  } else {
+    finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
+  }
+}
+
+// From the whole row: every row (all), or those sample_list_kernel left.  The border of top-k, then of top-p among those, then
+// the race.  One workgroup a row, bound by the 64-bit exponentials of its CU.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
+                                                        int64_t ld_noise, int V, SampleArgs args, bool all, int64_t* __restrict__ pred,
+                                                        float* __restrict__ conf) {
   __shared__ RowLds<NT> l;
   const int64_t t = blockIdx.x;
   const T* row = logits + t * ld;
   const float* q = noise + t * ld_noise;
   const RowFilter f = args.row(t);
-  const bool greedy = !(f.temperature > 0.f);
-  const double scale = LOG2E / (double)f.temperature;
-  uint64_t top;  // the row's first key
-  Race race = {-1.0, 0.0, ~0ull};
   float m;
-  auto weight = [&](float x) { return x == m ? 1.0 : exp2_f64(((double)x - (double)m) * scale); };
-  bool done = false;
-  if (nseg) {
-    // from the segments' lists, if the end of the kept entries lies within them
-    RowKeys<NT> rk;
-    rk.load(heads, lists, t, nseg, cap, l.ends);
-    const float c = greedy ? 0.f : (float)scale;
-    const int want = f.top_k > 0 && f.top_k < POOL / 4 ? f.top_k : POOL / 8;
-    const int n = rk.first(want, POOL, l.list, c, l);
-    if (n == 0) {
-      if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
-      return;
-    }
-    sort_keys<NT>(l.list, n);
-    top = l.list[0];
-    m = key_value((uint32_t)(top >> 32));
-    if (!greedy && m < INFINITY) {
-      const ExpSum out = block_exp_sum<NT>(rk.rest, c, l.red);
-      const double left = (double)out.s * (double)__builtin_amdgcn_exp2f((out.m - m) * c);  // the mass outside the list
-      const CutAt known = find_cut<NT>(n, ~0ull, l, [&](int i) { return (uint64_t)(l.list[i] >= rk.level); });
-      const int nv = (int)known.before;           // the list is complete that far
-      const bool whole = rk.level == 0;           // (every entry above -inf)
-      const int nk = f.top_k > 0 && f.top_k < V ? f.top_k : V;
-      const bool nk_in = nk <= nv || whole;
-      int keep = nk_in ? (nk < nv ? nk : nv) : V;
-      bool sure = true;
-      auto mass = [&](int i) { return (uint64_t)(weight(key_value((uint32_t)(l.list[i] >> 32))) * MASS_ONE); };
-      if (f.top_p < 1.f) {
-        if (nk_in || nk == V) {
-          const int among = nk_in ? keep : n;
-          const CutAt all = find_cut<NT>(among, ~0ull, l, mass);
-          // fp32 sums of up to 2^7 terms per thread and a tree: their relative error stays below 2^-15
-          const double rest = nk_in ? 0.0 : left * MASS_ONE, W = (double)all.before + rest, err = rest * 0x1p-15;
-          const double need = ceil((double)f.top_p * W);
-          const CutAt at = find_cut<NT>(nv, need < 1.0 ? 1 : (uint64_t)need, l, mass);
-          const double lo = need - err, hi = need + err;
-          if (at.i < nv) {
-            if (err > 0.0 && !((double)at.before < lo && (double)at.before + (double)mass(at.i) >= hi)) sure = false;
-            keep = keep < at.i + 1 ? keep : at.i + 1;
-          } else if (!nk_in && (double)at.before >= lo) {
-            sure = false;
-          }
-        } else {
-          sure = false;  // (the mass of the first k is not known)
-        }
-      }
-      if (f.min_p > 0.f) {
-        const CutAt above = find_cut<NT>(nv, ~0ull, l, [&](int i) { return (uint64_t)f.above_min_p(key_value((uint32_t)(l.list[i] >> 32)), m); });
-        const int na = (int)above.before;
-        if (na < nv || whole) keep = keep < na ? keep : na;
-      }
-      done = sure && keep <= nv;
-      if (done)
-        for (int i = threadIdx.x; i < keep; i += NT) {
-          const uint32_t at = ~(uint32_t)l.list[i];
-          race.add(weight(key_value((uint32_t)(l.list[i] >> 32))), q[at], at);
-        }
-    }
-  } else {
-    top = 0;
-    each<T, NT>(row, V, [&](int i, float x) { const uint64_t e = entry_key(x, i); top = e > top ? e : top; });
+  uint32_t arg;
+  if (all) {
+    float most = -INFINITY;
+    int first = -1;
+    each<T, NT>(row, V, [&](int i, float x) {
+      if (x > most || (first < 0 && x == most)) most = x, first = i;
+    });
+    uint64_t top = first < 0 ? entry_key(-INFINITY, ~0u) : entry_key(most, first);
     top = block_all<NT>(top, l.wave, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
     m = key_value((uint32_t)(top >> 32));
-    if (m == -INFINITY) {
-      if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
+    arg = ~(uint32_t)top;
+    if (m == -INFINITY || !(f.temperature > 0.f)) {
+      if (threadIdx.x == 0) pred[t] = m == -INFINITY ? -1 : (int64_t)arg, conf[t] = m == -INFINITY ? 0.f : 1.f;
       return;
     }
+  } else {
+    const int64_t left = pred[t];
+    if (left > -2) return;
+    arg = (uint32_t)(-2 - left);
+    m = conf[t];
+    __syncthreads();
   }
-  const uint32_t arg = ~(uint32_t)top;
-  if (greedy) {
-    if (threadIdx.x == 0) pred[t] = arg, conf[t] = 1.f;
-    return;
+  const Weight weight = {m, LOG2E / (double)f.temperature};
+  const Bins bins(m, (float)BINS / fminf(40.f * f.temperature, 32.f));
+  const bool by_k = f.top_k > 0 && f.top_k < V, by_p = f.top_p < 1.f;
+  // min_p as the smallest value it leaves; -inf and NaN never race
+  float least = -FLT_MAX;
+  if (f.min_p > 0.f) {
+    const double x = (double)m + (double)f.temperature * log((double)fminf(f.min_p, 1.f));
+    least = fmaxf((float)x, -FLT_MAX);
+    if ((double)least < x) least = key_value(value_key(least) + 1);
+    least = fminf(least, m);
   }
-  if (!done) {
-    // from the whole row: the boundary key of each filter, then the race
-    const float span = fminf(40.f * f.temperature, 32.f), per = (float)BINS / span;
-    uint64_t B = 0;
-    if (f.top_k > 0 && f.top_k < V) B = boundary<T, NT, false>(row, V, m, per, 0, f.top_k, 0.0, weight, l);
-    if (f.top_p < 1.f) B = boundary<T, NT, true>(row, V, m, per, B, 0, (double)f.top_p, weight, l);
-    each<T, NT>(row, V, [&](int i, float x) {
-      if (x > -INFINITY && entry_key(x, i) >= B && f.above_min_p(x, m)) race.add(weight(x), q[i], i);
-    });
+  Race race;
+  // The entries before the border race, those at it go to the list.  A wave first packs a vector's racing entries (each wave its
+  // own part of l.pack), so that a few among many do not take the 64-bit work of all; four vectors per thread are on their way
+  // meanwhile, and noise is read for the racing entries alone.
+  auto sweep = [&](uint64_t floor, const Border& at) {
+    constexpr int E = 16 / (int)sizeof(T);
+    PackedEntry* pack = l.pack + (threadIdx.x >> 6) * 512;
+    race = Race();
+    int n = 0;
+    auto look = [&](float x, int i) {  // (by whole waves)
+      bool go = x >= least;
+      if (!(x > at.hi)) {
+        const bool near = x >= at.lo;
+        go = go && near;
+        if (near) {
+          const uint64_t k = entry_key(x, i), digits = k & at.mask;
+          go = go && k >= floor && digits > at.prefix;
+          if (k >= floor && digits == at.prefix) {
+            const uint32_t p = atomicAdd(&l.n, 1u);
+            if (p < POOL) l.list[p] = k;
+          }
+        }
+      }
+      const uint64_t lanes = __ballot(go);
+      if (go) pack[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = {x, i};
+      n += __popcll(lanes);
+    };
+    auto run = [&]() {
+      if (n == 0) return;
+      race.screen = wave_max(race.screen);  // (alone, some lane of a wave nearly always has a new best of its own to divide for)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+      for (int j = threadIdx.x & 63; j < n; j += 256) {
+        PackedEntry e[4];
+        float z[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          e[u] = pack[min(j + 64 * u, n - 1)];
+          z[u] = q[e[u].i];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (j + 64 * u < n) race.add(weight(e[u].x), e[u].x, z[u], e[u].i);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      n = 0;
+    };
+    int head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
+    if (head > V) head = V;
+    const int nv = (V - head) / E, tail = head + nv * E;
+    const uint4* vec = reinterpret_cast<const uint4*>(row + head);
+    uint4 d[4] = {};
+    if (nv)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) d[u] = vec[min((int)threadIdx.x + u * NT, nv - 1)];
+#pragma unroll 1
+    for (int r0 = 0; r0 < nv; r0 += NT) {
+      const int v = r0 + threadIdx.x;
+      float o[E];
+      unpack(d[0], o);
+      d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
+      d[3] = vec[min(v + 4 * NT, nv - 1)];
+#pragma unroll
+      for (int e = 0; e < E; ++e) look(v < nv ? o[e] : NAN, head + v * E + e);
+      run();
+    }
+    const int end = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;  // (both ends: less than 2 E entries)
+    look(end < V && (int)threadIdx.x < head + V - tail ? to_f32<T>(row[end]) : NAN, end);
+    run();
+  };
+  Border at = {BINS, 0, 0, INFINITY, -INFINITY, 0, 0, 0};
+#pragma unroll 1
+  for (int last = by_k && by_p ? 0 : 1; last < 2; ++last) {  // one copy of the code for both filters
+    const uint64_t floor = at.B;
+    auto gather = [&](const Border& a) {
+      if (last) sweep(floor, a);
+      else gather_bin<T, NT>(row, V, floor, a, l);
+    };
+    at = border<T, NT>(row, V, bins, floor, last && by_p, by_k || by_p ? f.top_k : -1, (double)f.top_p, weight, l, gather);
   }
-  const double total = block_sum<NT>(race.total, l.redd);
-  const double best = block_all<NT>(race.best, l.redd, [](double a, double b) { return a > b ? a : b; });
-  const uint64_t at = block_all<NT>(race.best == best ? race.at : (uint64_t)~0ull, l.wave, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
-  if (threadIdx.x == 0) {
-    const uint32_t i = at == ~0ull ? arg : (uint32_t)at;
-    pred[t] = i;
-    conf[t] = (float)(weight(to_f32<T>(row[i])) / total);
+  for (int i = threadIdx.x; i < at.kept; i += NT) {
+    const float x = key_value((uint32_t)(l.list[i] >> 32));
+    const uint32_t j = ~(uint32_t)l.list[i];
+    if (x >= least) race.add(weight(x), x, q[j], j);
   }
+  const double kept_mass = block_sum<NT>(race.total, l.redd);
+  finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
 }
 
 template <typename T, int NT, int VPT>
@@ -825,7 +1089,9 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, i
   float m = -INFINITY;
   each<T, NT>(row, V, [&](int, float x) { m = fmaxf(m, x); });
   m = block_max<NT>(m, l.red);
-  const uint64_t B = boundary<T, NT, false>(row, V, m, BINS / 32.f, 0, K, 0.0, [](float) { return 0.0; }, l);
+  const Bins bins(m, BINS / 32.f);
+  const uint64_t B = border<T, NT>(row, V, bins, 0, false, K, 0.0, [](float) { return 0.0; }, l,
+                                              [&](const Border& at) { gather_bin<T, NT>(row, V, 0, at, l); }).B;
   __syncthreads();
   if (threadIdx.x == 0) l.n = 0;
   __syncthreads();
@@ -1254,11 +1520,11 @@ int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int 
       hipLaunchKernelGGL((sample_segment_kernel<T, 256, 4>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
     else if (cut.nt)
       hipLaunchKernelGGL((sample_segment_kernel<T, 256, 16>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
-    // one row per CU at most: the whole CU for a row
-    if (n <= 256)
-      hipLaunchKernelGGL((sample_row_kernel<T, 1024>), dim3(n), dim3(1024), 0, s, x, ld, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
-    else
-      hipLaunchKernelGGL((sample_row_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
+    if (cut.nt)
+      hipLaunchKernelGGL((sample_list_kernel<T, 256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
+    const bool settled = cut.nt && !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K;  // the lists hold the first k
+    if (!settled)
+      hipLaunchKernelGGL((sample_row_kernel<T, 512>), dim3(n), dim3(512), 0, s, x, ld, q, ldq, V, a, cut.nt == 0, pred, conf);
   }
   return check_launch();
 }
