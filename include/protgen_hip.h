@@ -354,7 +354,7 @@ int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* n
  * dlogits = dloss[t] d loss[t] / d logits (activation type, every entry of every row; dloss NULL = 1);
  * pg_distill_loss_grad is both in one call, for updates that know the weights beforehand. */
 int64_t pg_distill_stash_floats(void);
-int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k);
+int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k, int with_grad /* 1: for pg_distill_loss_grad */);
 int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
                    const float* rest, const float* weights, float temperature, float* loss, float* stash, void* workspace,
                    int64_t workspace_bytes, void* stream);

@@ -136,12 +136,12 @@ template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E]) {
   for (int e = 0; e < E; ++e) m = fmaxf(m, o[e]);
   return m;
 }
-// The exponentials of E entries of which vm is the largest, NaN as -inf, with one rescaling for all of them.
-template <int E> __device__ __forceinline__ void exp_sum_vec(ExpSum& a, const float (&o)[E], float vm, float c) {
+// The exponentials of E entries of which vm is the largest, with one rescaling for all of them.  NaN as -inf, or (KEEP_NAN) kept.
+template <int E, bool KEEP_NAN = false> __device__ __forceinline__ void exp_sum_vec(ExpSum& a, const float (&o)[E], float vm, float c) {
   const float m = fmaxf(a.m, vm);
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((fmaxf(o[e], -INFINITY) - m) * c);
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(((KEEP_NAN ? o[e] : fmaxf(o[e], -INFINITY)) - m) * c);
   a.s = a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + s;
   a.m = m;
 }
@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, i
 //   student probability of entry v:  exp2((x_v - [0]) c) [1]
 //   gradient (before tau, weight and upstream) of an entry outside the teacher's list:  [3] exp2((x_v - [2]) c)
 //   teacher probability of entry e:  exp2((v_e - [4]) c) [5]
-//   [6]: 1 if the row counts
+//   [6]: 1 if the row counts, [7]: 1 if an id may occur twice
 constexpr int STASH = 8;
 
 struct DistillArgs {
@@ -1122,121 +1122,273 @@ template <typename T> __device__ __forceinline__ bool valid_entry(const T* value
   return (uint32_t)ids[e] < (uint32_t)V && to_f32<T>(values[e]) > -INFINITY;
 }
 
-// Is entry e the first of its id in the list?  (A list from pg_top_logits has no id twice.)
+// Is entry e the first of its id in the list?
 template <typename T> __device__ __forceinline__ bool first_of_id(const T* values, const int32_t* ids, int e, int V) {
   for (int j = 0; j < e; ++j)
     if (ids[j] == ids[e] && valid_entry(values, ids, j, V)) return false;
   return true;
 }
 
+// Segment `seg` of `nseg` of a row: its whole 16-byte vectors [v0, v1); the elements before the first vector of the row belong to
+// the first segment, those behind the last one to the last.
+template <typename T> struct Span {
+  static constexpr int E = 16 / (int)sizeof(T);
+  int head, tail, v0, v1;  // head: elements before the row's first vector; tail: first element behind its last
+  bool first, last;
+  __device__ __forceinline__ Span(const T* row, int V, int seg, int nseg) {
+    head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
+    if (head > V) head = V;
+    const int nv = (V - head) / E, per = (nv + nseg - 1) / nseg;
+    tail = head + nv * E;
+    v0 = min(seg * per, nv);
+    v1 = min(v0 + per, nv);
+    first = seg == 0;
+    last = seg == nseg - 1;
+  }
+  __device__ __forceinline__ bool owns(int i) const {
+    return i < head ? first : i >= tail ? last : i >= head + v0 * E && i < head + v1 * E;
+  }
+  // vec(o, v) over the vectors, four in flight per thread; one(i) over the odd elements
+  template <int NT, typename F, typename G> __device__ __forceinline__ void each(const T* row, int V, F vec, G one) const {
+    const uint4* p = reinterpret_cast<const uint4*>(row + head);
+    if (v0 + (int)threadIdx.x < v1) {
+      uint4 d[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) d[u] = p[min(v0 + (int)threadIdx.x + u * NT, v1 - 1)];
+#pragma unroll 1
+      for (int v = v0 + threadIdx.x; v < v1; v += NT) {
+        float o[E];
+        unpack(d[0], o);
+        d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
+        d[3] = p[min(v + 4 * NT, v1 - 1)];
+        vec(o, v);
+      }
+    }
+    if (first && (int)threadIdx.x < head) one((int)threadIdx.x);
+    if (last && tail + (int)threadIdx.x < V) one(tail + (int)threadIdx.x);
+  }
+};
+
+// Which tokens are in the teacher's list: one bit per element of a segment in LDS, a vector's bits together (a byte for bf16, half
+// of one for fp32), so that the pass over the row looks at one byte per vector.  MAX_MEMBER bits; longer rows are cut.
+constexpr int MAX_MEMBER = 1 << 17;
+
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_fwd_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
-                                                         float* __restrict__ loss, float* __restrict__ stash) {
-  extern __shared__ uint32_t member[];  // one bit per entry of the vocabulary: in the teacher's list
-  __shared__ float red[16];
-  const int64_t t = blockIdx.x;
-  float* st = stash + t * STASH;
-  const float w = a.weights ? a.weights[t] : 1.f;
-  const T* row = logits + t * ld;
-  const T* values = (const T*)a.values + t * a.K;
-  const int32_t* ids = a.ids + t * a.K;
+__device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>& sp, const T* values, const int32_t* ids, int K, bool tail,
+                                              float c, uint32_t* member, int* repeated) {
+  constexpr int E = Span<T>::E;
+  const int start = sp.head + sp.v0 * E - E;  // element of bit 0: a vector's worth before the segment, for the odd elements in front
+  if (tail) {
+    const int bits = (sp.v1 - sp.v0 + 2) * E;
+    for (int i = threadIdx.x; i < (bits + 31) / 32; i += NT) member[i] = 0;
+    if (threadIdx.x == 0) *repeated = 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < K; e += NT)
+      if (valid_entry(values, ids, e, V) && sp.owns(ids[e])) {
+        const int b = ids[e] - start;
+        if (atomicOr(&member[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) *repeated = 1;
+      }
+    __syncthreads();
+  }
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(member);
+  ExpSum o = {-FLT_MAX, 0.f};
+  sp.template each<NT>(row, V, [&](const float (&x)[E], int v) {
+    const int at = v - sp.v0 + 1;
+    const uint32_t in = tail ? (E == 8 ? bytes[at] : bytes[at >> 1] >> (at & 1) * 4 & 15) : 0;
+    if (in == 0) {
+      exp_sum_vec<E, true>(o, x, vec_max<E>(x), c);
+    } else {
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = in >> e & 1 ? -INFINITY : x[e];
+      exp_sum_vec<E, true>(o, y, vec_max<E>(y), c);
+    }
+  }, [&](int i) {
+    const int b = i - start;
+    if (!tail || !(member[b >> 5] >> (b & 31) & 1)) exp_sum_add(o, to_f32<T>(row[i]), c);
+  });
+  return o;
+}
+
+// The row's loss and stash from its sum over the tokens outside the list (tail) or over all of them.  Every thread of the
+// workgroup returns with the stash's numbers in st.
+template <typename T, int NT>
+__device__ __forceinline__ void distill_row(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
+                                            ExpSum o, bool repeated, float* red, float (&st)[STASH], float* loss) {
   const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
   const bool tail = a.rest != nullptr;
-  if (w == 0.f) {
-    if (threadIdx.x < STASH) st[threadIdx.x] = 0.f;
-    if (threadIdx.x == 0) loss[t] = 0.f;
-    return;
-  }
-  if (tail) {
-    for (int i = threadIdx.x; i < (V + 31) / 32; i += NT) member[i] = 0;
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.K; e += NT)
-      if (valid_entry(values, ids, e, V)) atomicOr(&member[ids[e] >> 5], 1u << (ids[e] & 31));
-    __syncthreads();
-  }
-  ExpSum o = {-FLT_MAX, 0.f};  // entries outside the list (tail) or all
-  each<T, NT>(row, V, [&](int i, float x) {
-    if (!tail || !((member[i >> 5] >> (i & 31)) & 1)) exp_sum_add(o, x, c);
-  });
-  // (a NaN never becomes the maximum, but makes the sum NaN)
-  o = block_exp_sum<NT>(o, c, red);
-  ExpSum all = o;
-  ExpSum te = {-FLT_MAX, 0.f};
-  if (tail) {
-    ExpSum in = {-FLT_MAX, 0.f};
-    for (int e = threadIdx.x; e < a.K; e += NT)
-      if (valid_entry(values, ids, e, V) && first_of_id(values, ids, e, V)) exp_sum_add(in, to_f32<T>(row[ids[e]]), c);
-    all = exp_sum_join(o, block_exp_sum<NT>(in, c, red), c);
-  }
+  ExpSum in = {-FLT_MAX, 0.f}, te = {-FLT_MAX, 0.f};
   for (int e = threadIdx.x; e < a.K; e += NT)
-    if (valid_entry(values, ids, e, V)) exp_sum_add(te, to_f32<T>(values[e]), c);
+    if (valid_entry(values, ids, e, V)) {
+      exp_sum_add(te, to_f32<T>(values[e]), c);
+      if (tail && (!repeated || first_of_id(values, ids, e, V))) exp_sum_add(in, to_f32<T>(row[ids[e]]), c);
+    }
+  ExpSum all = o;
+  if (tail) all = exp_sum_join(o, block_exp_sum<NT>(in, c, red), c);
   te = block_exp_sum<NT>(te, c, red);
   const float rest = tail ? a.rest[t] : -INFINITY;  // in units of x / tau
-  const bool has_rest = rest > -INFINITY;
+  const bool entries = te.s > 0.f, has_rest = rest > -INFINITY;
   float tr = 0.f, log_tr = 0.f;
-  const bool entries = te.s > 0.f;
   if (has_rest) {
     const ExpSum r = {rest * a.tau, 1.f};
-    const ExpSum both = entries ? exp_sum_join(te, r, c) : r;
-    te = both;
+    te = entries ? exp_sum_join(te, r, c) : r;
     tr = __builtin_amdgcn_exp2f((r.m - te.m) * c) / te.s;
     log_tr = (r.m - te.m) * inv_tau - logf(te.s);
   }
-  const bool live = entries && all.s != 0.f;
+  const bool live = entries && all.s != 0.f;  // (NaN lives)
   float part = 0.f;
   const float shift = logf(all.s) - logf(te.s);
   if (live)
     for (int e = threadIdx.x; e < a.K; e += NT)
       if (valid_entry(values, ids, e, V)) {
-        const float v = to_f32<T>(values[e]), pe = __builtin_amdgcn_exp2f((v - te.m) * c) / te.s;
-        if (pe > 0.f) part += pe * (((v - te.m) - (to_f32<T>(row[ids[e]]) - all.m)) * inv_tau + shift);
+        const float v = to_f32<T>(values[e]), p = __builtin_amdgcn_exp2f((v - te.m) * c) / te.s;
+        if (p > 0.f) part += p * (((v - te.m) - (to_f32<T>(row[ids[e]]) - all.m)) * inv_tau + shift);
       }
   part = block_all<NT>(part, red, [](float x, float y) { return x + y; });
-  if (threadIdx.x == 0) {
-    float coef = 0.f;
-    if (live) {
-      if (tr > 0.f) part += tr * (log_tr - ((o.m - all.m) * inv_tau + logf(o.s) - logf(all.s)));
-      const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
-      coef = o.s != 0.f ? (sr - tr) / o.s : 0.f;
-    }
-    loss[t] = live ? w * a.tau * a.tau * part : 0.f;
-    st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
-    st[2] = o.m; st[3] = coef;
-    st[4] = te.m; st[5] = live ? 1.f / te.s : 0.f;
-    st[6] = live ? 1.f : 0.f; st[7] = 0.f;
+  float coef = 0.f;
+  if (live) {
+    if (tr > 0.f) part += tr * (log_tr - ((o.m - all.m) * inv_tau + logf(o.s) - logf(all.s)));
+    const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
+    coef = o.s != 0.f ? (sr - tr) / o.s : 0.f;
   }
+  st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
+  st[2] = o.m; st[3] = coef;
+  st[4] = te.m; st[5] = live ? 1.f / te.s : 0.f;
+  st[6] = live ? 1.f : 0.f;
+  st[7] = !tail || repeated ? 1.f : 0.f;  // (without the tail nobody looked)
+  if (threadIdx.x == 0) *loss = live ? w * a.tau * a.tau * part : 0.f;
+}
+
+// The gradient of one segment: the tokens outside the list in one pass of 16-byte loads and stores, then those in the list.
+template <typename T, int NT>
+__device__ __forceinline__ void distill_grad(const T* row, int V, const Span<T>& sp, const T* values, const int32_t* ids,
+                                             const DistillArgs& a, const float (&st)[STASH], float f, T* out) {
+  constexpr int E = Span<T>::E;
+  const float c = (float)(LOG2E / (double)a.tau);
+  const bool together = (((uintptr_t)out ^ (uintptr_t)row) & 15) == 0;  // (vectors of the gradient are vectors of the logits)
+  const float mo = st[2], co = st[3] * f;
+  if (st[6] == 0.f) {  // (the logits are not read: they may hold anything)
+    const float zero[E] = {};
+    for (int v = sp.v0 + threadIdx.x; v < sp.v1; v += NT) {
+      T* p = out + sp.head + v * E;
+      if (together) VecIO<T, E>::store(p, zero);
+      else
+        for (int e = 0; e < E; ++e) p[e] = from_f32<T>(0.f);
+    }
+    if (sp.first && (int)threadIdx.x < sp.head) out[threadIdx.x] = from_f32<T>(0.f);
+    if (sp.last && sp.tail + (int)threadIdx.x < V) out[sp.tail + threadIdx.x] = from_f32<T>(0.f);
+    return;
+  }
+  auto grad = [&](float x) { return __builtin_amdgcn_exp2f((x - mo) * c) * co; };
+  sp.template each<NT>(row, V, [&](const float (&x)[E], int v) {
+    float g[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) g[e] = grad(x[e]);
+    T* p = out + sp.head + v * E;
+    if (together) VecIO<T, E>::store(p, g);
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = from_f32<T>(g[e]);
+  }, [&](int i) { out[i] = from_f32<T>(grad(to_f32<T>(row[i]))); });
+  __threadfence_block();  // (the list's tokens are written again, by other threads)
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.K; e += NT) {
+    if (!valid_entry(values, ids, e, V) || !sp.owns(ids[e])) continue;
+    bool mine = true;
+    float te = 0.f;
+    const bool single = st[7] == 0.f;
+    for (int j = single ? e : 0; j < (single ? e + 1 : a.K) && mine; ++j)
+      if (ids[j] == ids[e] && valid_entry(values, ids, j, V)) {
+        mine = j >= e;
+        te += __builtin_amdgcn_exp2f((to_f32<T>(values[j]) - st[4]) * c) * st[5];
+      }
+    if (mine) out[ids[e]] = from_f32<T>((__builtin_amdgcn_exp2f((to_f32<T>(row[ids[e]]) - st[0]) * c) * st[1] - te) * f);
+  }
+}
+
+// LOSS: loss and, without GRAD, the stash; GRAD: the gradient, from this pass's numbers or (not LOSS) the stash.  LOSS takes whole
+// rows (grid n x 1), GRAD alone may have them cut (grid n x nseg).
+template <typename T, int NT, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
+                                                     float* __restrict__ loss, float* __restrict__ stash,
+                                                     const float* __restrict__ upstream, T* __restrict__ grad, int64_t ld_grad) {
+  extern __shared__ uint32_t member[];
+  __shared__ float red[16];
+  __shared__ int repeated;
+  const int64_t t = blockIdx.x;
+  const float w = a.weights ? a.weights[t] : 1.f, c = (float)(LOG2E / (double)a.tau);
+  const T* row = logits + t * ld;
+  const T* values = (const T*)a.values + t * a.K;
+  const int32_t* ids = a.ids + t * a.K;
+  const Span<T> sp(row, V, blockIdx.y, gridDim.y);
+  float st[STASH] = {};
+  if (LOSS) {
+    if (w != 0.f) {
+      const ExpSum o = block_exp_sum<NT>(distill_sum<T, NT>(row, V, sp, values, ids, a.K, a.rest != nullptr, c, member, &repeated), c, red);
+      distill_row<T, NT>(row, V, values, ids, a, t, w, o, repeated != 0, red, st, loss + t);
+    } else if (threadIdx.x == 0) {
+      loss[t] = 0.f;
+    }
+    if (!GRAD && threadIdx.x < STASH) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < STASH; ++i) v = (int)threadIdx.x == i ? st[i] : v;
+      stash[t * STASH + threadIdx.x] = v;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < STASH; ++i) st[i] = stash[t * STASH + i];
+  }
+  if (GRAD) distill_grad<T, NT>(row, V, sp, values, ids, a, st, w * a.tau * (upstream ? upstream[t] : 1.f), grad + t * ld_grad);
+}
+
+// Few or long rows: the sums of a row's segments, then the row's loss and stash from them.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void distill_part_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
+                                                          float4* __restrict__ parts) {
+  extern __shared__ uint32_t member[];
+  __shared__ float red[16];
+  __shared__ int repeated;
+  const int64_t t = blockIdx.x;
+  const int seg = blockIdx.y, nseg = gridDim.y;
+  if (a.weights && a.weights[t] == 0.f) return;
+  const float c = (float)(LOG2E / (double)a.tau);
+  const T* row = logits + t * ld;
+  const Span<T> sp(row, V, seg, nseg);
+  const ExpSum o = block_exp_sum<NT>(distill_sum<T, NT>(row, V, sp, (const T*)a.values + t * a.K, a.ids + t * a.K, a.K, a.rest != nullptr, c,
+                                                        member, &repeated), c, red);
+  if (threadIdx.x == 0) parts[t * nseg + seg] = make_float4(o.m, o.s, a.rest && repeated ? 1.f : 0.f, 0.f);
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
-                                                         const float* __restrict__ upstream, const float* __restrict__ stash,
-                                                         T* __restrict__ grad, int64_t ld_grad) {
+__global__ __launch_bounds__(NT) void distill_join_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a, int nseg,
+                                                          const float4* __restrict__ parts, float* __restrict__ loss,
+                                                          float* __restrict__ stash) {
+  __shared__ float red[16];
   const int64_t t = blockIdx.x;
-  const float* st = stash + t * STASH;
-  const T* row = logits + t * ld;
-  T* out = grad + t * ld_grad;
-  const T* values = (const T*)a.values + t * a.K;
-  const int32_t* ids = a.ids + t * a.K;
-  const float c = (float)(LOG2E / (double)a.tau);
-  if (st[6] == 0.f) {
-    for (int i = threadIdx.x; i < V; i += NT) out[i] = from_f32<T>(0.f);
-    return;
+  const float w = a.weights ? a.weights[t] : 1.f, c = (float)(LOG2E / (double)a.tau);
+  float st[STASH] = {};
+  if (w != 0.f) {
+    ExpSum o = {-FLT_MAX, 0.f};
+    bool repeated = false;
+    for (int s = threadIdx.x; s < nseg; s += NT) {
+      const float4 p = parts[t * nseg + s];
+      o = exp_sum_join(o, {p.x, p.y}, c);
+      repeated = repeated || p.z != 0.f;
+    }
+    o = block_exp_sum<NT>(o, c, red);
+    repeated = block_max<NT>(repeated ? 1.f : 0.f, red) > 0.f;
+    distill_row<T, NT>(logits + t * ld, V, (const T*)a.values + t * a.K, a.ids + t * a.K, a, t, w, o, repeated, red, st, loss + t);
+  } else if (threadIdx.x == 0) {
+    loss[t] = 0.f;
   }
-  const float f = (a.weights ? a.weights[t] : 1.f) * a.tau * (upstream ? upstream[t] : 1.f);
-  const float mo = st[2], co = st[3] * f;
-  each<T, NT>(row, V, [&](int i, float x) { out[i] = from_f32<T>(__builtin_amdgcn_exp2f((x - mo) * c) * co); });
-  __threadfence_block();
-  __syncthreads();
-  for (int e = threadIdx.x; e < a.K; e += NT) {
-    if (!valid_entry(values, ids, e, V) || !first_of_id(values, ids, e, V)) continue;
-    float te = 0.f;
-    for (int j = e; j < a.K; ++j)
-      if (ids[j] == ids[e] && valid_entry(values, ids, j, V)) te += __builtin_amdgcn_exp2f((to_f32<T>(values[j]) - st[4]) * c) * st[5];
-    const float s = __builtin_amdgcn_exp2f((to_f32<T>(row[ids[e]]) - st[0]) * c) * st[1];
-    out[ids[e]] = from_f32<T>((s - te) * f);
+  if (threadIdx.x < STASH) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < STASH; ++i) v = (int)threadIdx.x == i ? st[i] : v;
+    stash[t * STASH + threadIdx.x] = v;
   }
 }
-
 
 // ------------------------------------------------------------------ vocabularies of at most 64 entries: G lanes a row
 // One lane per entry, G = 32 (two rows a wave) or 64.  The fill loop's 30-entry rows are 120 bytes: a workgroup per row costs
@@ -1542,13 +1694,30 @@ int distill_small(const T* x, int64_t ld, int n, int V, const DistillArgs& a, fl
 }
 bool small_rows(int V, int k) { return V <= 64 && k <= 64; }
 
+// Segments of a row: one where the rows fill the chip (four workgroups a CU), else as many as do, none below 1024 vectors; a
+// segment's membership bits fit MAX_MEMBER.
+int distill_segs(int dtype, int T, int V) {
+  const int e = dtype == PG_F32 ? 4 : 8;
+  int nseg = (1024 + T - 1) / T;
+  const int most = V / (1024 * e), least = (V + MAX_MEMBER - 1) / MAX_MEMBER;
+  if (nseg > most) nseg = most;
+  return nseg < least ? least : nseg < 1 ? 1 : nseg;
+}
+size_t member_bytes(int V, int nseg, bool tail) { return tail ? ((size_t)(V / nseg) + 64) / 32 * 4 + 16 : 0; }
+
 template <typename T>
-int distill_forward(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, float* stash, hipStream_t s) {
+int distill_forward(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, float* stash, void* ws, hipStream_t s) {
   if (small_rows(V, a.K))
     return distill_small<T, true, false>(x, ld, n, V, a, loss, stash, nullptr, nullptr, 0, s);
-  const size_t lds = a.rest ? (size_t)((V + 31) / 32) * 4 : 0;
-  if (lds > 128 * 1024) return PG_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((distill_fwd_kernel<T, 256>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, stash);
+  const int nseg = distill_segs(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V);
+  const size_t lds = member_bytes(V, nseg, a.rest != nullptr);
+  if (nseg == 1) {
+    hipLaunchKernelGGL((distill_kernel<T, 256, true, false>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, stash,
+                       (const float*)nullptr, (T*)nullptr, (int64_t)0);
+  } else {
+    hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(n, nseg), dim3(256), lds, s, x, ld, V, a, (float4*)ws);
+    hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, V, a, nseg, (const float4*)ws, loss, stash);
+  }
   return check_launch();
 }
 
@@ -1557,15 +1726,21 @@ int distill_backward(const T* x, int64_t ld, int n, int V, const DistillArgs& a,
                      int64_t ldg, hipStream_t s) {
   if (small_rows(V, a.K))
     return distill_small<T, false, true>(x, ld, n, V, a, nullptr, const_cast<float*>(stash), up, grad, ldg, s);
-  hipLaunchKernelGGL((distill_bwd_kernel<T, 256>), dim3(n), dim3(256), 0, s, x, ld, V, a, up, stash, grad, ldg);
+  hipLaunchKernelGGL((distill_kernel<T, 256, false, true>), dim3(n, distill_segs(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V)), dim3(256),
+                     0, s, x, ld, V, a, (float*)nullptr, const_cast<float*>(stash), up, grad, ldg);
   return check_launch();
 }
 
 template <typename T>
-int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, T* grad, int64_t ldg, float* stash,
-                 hipStream_t s) {
+int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, T* grad, int64_t ldg, void* ws, hipStream_t s) {
   if (small_rows(V, a.K)) return distill_small<T, true, true>(x, ld, n, V, a, loss, nullptr, nullptr, grad, ldg, s);
-  const int rc = distill_forward(x, ld, n, V, a, loss, stash, s);
+  if (distill_segs(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V) == 1) {
+    hipLaunchKernelGGL((distill_kernel<T, 256, true, true>), dim3(n), dim3(256), member_bytes(V, 1, a.rest != nullptr), s, x, ld, V, a,
+                       loss, (float*)nullptr, (const float*)nullptr, grad, ldg);
+    return check_launch();
+  }
+  float* stash = (float*)ws;
+  const int rc = distill_forward(x, ld, n, V, a, loss, stash, stash + (int64_t)n * STASH, s);
   return rc != PG_OK ? rc : distill_backward(x, ld, n, V, a, nullptr, stash, grad, ldg, s);
 }
 
@@ -1613,7 +1788,11 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
 }
 
 extern "C" int64_t pg_distill_stash_floats(void) { return STASH; }
-extern "C" int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k) { return (int64_t)T * STASH * 4; }
+extern "C" int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k, int with_grad) {
+  if (small_rows(V, k)) return 0;
+  const int64_t nseg = distill_segs(dtype, T, V);
+  return nseg == 1 ? 0 : T * (nseg * 16 + (with_grad ? STASH * 4 : 0));
+}
 
 extern "C" int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids,
                               int k, const float* rest, const float* weights, float temperature, float* loss, float* stash,
@@ -1622,10 +1801,13 @@ extern "C" int pg_distill_fwd(int dtype, const void* logits, int64_t ld, int T, 
   if (rc != PG_OK) return rc;
   if (!loss || !stash) return PG_ERR_ARG;
   if ((uintptr_t)stash & 15) return PG_ERR_ALIGN;
+  const int64_t need = pg_distill_workspace_bytes(dtype, T, V, k, 0);
+  if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
+  if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
   const DistillArgs a = {values, ids, rest, weights, k, temperature};
   hipStream_t s = (hipStream_t)stream;
-  return dtype == PG_F32 ? distill_forward((const float*)logits, ld, T, V, a, loss, stash, s)
-                         : distill_forward((const bf16_t*)logits, ld, T, V, a, loss, stash, s);
+  return dtype == PG_F32 ? distill_forward((const float*)logits, ld, T, V, a, loss, stash, workspace, s)
+                         : distill_forward((const bf16_t*)logits, ld, T, V, a, loss, stash, workspace, s);
 }
 
 extern "C" int pg_distill_bwd(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids,
@@ -1649,11 +1831,12 @@ extern "C" int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, i
   const int bad = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
   if (bad != PG_OK) return bad;
   if (!loss || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
-  if (!workspace || workspace_bytes < pg_distill_workspace_bytes(dtype, T, V, k)) return PG_ERR_WORKSPACE;
+  const int64_t need = pg_distill_workspace_bytes(dtype, T, V, k, 1);
+  if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
   const DistillArgs a = {values, ids, rest, weights, k, temperature};
   hipStream_t s = (hipStream_t)stream;
   return dtype == PG_F32
-             ? distill_both((const float*)logits, ld, T, V, a, loss, (float*)dlogits, ld_dlogits, (float*)workspace, s)
-             : distill_both((const bf16_t*)logits, ld, T, V, a, loss, (bf16_t*)dlogits, ld_dlogits, (float*)workspace, s);
+             ? distill_both((const float*)logits, ld, T, V, a, loss, (float*)dlogits, ld_dlogits, workspace, s)
+             : distill_both((const bf16_t*)logits, ld, T, V, a, loss, (bf16_t*)dlogits, ld_dlogits, workspace, s);
 }

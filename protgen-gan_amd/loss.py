@@ -149,10 +149,16 @@ class _DistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
+        if torch.is_grad_enabled():  # (create_graph: a second derivative is refused when it is asked for)
+            return _DistillFn._backward_once(ctx, dloss)
         logits, values, ids, weights, stash = ctx.saved_tensors
-        return (ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature),) + (None,) * 5
+        return ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature), None, None, None, None, None
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def _backward_once(ctx, dloss):
+        return _DistillFn.backward(ctx, dloss)
 
 
 def distillation_loss(student_logits, top_values, top_ids, rest=None, temperature=1.0, weights=None):
@@ -164,7 +170,6 @@ def distillation_loss(student_logits, top_values, top_ids, rest=None, temperatur
     over the record's entries e and, with `rest`, the event "any other token" (without it the teacher is renormalised over its
     entries).  `weights` fp32 [...]: rows with weight 0 (padding, positions that are not scored) are not read and get no
     gradient, whatever they hold.  Differentiable in student_logits, once; ids outside the vocabulary (-1) mark absent entries."""
-    for name, t in (("top_values", top_values), ("rest", rest), ("weights", weights)):
-        if t is not None and t.requires_grad:
-            raise ValueError(f"{name} requires a gradient: the loss is differentiable in the student's logits only")
+    if top_values.requires_grad or (rest is not None and rest.requires_grad) or (weights is not None and weights.requires_grad):
+        raise ValueError("top_values, rest and weights must not require a gradient: the loss is differentiable in the student's logits")
     return _DistillFn.apply(student_logits, top_values, top_ids, rest, weights, float(temperature))

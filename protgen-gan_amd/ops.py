@@ -240,26 +240,28 @@ def _rows(x, what="logits"):
 def _launch(x, name, args, nbytes=0):
     """check(lib.name(*args[, workspace, bytes], stream)) on x's device and its current stream.  The workspace comes from the
     caching allocator: calls on other streams, and captured graphs, have their own."""
-    dev = x.device
-    if dev.index != torch.cuda.current_device():
+    dev = x.device.index
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _launch(x, name, args, nbytes)
     if nbytes is not None:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         args += (ptr(ws), nbytes)
-    check(getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream), name)
+    rc = getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, name)
 
 
-def _same(device, **tensors):
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{name} on {t.device}, logits on {device}")
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+def _same(like, name, t, dtype, shape):
+    """`t` is of the given type and shape on the logits' device."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} on {t.device}, logits on {like.device}")
 
 
 def _positive(temperature):
@@ -304,13 +306,13 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     dt = dt_code(logits.dtype)
     T, V, ld = _rows(logits)
     dev = logits.device
-    _same(dev, noise=(noise, torch.float32, (T, V)))
+    _same(logits, "noise", noise, torch.float32, (T, V))
     ld_noise = _rows(noise, "noise")[2]
     rows = {}
     for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                            ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if torch.is_tensor(v) and v.dim():
-            _same(dev, **{name: (v, dtype, (T,))})
+            _same(logits, name, v, dtype, (T,))
             rows[name] = v.contiguous()
     num = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
     for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
@@ -329,7 +331,8 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         pred = torch.empty(T, dtype=torch.int64, device=dev)
     if conf is None:
         conf = torch.empty(T, dtype=torch.float32, device=dev)
-    _same(dev, pred=(pred, torch.int64, (T,)), conf=(conf, torch.float32, (T,)))
+    _same(logits, "pred", pred, torch.int64, (T,))
+    _same(logits, "conf", conf, torch.float32, (T,))
     if not (pred.is_contiguous() and conf.is_contiguous()):
         raise ValueError("pred and conf must be contiguous")
     if T:
@@ -346,8 +349,10 @@ def _distill_args(logits, values, ids, rest, weights, temperature):
     lead, k = logits.shape[:-1], values.shape[-1] if values.dim() else 0
     if not 1 <= k <= TOP_LOGITS_MAX:
         raise ValueError(f"values must hold 1..{TOP_LOGITS_MAX} entries per row, got {k}")
-    _same(logits.device, values=(values, logits.dtype, (*lead, k)), ids=(ids, torch.int32, (*lead, k)),
-          rest=(rest, torch.float32, lead), weights=(weights, torch.float32, lead))
+    _same(logits, "values", values, logits.dtype, lead + (k,))
+    _same(logits, "ids", ids, torch.int32, values.shape)
+    _same(logits, "rest", rest, torch.float32, lead)
+    _same(logits, "weights", weights, torch.float32, lead)
     temperature = _positive(temperature)
     _need_cuda(logits)
     values, ids = values.contiguous(), ids.contiguous()
@@ -364,14 +369,14 @@ def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
     if T:
         _launch(logits, "pg_distill_fwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest),
                                            ptr(weights), temperature, loss.data_ptr(), stash.data_ptr()),
-                lib.pg_distill_workspace_bytes(dt, T, V, k))
+                lib.pg_distill_workspace_bytes(dt, T, V, k, 0))
     return loss, stash
 
 
 def distill_bwd(logits, values, ids, stash, dloss, weights=None, temperature=1.0):
     """d sum(dloss * loss) / d logits, contiguous, in the logits' type.  `stash` from distill_fwd on the same arguments."""
     dt, T, V, ld, k, values, ids, _, weights, temperature = _distill_args(logits, values, ids, None, weights, temperature)
-    _same(logits.device, dloss=(dloss, torch.float32, logits.shape[:-1]))
+    _same(logits, "dloss", dloss, torch.float32, logits.shape[:-1])
     dloss = dloss.contiguous()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if T:
@@ -389,7 +394,7 @@ def distill_loss_grad(logits, values, ids, rest=None, temperature=1.0, weights=N
     if T:
         _launch(logits, "pg_distill_loss_grad",
                 (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest), ptr(weights), temperature,
-                 loss.data_ptr(), out.data_ptr(), V), lib.pg_distill_workspace_bytes(dt, T, V, k))
+                 loss.data_ptr(), out.data_ptr(), V), lib.pg_distill_workspace_bytes(dt, T, V, k, 1))
     return loss, out
 
 

@@ -104,7 +104,17 @@ def test_c_abi_refusals(pg):
     assert fwd(stash=p + 4) == -2 and bwd(stash=p + 4) == -2
     assert bwd(stash=None) == ARG and bwd(out=None) == ARG and bwd(ldo=7) == ARG
 
-    def both(ws=p, n=0, ldo=8):
-        return lib.pg_distill_loss_grad(0, p, 8, 2, 8, p, p, 3, None, None, 1.0, p, p, ldo, ws, n, None)
-    need = lib.pg_distill_workspace_bytes(0, 2, 8, 3)
+    # two rows of 100000: cut into segments, which need a workspace
+    def both(ws=p, n=0, ldo=100000, T=2, V=100000):
+        return lib.pg_distill_loss_grad(0, p, V, T, V, p, p, 3, None, None, 1.0, p, p, ldo, ws, n, None)
+    need = lib.pg_distill_workspace_bytes(0, 2, 100000, 3, 1)
     assert need > 0 and both(n=need - 1) == WORKSPACE and both(ws=None, n=need) == WORKSPACE and both(n=need, ldo=7) == ARG
+    assert both(ws=p + 4, n=need) == -2
+    fneed = lib.pg_distill_workspace_bytes(0, 2, 100000, 3, 0)
+    assert 0 < fneed < need
+    assert lib.pg_distill_fwd(0, p, 100000, 2, 100000, p, p, 3, None, None, 1.0, p, p, p, fneed - 1, None) == WORKSPACE
+    tneed = lib.pg_top_logits_workspace_bytes(0, 2, 100000, 3)
+    assert tneed > 0 and lib.pg_top_logits(0, p, 100000, 2, 100000, 3, 1.0, p, p, p, p, tneed - 1, None) == WORKSPACE
+    sneed = lib.pg_sample_filtered_workspace_bytes(0, 2, 100000, 5)
+    assert sneed > 0 and lib.pg_sample_filtered(0, p, 100000, p, 100000, 2, 100000, 1.0, 5, 1.0, 0.0, None, None, None, None, p, p, None,
+                                                0, None) == WORKSPACE
