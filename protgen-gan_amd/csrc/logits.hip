@@ -96,6 +96,29 @@ __device__ __forceinline__ ExpSum exp_sum_join(ExpSum a, ExpSum b, float c) {
   const float m = fmaxf(a.m, b.m);
   return {m, a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + b.s * __builtin_amdgcn_exp2f((b.m - m) * c)};
 }
+// N such sums over the workgroup at once: each wave's by shuffles, the waves' through LDS (4 * N words per wave) behind one barrier.
+template <int NT, int N> __device__ __forceinline__ void block_exp_sums(ExpSum (&a)[N], float c, float2* lds) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float m = a[i].m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float s = a[i].s * __builtin_amdgcn_exp2f((a[i].m - m) * c);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    a[i] = {m, s};
+    if (NT > 64 && (threadIdx.x & 63) == 0) lds[(threadIdx.x >> 6) * N + i] = make_float2(m, s);
+  }
+  if (NT == 64) return;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    ExpSum t = {lds[i].x, lds[i].y};
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) t = exp_sum_join(t, {lds[w * N + i].x, lds[w * N + i].y}, c);
+    a[i] = t;
+  }
+}
 template <int NT> __device__ __forceinline__ ExpSum block_exp_sum(ExpSum a, float c, float* lds) {
   const float m = block_max<NT>(a.m, lds);
   const float s = block_all<NT>(a.s * __builtin_amdgcn_exp2f((a.m - m) * c), lds, [](float x, float y) { return x + y; });
@@ -1148,13 +1171,16 @@ template <typename T> struct Span {
   __device__ __forceinline__ bool owns(int i) const {
     return i < head ? first : i >= tail ? last : i >= head + v0 * E && i < head + v1 * E;
   }
-  // vec(o, v) over the vectors, four in flight per thread; one(i) over the odd elements
-  template <int NT, typename F, typename G> __device__ __forceinline__ void each(const T* row, int V, F vec, G one) const {
+  // vec(o, v) over the vectors, four in flight per thread (begin() sends the first off); one(i) over the odd elements
+  template <int NT> __device__ __forceinline__ void begin(const T* row, uint4 (&d)[4]) const {
     const uint4* p = reinterpret_cast<const uint4*>(row + head);
-    if (v0 + (int)threadIdx.x < v1) {
-      uint4 d[4];
+    if (v0 + (int)threadIdx.x < v1)
 #pragma unroll
       for (int u = 0; u < 4; ++u) d[u] = p[min(v0 + (int)threadIdx.x + u * NT, v1 - 1)];
+  }
+  template <int NT, typename F, typename G> __device__ __forceinline__ void each(const T* row, int V, uint4 (&d)[4], F vec, G one) const {
+    const uint4* p = reinterpret_cast<const uint4*>(row + head);
+    if (v0 + (int)threadIdx.x < v1) {
 #pragma unroll 1
       for (int v = v0 + threadIdx.x; v < v1; v += NT) {
         float o[E];
@@ -1177,6 +1203,8 @@ template <typename T, int NT>
 __device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>& sp, const T* values, const int32_t* ids, int K, bool tail,
                                               float c, uint32_t* member, int* repeated) {
   constexpr int E = Span<T>::E;
+  uint4 d[4];
+  sp.template begin<NT>(row, d);
   const int start = sp.head + sp.v0 * E - E;  // element of bit 0: a vector's worth before the segment, for the odd elements in front
   if (tail) {
     const int bits = (sp.v1 - sp.v0 + 2) * E;
@@ -1192,7 +1220,7 @@ __device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>
   }
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(member);
   ExpSum o = {-FLT_MAX, 0.f};
-  sp.template each<NT>(row, V, [&](const float (&x)[E], int v) {
+  sp.template each<NT>(row, V, d, [&](const float (&x)[E], int v) {
     const int at = v - sp.v0 + 1;
     const uint32_t in = tail ? (E == 8 ? bytes[at] : bytes[at >> 1] >> (at & 1) * 4 & 15) : 0;
     if (in == 0) {
@@ -1210,23 +1238,41 @@ __device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>
   return o;
 }
 
-// The row's loss and stash from its sum over the tokens outside the list (tail) or over all of them.  Every thread of the
+// One entry of the teacher's list per thread, loaded before the pass over the row (longer lists: the rest in loops).
+struct ListEntry { int id; float v, x; };  // id -1: absent
+template <typename T> __device__ __forceinline__ ListEntry list_entry(const T* row, int V, const T* values, const int32_t* ids, int e, int K) {
+  if (e >= K || !valid_entry(values, ids, e, V)) return {-1, -INFINITY, 0.f};
+  return {ids[e], to_f32<T>(values[e]), to_f32<T>(row[ids[e]])};
+}
+struct DistillLds {
+  float2 sums[16 * 3];
+  float red[16];
+  int repeated;
+};
+
+// The row's loss and stash from each thread's sum over the tokens outside the list (tail) or over all of them.  Every thread of the
 // workgroup returns with the stash's numbers in st.
 template <typename T, int NT>
 __device__ __forceinline__ void distill_row(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
-                                            ExpSum o, bool repeated, float* red, float (&st)[STASH], float* loss) {
+                                            ListEntry mine, ExpSum own, bool repeated, DistillLds& l, float (&st)[STASH], float* loss) {
   const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
   const bool tail = a.rest != nullptr;
-  ExpSum in = {-FLT_MAX, 0.f}, te = {-FLT_MAX, 0.f};
-  for (int e = threadIdx.x; e < a.K; e += NT)
-    if (valid_entry(values, ids, e, V)) {
-      exp_sum_add(te, to_f32<T>(values[e]), c);
-      if (tail && (!repeated || first_of_id(values, ids, e, V))) exp_sum_add(in, to_f32<T>(row[ids[e]]), c);
-    }
-  ExpSum all = o;
-  if (tail) all = exp_sum_join(o, block_exp_sum<NT>(in, c, red), c);
-  te = block_exp_sum<NT>(te, c, red);
   const float rest = tail ? a.rest[t] : -INFINITY;  // in units of x / tau
+  ExpSum sums[3] = {own, {-FLT_MAX, 0.f}, {-FLT_MAX, 0.f}};  // outside, inside the list; the teacher's
+  auto entries_of = [&](auto f) {
+    if (mine.id >= 0) f(mine, (int)threadIdx.x);
+    for (int e = threadIdx.x + NT; e < a.K; e += NT) {
+      const ListEntry n = list_entry(row, V, values, ids, e, a.K);
+      if (n.id >= 0) f(n, e);
+    }
+  };
+  entries_of([&](ListEntry n, int e) {
+    exp_sum_add(sums[2], n.v, c);
+    if (tail && (!repeated || first_of_id(values, ids, e, V))) exp_sum_add(sums[1], n.x, c);
+  });
+  block_exp_sums<NT, 3>(sums, c, l.sums);
+  const ExpSum o = sums[0], all = tail ? exp_sum_join(o, sums[1], c) : o;
+  ExpSum te = sums[2];
   const bool entries = te.s > 0.f, has_rest = rest > -INFINITY;
   float tr = 0.f, log_tr = 0.f;
   if (has_rest) {
@@ -1239,12 +1285,11 @@ __device__ __forceinline__ void distill_row(const T* row, int V, const T* values
   float part = 0.f;
   const float shift = logf(all.s) - logf(te.s);
   if (live)
-    for (int e = threadIdx.x; e < a.K; e += NT)
-      if (valid_entry(values, ids, e, V)) {
-        const float v = to_f32<T>(values[e]), p = __builtin_amdgcn_exp2f((v - te.m) * c) / te.s;
-        if (p > 0.f) part += p * (((v - te.m) - (to_f32<T>(row[ids[e]]) - all.m)) * inv_tau + shift);
-      }
-  part = block_all<NT>(part, red, [](float x, float y) { return x + y; });
+    entries_of([&](ListEntry n, int) {
+      const float p = __builtin_amdgcn_exp2f((n.v - te.m) * c) / te.s;
+      if (p > 0.f) part += p * (((n.v - te.m) - (n.x - all.m)) * inv_tau + shift);
+    });
+  part = block_all<NT>(part, l.red, [](float x, float y) { return x + y; });
   float coef = 0.f;
   if (live) {
     if (tr > 0.f) part += tr * (log_tr - ((o.m - all.m) * inv_tau + logf(o.s) - logf(all.s)));
@@ -1280,7 +1325,9 @@ __device__ __forceinline__ void distill_grad(const T* row, int V, const Span<T>&
     return;
   }
   auto grad = [&](float x) { return __builtin_amdgcn_exp2f((x - mo) * c) * co; };
-  sp.template each<NT>(row, V, [&](const float (&x)[E], int v) {
+  uint4 d[4];
+  sp.template begin<NT>(row, d);
+  sp.template each<NT>(row, V, d, [&](const float (&x)[E], int v) {
     float g[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) g[e] = grad(x[e]);
@@ -1313,8 +1360,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logit
                                                      float* __restrict__ loss, float* __restrict__ stash,
                                                      const float* __restrict__ upstream, T* __restrict__ grad, int64_t ld_grad) {
   extern __shared__ uint32_t member[];
-  __shared__ float red[16];
-  __shared__ int repeated;
+  __shared__ DistillLds l;
   const int64_t t = blockIdx.x;
   const float w = a.weights ? a.weights[t] : 1.f, c = (float)(LOG2E / (double)a.tau);
   const T* row = logits + t * ld;
@@ -1324,8 +1370,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logit
   float st[STASH] = {};
   if (LOSS) {
     if (w != 0.f) {
-      const ExpSum o = block_exp_sum<NT>(distill_sum<T, NT>(row, V, sp, values, ids, a.K, a.rest != nullptr, c, member, &repeated), c, red);
-      distill_row<T, NT>(row, V, values, ids, a, t, w, o, repeated != 0, red, st, loss + t);
+      const ListEntry mine = list_entry(row, V, values, ids, threadIdx.x, a.K);
+      const ExpSum o = distill_sum<T, NT>(row, V, sp, values, ids, a.K, a.rest != nullptr, c, member, &l.repeated);
+      distill_row<T, NT>(row, V, values, ids, a, t, w, mine, o, l.repeated != 0, l, st, loss + t);
     } else if (threadIdx.x == 0) {
       loss[t] = 0.f;
     }
@@ -1340,6 +1387,117 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logit
     for (int i = 0; i < STASH; ++i) st[i] = stash[t * STASH + i];
   }
   if (GRAD) distill_grad<T, NT>(row, V, sp, values, ids, a, st, w * a.tau * (upstream ? upstream[t] : 1.f), grad + t * ld_grad);
+}
+
+// A word of one or two entries, those marked in `in` replaced by -inf.
+template <typename T> __device__ __forceinline__ uint32_t without(uint32_t d, uint32_t in) {
+  if (sizeof(T) == 4) return in & 1 ? 0xff800000u : d;
+  d = in & 1 ? (d & 0xffff0000u) | 0xff80u : d;
+  return in & 2 ? (d & 0xffffu) | 0xff800000u : d;
+}
+
+// Loss and gradient with the row in registers, read once: NT * 16 vectors of 16 bytes.  (Two passes read it a second time from the
+// memory-side cache: 168 us against the 105 us of reading and writing 4096 x 32768 bf16 once at the rate of a copy.)
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, 4) void distill_resident_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
+                                                                  float* __restrict__ loss, T* __restrict__ grad, int64_t ld_grad) {
+  extern __shared__ uint32_t member[];
+  __shared__ DistillLds l;
+  constexpr int VPT = 16, E = Span<T>::E;
+  const int64_t t = blockIdx.x;
+  const float w = a.weights ? a.weights[t] : 1.f, c = (float)(LOG2E / (double)a.tau);
+  const T* row = logits + t * ld;
+  const T* values = (const T*)a.values + t * a.K;
+  const int32_t* ids = a.ids + t * a.K;
+  T* out = grad + t * ld_grad;
+  const Span<T> sp(row, V, 0, 1);
+  float st[STASH] = {};
+  if (w == 0.f) {
+    if (threadIdx.x == 0) loss[t] = 0.f;
+    distill_grad<T, NT>(row, V, sp, values, ids, a, st, 0.f, out);
+    return;
+  }
+  Segment<T, NT, VPT> sg;
+  sg.load(row, V, 0, 1);
+  const ListEntry mine = list_entry(row, V, values, ids, threadIdx.x, a.K);
+  const bool tail = a.rest != nullptr;
+  // bits as in distill_sum: element i at i - head + E
+  const int off = E - sp.head;
+  for (int i = threadIdx.x; i < (V + 2 * E + 31) / 32; i += NT) member[i] = 0;
+  if (threadIdx.x == 0) l.repeated = 0;
+  __syncthreads();
+  auto mark = [&](int id) {
+    const int b = id + off;
+    if (atomicOr(&member[b >> 5], 1u << (b & 31)) >> (b & 31) & 1) l.repeated = 1;
+  };
+  if (mine.id >= 0) mark(mine.id);
+  for (int e = threadIdx.x + NT; e < a.K; e += NT)
+    if (valid_entry(values, ids, e, V)) mark(ids[e]);
+  __syncthreads();
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(member);
+  auto is_member = [&](int i) { return (member[(i + off) >> 5] >> ((i + off) & 31) & 1) != 0; };
+  if (tail)  // the list's tokens leave the row here: their gradient is written at the end
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int at = j * NT + (int)threadIdx.x + 1;
+      const uint32_t in = sg.has(j) ? (uint32_t)(E == 8 ? bytes[at] : bytes[at >> 1] >> (at & 1) * 4 & 15) : 0;
+      if (in) {
+        sg.d[j].x = without<T>(sg.d[j].x, in);
+        sg.d[j].y = without<T>(sg.d[j].y, in >> E / 4);
+        sg.d[j].z = without<T>(sg.d[j].z, in >> E / 2);
+        sg.d[j].w = without<T>(sg.d[j].w, in >> E * 3 / 4);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  ExpSum o = {-FLT_MAX, 0.f};
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    float x[E];
+    unpack(sg.d[j], x);
+    exp_sum_vec<E, true>(o, x, vec_max<E>(x), c);
+    __builtin_amdgcn_sched_barrier(0);  // (one vector unpacked at a time: the others' values would not fit the registers)
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (sg.end_at[i] >= 0 && !(tail && is_member(sg.end_at[i]))) exp_sum_add(o, sg.ends[i], c);
+  distill_row<T, NT>(row, V, values, ids, a, t, w, mine, o, l.repeated != 0, l, st, loss + t);
+  const float f = w * a.tau, mo = st[2], co = st[3] * f;
+  const bool together = (((uintptr_t)out ^ (uintptr_t)row) & 15) == 0, live = st[6] != 0.f;
+  auto g_of = [&](float x) { return live ? __builtin_amdgcn_exp2f((x - mo) * c) * co : 0.f; };
+  sg.fresh();
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    if (!sg.has(j)) continue;
+    float x[E];
+    unpack(sg.d[j], x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = g_of(x[e]);
+    T* p = out + sg.index(j);
+    if (together) VecIO<T, E>::store(p, x);
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = from_f32<T>(x[e]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (sg.end_at[i] >= 0) out[sg.end_at[i]] = from_f32<T>(g_of(sg.ends[i]));
+  if (!live) return;
+  __threadfence_block();  // (the list's tokens are written again, by other threads)
+  __syncthreads();
+  const bool repeated = l.repeated != 0;
+  for (int e = threadIdx.x; e < a.K; e += NT) {
+    const ListEntry n = e < NT ? mine : list_entry(row, V, values, ids, e, a.K);
+    if (n.id < 0) continue;
+    bool first = true;
+    float te = 0.f;
+    for (int j = repeated ? 0 : e; j < (repeated ? a.K : e + 1) && first; ++j)
+      if (ids[j] == n.id && valid_entry(values, ids, j, V)) {
+        first = j >= e;
+        te += __builtin_amdgcn_exp2f((to_f32<T>(values[j]) - st[4]) * c) * st[5];
+      }
+    if (first) out[n.id] = from_f32<T>((__builtin_amdgcn_exp2f((n.x - st[0]) * c) * st[1] - te) * f);
+  }
 }
 
 // Few or long rows: the sums of a row's segments, then the row's loss and stash from them.
@@ -1364,11 +1522,15 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_join_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a, int nseg,
                                                           const float4* __restrict__ parts, float* __restrict__ loss,
                                                           float* __restrict__ stash) {
-  __shared__ float red[16];
+  __shared__ DistillLds l;
   const int64_t t = blockIdx.x;
   const float w = a.weights ? a.weights[t] : 1.f, c = (float)(LOG2E / (double)a.tau);
+  const T* row = logits + t * ld;
+  const T* values = (const T*)a.values + t * a.K;
+  const int32_t* ids = a.ids + t * a.K;
   float st[STASH] = {};
   if (w != 0.f) {
+    const ListEntry mine = list_entry(row, V, values, ids, threadIdx.x, a.K);
     ExpSum o = {-FLT_MAX, 0.f};
     bool repeated = false;
     for (int s = threadIdx.x; s < nseg; s += NT) {
@@ -1376,9 +1538,8 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(const T* __restrict__ 
       o = exp_sum_join(o, {p.x, p.y}, c);
       repeated = repeated || p.z != 0.f;
     }
-    o = block_exp_sum<NT>(o, c, red);
-    repeated = block_max<NT>(repeated ? 1.f : 0.f, red) > 0.f;
-    distill_row<T, NT>(logits + t * ld, V, (const T*)a.values + t * a.K, a.ids + t * a.K, a, t, w, o, repeated, red, st, loss + t);
+    repeated = __syncthreads_or(repeated);
+    distill_row<T, NT>(row, V, values, ids, a, t, w, mine, o, repeated, l, st, loss + t);
   } else if (threadIdx.x == 0) {
     loss[t] = 0.f;
   }
@@ -1735,8 +1896,15 @@ template <typename T>
 int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, float* loss, T* grad, int64_t ldg, void* ws, hipStream_t s) {
   if (small_rows(V, a.K)) return distill_small<T, true, true>(x, ld, n, V, a, loss, nullptr, nullptr, grad, ldg, s);
   if (distill_segs(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V) == 1) {
-    hipLaunchKernelGGL((distill_kernel<T, 256, true, true>), dim3(n), dim3(256), member_bytes(V, 1, a.rest != nullptr), s, x, ld, V, a,
-                       loss, (float*)nullptr, (const float*)nullptr, grad, ldg);
+    const int vecs = V / (16 / (int)sizeof(T));
+    const size_t lds = member_bytes(V, 1, true);
+    if (vecs <= 256 * 16)
+      hipLaunchKernelGGL((distill_resident_kernel<T, 256>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, grad, ldg);
+    else if (vecs <= 512 * 16)
+      hipLaunchKernelGGL((distill_resident_kernel<T, 512>), dim3(n), dim3(512), lds, s, x, ld, V, a, loss, grad, ldg);
+    else  // (a workgroup of 1024 holds 131072 bf16 entries, alone on its CU: 408 us for 2048 rows, two passes 350)
+      hipLaunchKernelGGL((distill_kernel<T, 256, true, true>), dim3(n), dim3(256), member_bytes(V, 1, a.rest != nullptr), s, x, ld, V, a,
+                         loss, (float*)nullptr, (const float*)nullptr, grad, ldg);
     return check_launch();
   }
   float* stash = (float*)ws;

@@ -237,6 +237,10 @@ def _rows(x, what="logits"):
     return T, V, (x.stride(0) if T > 1 else V)
 
 
+# (torch.cuda.current_stream builds an object a call, 2 us of the 12 a small call takes on the host)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _launch(x, name, args, nbytes=0):
     """check(lib.name(*args[, workspace, bytes], stream)) on x's device and its current stream.  The workspace comes from the
     caching allocator: calls on other streams, and captured graphs, have their own."""
@@ -247,7 +251,7 @@ def _launch(x, name, args, nbytes=0):
     if nbytes is not None:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         args += (ptr(ws), nbytes)
-    rc = getattr(lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    rc = getattr(lib, name)(*args, _raw_stream(dev))
     if rc:
         check(rc, name)
 

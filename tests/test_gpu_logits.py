@@ -335,6 +335,47 @@ def test_distill_strides_and_leading_dims(pg):
     assert e[0].shape == (0,) and e[1].shape == (0, 77)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,pad", [(1100, 300, 3), (1030, 9001, 0), (1030, 40003, 5), (1030, 90000, 0), (1030, 131072, 0), (1025, 140001, 7)])
+def test_many_rows(pg, dtype, T, V, pad):
+    """The cuts of calls with more rows than the chip takes at once (the other tests' calls are small): rows whole or in large
+    segments, gradients from registers.  All rows run, a few are compared."""
+    at = torch.tensor([0, 1, T // 2, T - 1])
+    g = torch.Generator().manual_seed(V)
+    few = rows(4, V, dtype, V)
+    x = torch.empty(T, V + pad, dtype=dtype, device=DEV).normal_(generator=torch.Generator(DEV).manual_seed(1))[:, :V]
+    x[at] = few
+    k = 33
+    v, i, r = pg.ops.top_logits(x, k, temperature=2.0)
+    wv, wi, wr = spec.top_logits(few, k, 2.0)
+    assert np.array_equal(i[at].cpu().numpy(), wi) and np.array_equal(v[at].double().cpu().numpy(), wv)
+    assert (np.abs(r[at].double().cpu().numpy() - wr) <= ADDS(V) * U + 2 * U * np.abs(wr)).all()
+    q = torch.empty(T, V, device=DEV).exponential_(1.0, generator=torch.Generator(DEV).manual_seed(2))
+    temp = (0.7 + torch.rand(T, generator=g)).to(DEV)
+    for f in ({"top_k": 40, "top_p": 0.9}, {"top_p": 0.97, "temperature": temp}, {"min_p": 0.02}, {"top_k": 700}):
+        full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(f)
+        pred, conf = pg.ops.sample_filtered(x, q, **full)
+        if torch.is_tensor(full["temperature"]):
+            full["temperature"] = temp[at.to(DEV)]
+        wp, wc = spec.sample(few, q[at], full["temperature"], full["top_k"], full["top_p"], full["min_p"])
+        assert np.array_equal(pred[at].cpu().numpy(), wp) and (np.abs(conf[at].double().cpu().numpy() - wc) <= 2 * U * wc).all()
+    del q
+    w = torch.ones(T, device=DEV)
+    w[2::3] = 0.0
+    w[at] = 1.5
+    a, half = (ADDS(V) + 64) * U, torch.finfo(dtype).eps / 2 * 1.01
+    for rest in (r, None):
+        wl, wg, ls, gs = spec.distill(few, v[at], i[at], None if rest is None else rest[at], 2.0, w[at])
+        stash = pg.ops.distill_fwd(x, v, i, rest, w, 2.0)
+        for loss, grad in (pg.ops.distill_loss_grad(x, v, i, rest=rest, temperature=2.0, weights=w),
+                           (stash[0], pg.ops.distill_bwd(x, v, i, stash[1], torch.ones(T, device=DEV), w, 2.0))):
+            assert (np.abs(loss[at].double().cpu().numpy() - wl) <= a * ls).all()
+            assert (np.abs(grad[at].double().cpu().numpy() - wg) <= a * gs + half * np.abs(wg) + 1e-38).all()
+            off = (w == 0).nonzero()[:, 0]
+            assert not grad[off[:7]].any() and not loss[off].any() and torch.isfinite(loss).all()
+
+
 def test_repeat_calls_are_bit_equal(pg):
     for V in (30, 2000, 70001):
         x, v, i, r = record(pg, 5, V, 7, torch.float32, V, 1.0, True)
