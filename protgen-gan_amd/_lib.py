@@ -107,7 +107,7 @@ SIGNATURES = {
     "pg_top_logits_workspace_bytes": (i64, [i32, i32, i32, i32]),
     "pg_top_logits": (i32, [i32, vp, i64, i32, i32, i32, f32, vp, vp, vp, vp, i64, vp]),
     "pg_sample_filtered_workspace_bytes": (i64, [i32, i32, i32, i32]),
-    "pg_sample_filtered": (i32, [i32, vp, i64, vp, i64, i32, i32, f32, i32, f32, f32, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+    "pg_sample_filtered": (i32, [i32, vp, i64, vp, i64, i32, i32, f32, i32, f32, f32, vp, vp, vp, vp, i32, vp, vp, vp, i64, vp]),
     "pg_distill_stash_floats": (i64, []),
     "pg_distill_workspace_bytes": (i64, [i32, i32, i32, i32, i32]),
     "pg_distill_fwd": (i32, [i32, vp, i64, i32, i32, vp, vp, i32, vp, vp, f32, vp, vp, vp, i64, vp]),

@@ -605,7 +605,7 @@ struct RowFilter {
 };
 struct SampleArgs {
   float temperature, top_p, min_p;
-  int top_k;
+  int top_k, empty;  // empty: the token of a row with nothing above -inf
   const float* temps; const int32_t* ks; const float* ps; const float* mins;
   __device__ __forceinline__ RowFilter row(int64_t t) const {
     return {temps ? temps[t] : temperature, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
@@ -849,7 +849,7 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict
   const int want = f.top_k > 0 && f.top_k < POOL / 4 ? f.top_k : 192;  // (what 256 threads sort by counting)
   const int n = rk.first(want, POOL, l.list, c, l);
   if (n == 0) {
-    if (threadIdx.x == 0) pred[t] = -1, conf[t] = 0.f;
+    if (threadIdx.x == 0) pred[t] = args.empty, conf[t] = 0.f;
     return;
   }
   sort_keys<NT>(l.list, n);
@@ -971,7 +971,7 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
     m = key_value((uint32_t)(top >> 32));
     arg = ~(uint32_t)top;
     if (m == -INFINITY || !(f.temperature > 0.f)) {
-      if (threadIdx.x == 0) pred[t] = m == -INFINITY ? -1 : (int64_t)arg, conf[t] = m == -INFINITY ? 0.f : 1.f;
+      if (threadIdx.x == 0) pred[t] = m == -INFINITY ? (int64_t)args.empty : (int64_t)arg, conf[t] = m == -INFINITY ? 0.f : 1.f;
       return;
     }
   } else {
@@ -1664,7 +1664,7 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
   if (at == G) at = Group<G>::min(keep && x == m ? v : G);  // (noise without a usable draw)
   if (t0 >= rows) return;
   if (m == -INFINITY) {
-    if (v == 0) pred[t] = -1, conf[t] = 0.f;
+    if (v == 0) pred[t] = a.empty, conf[t] = 0.f;
   } else if (v == at) {
     pred[t] = v;
     conf[t] = greedy ? 1.f : (float)(w / total);
@@ -1939,18 +1939,18 @@ extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, i
 
 extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
                                   float temperature, int top_k, float top_p, float min_p, const float* temps, const int32_t* ks,
-                                  const float* ps, const float* mins, int64_t* pred, float* conf, void* workspace,
+                                  const float* ps, const float* mins, int empty, int64_t* pred, float* conf, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
-  if (!noise || ld_noise < 0 || !pred || !conf) return PG_ERR_ARG;
+  if (!noise || ld_noise < 0 || !pred || !conf || empty < -1) return PG_ERR_ARG;  // (below -1: rows still open between two launches)
   if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
       (!mins && !(min_p >= 0.f && min_p <= 1.f)))
     return PG_ERR_ARG;
   const int64_t need = pg_sample_filtered_workspace_bytes(dtype, T, V, ks ? 0 : top_k);
   if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
-  const SampleArgs a = {temperature, top_p, min_p, top_k, temps, ks, ps, mins};
+  const SampleArgs a = {temperature, top_p, min_p, top_k, empty, temps, ks, ps, mins};
   return dtype == PG_F32 ? sample_rows((const float*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream)
                          : sample_rows((const bf16_t*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream);
 }

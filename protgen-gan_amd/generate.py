@@ -146,24 +146,34 @@ def _row_packing(generator: Generator, ids: torch.Tensor, widths: List[int]):
 
 def _fill(generator: Generator, ids: torch.Tensor, attn: torch.Tensor, open_masks: List[int], meaningful: List[int],
           first_rate: float, steps: int, keep_percent: float, temperature: float, mask_id: int,
-          widths: List[int]) -> torch.Tensor:
+          widths: List[int], filters=None) -> torch.Tensor:
     """Up to `steps` fill iterations at rates first_rate, first_rate - keep_percent, ...; stops before an iteration
     that would find no mask anywhere (the reference's per-iteration check, generate.py:147-149,185-187).
     open_masks / meaningful: per row, the masks in the template and its tokens outside {PAD, CLS, SEP};
-    widths: per row, the columns its sequence occupies (the ones of its attention mask)."""
+    widths: per row, the columns its sequence occupies (the ones of its attention mask); filters: generate()'s top_k,
+    top_p, min_p."""
     low = list(open_masks)  # lower bound of each row's open masks (module docstring)
     rate = first_rate
     packing = _row_packing(generator, ids, widths)
     for _ in range(steps):
         if not any(low) and int((ids == mask_id).sum().item()) == 0:
             break
-        kw = {} if packing is None else {"packing": packing}
+        kw = dict(filters or {})
+        if packing is not None:
+            kw["packing"] = packing
         ids = generator.generate(ids, attention_mask=attn, keep_percent=keep_percent, current_rate=rate,
                                  temperature=temperature, **kw)
         fill_all = rate <= 0.1
         low = [0 if fill_all else m - min(max(1, int(keep_percent * n)), m) for m, n in zip(low, meaningful)]
         rate = max(0.0, rate - keep_percent)
     return ids
+
+
+def _filters(top_k: int, top_p: float, min_p: float) -> dict:
+    """generate()'s sampling filters, checked before the first pass; empty when all are off (the reference's sampling)."""
+    if top_k < 0 or not 0.0 < top_p <= 1.0 or not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"top_k must be >= 0, top_p in (0, 1], min_p in [0, 1]: got {top_k}, {top_p}, {min_p}")
+    return {} if top_k == 0 and top_p == 1.0 and min_p == 0.0 else {"top_k": top_k, "top_p": top_p, "min_p": min_p}
 
 
 def _decode_rows(tokenizer, ids: torch.Tensor) -> List[str]:
@@ -173,8 +183,10 @@ def _decode_rows(tokenizer, ids: torch.Tensor) -> List[str]:
 @torch.no_grad()
 def generate_full_mode_sequences(generator: Generator, tokenizer, num_sequences: int, length_pool: List[int],
                                  keep_percent: float = 0.10, temperature: float = 1.0, batch_size: int = 64,
-                                 device: str = "cuda", rng_seed: int = 42) -> List[str]:
+                                 device: str = "cuda", rng_seed: int = 42, top_k: int = 0, top_p: float = 1.0,
+                                 min_p: float = 0.0) -> List[str]:
     assert 0.0 < keep_percent <= 1.0
+    filters = _filters(top_k, top_p, min_p)
     dev = torch.device(device)
     generator.eval()
     rng = random.Random(rng_seed)
@@ -185,7 +197,7 @@ def generate_full_mode_sequences(generator: Generator, tokenizer, num_sequences:
         lengths = [sample_sequence_length(length_pool, rng) for _ in range(min(batch_size, num_sequences - start))]
         ids, attn = build_fully_masked_batch(lengths, cls_id, sep_id, mask_id, pad_id, dev)
         ids = _fill(generator, ids, attn, lengths, lengths, 1.0, steps, keep_percent, temperature, mask_id,
-                    [L + 2 for L in lengths])
+                    [L + 2 for L in lengths], filters)
         sequences += _decode_rows(tokenizer, ids)
     return sequences
 
@@ -193,8 +205,10 @@ def generate_full_mode_sequences(generator: Generator, tokenizer, num_sequences:
 @torch.no_grad()
 def generate_seeded_mode_sequences(generator: Generator, tokenizer, num_sequences: int, seed_pool: List[str],
                                    keep_init: float = 0.10, keep_percent: float = 0.10, temperature: float = 1.0,
-                                   batch_size: int = 64, device: str = "cuda", rng_seed: int = 123) -> List[str]:
+                                   batch_size: int = 64, device: str = "cuda", rng_seed: int = 123, top_k: int = 0,
+                                   top_p: float = 1.0, min_p: float = 0.0) -> List[str]:
     assert 0.0 < keep_init < 1.0 and 0.0 < keep_percent <= 1.0
+    filters = _filters(top_k, top_p, min_p)
     dev = torch.device(device)
     generator.eval()
     rng = random.Random(rng_seed)
@@ -211,7 +225,7 @@ def generate_seeded_mode_sequences(generator: Generator, tokenizer, num_sequence
         inner = host[:, 1:]  # (the row's own CLS / SEP / pads do not count; a residue that encodes to one of them does not either)
         meaningful = [int(((row != specials[0]) & (row != specials[1]) & (row != specials[2])).sum()) for row in inner]
         ids = _fill(generator, ids, attn, open_masks, meaningful, 1.0 - keep_init, steps, keep_percent, temperature, mask_id,
-                    attn.sum(dim=1).tolist())
+                    attn.sum(dim=1).tolist(), filters)
         sequences += _decode_rows(tokenizer, ids)
     return sequences
 
@@ -224,7 +238,8 @@ def _parser() -> argparse.ArgumentParser:
                                 ("--num_full", int, 5000), ("--num_seeded", int, 5000), ("--keep_init", float, 0.10),
                                 ("--keep_percent", float, 0.10), ("--temperature", float, 1.0), ("--max_len", int, 600),
                                 ("--min_len", int, 30), ("--batch_size", int, 64), ("--device", str, "cuda"),
-                                ("--rng_seed", int, None), ("--out_dir", str, "./results/")):
+                                ("--rng_seed", int, None), ("--out_dir", str, "./results/"), ("--top_k", int, 0),
+                                ("--top_p", float, 1.0), ("--min_p", float, 0.0)):
         ap.add_argument(flag, type=kind, default=default)
     ap.add_argument("--tokenizer_dir", type=str, default=None, help="Tokenizer path (defaults to finetuned).")
     ap.add_argument("--dtype", choices=["bf16", "fp32"], default="fp32",
@@ -260,7 +275,8 @@ def main(argv=None):
 
     lengths = load_length_distribution(args.dataset_path, max_len=args.max_len, min_len=args.min_len)
     seeds = load_seed_sequences(args.seed_file or args.dataset_path, max_len=args.max_len, min_len=args.min_len)
-    common = dict(keep_percent=args.keep_percent, temperature=args.temperature, batch_size=args.batch_size, device=args.device)
+    common = dict(keep_percent=args.keep_percent, temperature=args.temperature, batch_size=args.batch_size, device=args.device,
+                  **_filters(args.top_k, args.top_p, args.min_p))
     counts = {}
     if args.num_full > 0:
         seqs = generate_full_mode_sequences(generator, tokenizer, args.num_full, lengths, rng_seed=args.rng_seed, **common)

@@ -150,15 +150,23 @@ class _DistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
-        if torch.is_grad_enabled():  # (create_graph: a second derivative is refused when it is asked for)
-            return _DistillFn._backward_once(ctx, dloss)
         logits, values, ids, weights, stash = ctx.saved_tensors
-        return ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature), None, None, None, None, None
+        grad = ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature)
+        if torch.is_grad_enabled():  # (create_graph)
+            grad = _NoSecondDerivative.apply(grad, logits, dloss)
+        return grad, None, None, None, None, None
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """The gradient as a function of the logits and the upstream gradient, of which nobody has written the derivative."""
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def _backward_once(ctx, dloss):
-        return _DistillFn.backward(ctx, dloss)
+    def forward(ctx, grad, logits, dloss):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("distillation_loss is differentiable once")
 
 
 def distillation_loss(student_logits, top_values, top_ids, rest=None, temperature=1.0, weights=None):

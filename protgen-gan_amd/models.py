@@ -53,7 +53,7 @@ class Generator(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids, attention_mask=None, temperature=1.0, keep_percent=0.1, current_rate=None,
-                 noise=None, packing: "RowPacking | None" = None):
+                 noise=None, packing: "RowPacking | None" = None, top_k=0, top_p=1.0, min_p=0.0):
         """One iterative-fill step; mutates and returns `input_ids` (models.py:18-64).
 
         Every position of every row is sampled (pad and already-filled ones too), so the
@@ -61,13 +61,15 @@ class Generator(nn.Module):
         is taken from the device's global generator unless `noise` is given (tests inject
         the reference's draw).  Ties in the top-k are broken towards the lowest index.
 
-        `packing` (not in the reference's signature; bf16): see generate_groups."""
+        `packing` (not in the reference's signature; bf16): see generate_groups.  `top_k`, `top_p`, `min_p` (neither; off by
+        default): sample every position from the head of its distribution only (ops.sample_filtered, same draw of noise);
+        the confidence that ranks the commits is then the token's probability among the entries kept."""
         return self._fill_step(input_ids, attention_mask, [(0, input_ids.shape[0], float(temperature))], keep_percent,
-                               current_rate, noise, packing)
+                               current_rate, noise, packing, (top_k, top_p, min_p))
 
     @torch.no_grad()
     def generate_groups(self, input_ids, attention_mask, groups, keep_percent=0.1, current_rate=None, noise=None,
-                        packing: "RowPacking | None" = None):
+                        packing: "RowPacking | None" = None, top_k=0, top_p=1.0, min_p=0.0):
         """The same fill step for several independent batches stacked along dim 0, one encoder
         pass for all of them.  `groups` = [(row_begin, row_end, temperature), ...] covers the
         rows; each group is sampled at its own temperature, exactly as separate generate()
@@ -77,11 +79,20 @@ class Generator(nn.Module):
         `packing` (bf16 only): the batches have different padded widths and the columns beyond a
         row's own batch hold nothing (pad ids, never attended).  The encoder pass then runs on
         the kept columns only, laid back to back; tokens, confidences and commits are those of
-        the full-width pass."""
+        the full-width pass.  `top_k`, `top_p`, `min_p`: see generate."""
         return self._fill_step(input_ids, attention_mask, [(int(a), int(b), float(t)) for a, b, t in groups],
-                               keep_percent, current_rate, noise, packing)
+                               keep_percent, current_rate, noise, packing, (top_k, top_p, min_p))
 
-    def _fill_step(self, input_ids, attention_mask, groups, keep_percent, current_rate, noise, packing=None):
+    @staticmethod
+    def _sample(logits, noise, temperature, filters, pred=None, conf=None):
+        top_k, top_p, min_p = filters
+        if top_k == 0 and top_p == 1.0 and min_p == 0.0:
+            return ops.sample_tokens(logits, noise, temperature, pred=pred, conf=conf)
+        # (empty=0: what sample_tokens gives for a row of NaN; the commit must write ids of the vocabulary only)
+        return ops.sample_filtered(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, empty=0, pred=pred,
+                                   conf=conf)
+
+    def _fill_step(self, input_ids, attention_mask, groups, keep_percent, current_rate, noise, packing=None, filters=(0, 1.0, 0.0)):
         m: ProtBertForMaskedLM = self.protbert
         ids = m._check_ids(input_ids)
         inplace = ids.data_ptr() == input_ids.data_ptr()
@@ -92,7 +103,7 @@ class Generator(nn.Module):
             raise ValueError("groups must partition the rows of input_ids")
         mask = m._mask01(attention_mask, B, S)
         if packing is not None and packing.T < B * S:
-            return self._fill_step_packed(input_ids, ids, mask, groups, keep_percent, current_rate, noise, packing)
+            return self._fill_step_packed(input_ids, ids, mask, groups, keep_percent, current_rate, noise, packing, filters)
         hidden, _ = m._encode(ids, None, mask, want_stash=False)
         logits = m.lm_logits(hidden).view(B * S, V)
         if noise is None:
@@ -100,12 +111,12 @@ class Generator(nn.Module):
         else:
             noise = noise.to(device=ids.device, dtype=torch.float32).contiguous().view(B * S, V)
         if len(groups) == 1:
-            pred, conf = ops.sample_tokens(logits, noise, groups[0][2])
+            pred, conf = self._sample(logits, noise, groups[0][2], filters)
         else:
             pred = torch.empty(B * S, dtype=torch.long, device=ids.device)
             conf = torch.empty(B * S, dtype=torch.float32, device=ids.device)
             for a, b, t in groups:
-                ops.sample_tokens(logits[a * S:b * S], noise[a * S:b * S], t, pred=pred[a * S:b * S], conf=conf[a * S:b * S])
+                self._sample(logits[a * S:b * S], noise[a * S:b * S], t, filters, pred=pred[a * S:b * S], conf=conf[a * S:b * S])
         fill_all = current_rate is not None and current_rate <= 0.1
         counts = torch.empty(B, 2, dtype=torch.int32, device=ids.device)
         ops.commit_topk(ids, pred, conf, float(keep_percent), fill_all, self.mask_token_id, self.pad_token_id,
@@ -120,7 +131,7 @@ class Generator(nn.Module):
         return input_ids
 
 
-    def _fill_step_packed(self, input_ids, ids, mask, groups, keep_percent, current_rate, noise, pk):
+    def _fill_step_packed(self, input_ids, ids, mask, groups, keep_percent, current_rate, noise, pk, filters):
         m: ProtBertForMaskedLM = self.protbert
         B, S = ids.shape
         V = m.config.vocab_size
@@ -141,7 +152,7 @@ class Generator(nn.Module):
         conf_p = torch.empty(T, dtype=torch.float32, device=ids.device)
         for a, b, t in groups:
             lo, hi = pk.offsets[a], pk.offsets[b]
-            ops.sample_tokens(logits[lo:hi], noise[lo:hi], t, pred=pred_p[lo:hi], conf=conf_p[lo:hi])
+            self._sample(logits[lo:hi], noise[lo:hi], t, filters, pred=pred_p[lo:hi], conf=conf_p[lo:hi])
         # columns outside a row's batch hold pad ids: the commit never looks at their prediction
         pred = torch.zeros(B * S, dtype=torch.long, device=ids.device).index_copy_(0, pk.idx, pred_p)
         conf = torch.zeros(B * S, dtype=torch.float32, device=ids.device).index_copy_(0, pk.idx, conf_p)

@@ -298,13 +298,13 @@ def top_logits(logits, k: int, temperature: float = 1.0):
 TOP_LOGITS_MAX = 1024  # entries of a teacher's record
 
 
-def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, pred=None, conf=None):
+def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, empty=-1, pred=None, conf=None):
     """One token per row of logits [T, V] (fp32 or bf16, any V) from the softmax at `temperature`, cut to the first `top_k`
     entries (0: all), of those to the smallest leading set that holds `top_p` of their mass, and to the entries of at least
     `min_p` times the largest probability.  `noise` fp32 [T, V] ~ Exp(1): the token is the argmax of p / noise, as in
     sample_tokens; only the kept entries' noise is read.  Every setting is a number or a tensor [T] on the device (fp32; top_k:
     int32), read per row without a check.  temperature 0: the largest entry.  Returns (pred int64 [T], conf fp32 [T]), conf the
-    token's probability among the kept entries; a row with nothing above -inf gives (-1, 0)."""
+    token's probability among the kept entries; a row with nothing above -inf gives (`empty`, 0)."""
     if logits.dim() != 2:
         raise ValueError(f"logits: expected [T, V], got {tuple(logits.shape)}")
     dt = dt_code(logits.dtype)
@@ -328,6 +328,8 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError(f"top_k must not be negative, got {num['top_k']}")
     if not 0.0 < num["top_p"] <= 1.0:
         raise ValueError(f"top_p must lie in (0, 1], got {num['top_p']}")
+    if empty < -1:
+        raise ValueError(f"empty must be a token or -1, got {empty}")
     if not 0.0 <= num["min_p"] <= 1.0:
         raise ValueError(f"min_p must lie in [0, 1], got {num['min_p']}")
     _need_cuda(logits)
@@ -343,7 +345,7 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         _launch(logits, "pg_sample_filtered",
                 (dt, logits.data_ptr(), ld, noise.data_ptr(), ld_noise, T, V, num["temperature"], min(num["top_k"], V), num["top_p"],
                  num["min_p"], ptr(rows.get("temperature")), ptr(rows.get("top_k")), ptr(rows.get("top_p")),
-                 ptr(rows.get("min_p")), pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V, min(num["top_k"], V)))
+                 ptr(rows.get("min_p")), empty, pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V, min(num["top_k"], V)))
     return pred, conf
 
 

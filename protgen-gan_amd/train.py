@@ -731,6 +731,30 @@ def generator_update_soft(generator: Generator, critic: Critic, gen_optimizer, m
     return g_loss.detach()
 
 
+def generator_distill_update(student: Generator, teacher: Generator, optimizer, input_ids, attention_mask, k: int = 8,
+                             temperature: float = 2.0, weights=None, grad_sync=None) -> torch.Tensor:
+    """One update of a smaller generator towards a larger one on the masked templates both fill (no counterpart in the
+    reference; a fill iteration's time is its encoder pass, so a student of a few layers fills that much faster).  The teacher's
+    rows are kept as their `k` largest logits and the rest's log-mass (ops.top_logits); the loss is
+    temperature^2 KL(teacher || student) over those k tokens and "any other", a mean over the masked positions (`weights` fp32
+    [B, S]: other positions, other weights, used as they are).  `grad_sync`: called between backward and the optimizer step."""
+    optimizer.zero_grad()
+    with torch.no_grad():
+        logits = teacher.protbert(input_ids=input_ids, attention_mask=attention_mask).logits
+        values, ids, rest = ops.top_logits(logits, min(k, logits.shape[-1]), temperature=temperature)
+        if weights is None:
+            masked = (input_ids == student.mask_token_id).to(torch.float32)
+            weights = masked / masked.sum().clamp_min(1.0)
+    logits = student.protbert(input_ids=input_ids, attention_mask=attention_mask).logits
+    loss, dlogits = ops.distill_loss_grad(logits.detach(), values, ids, rest=rest, temperature=temperature, weights=weights)
+    if logits.requires_grad:
+        logits.backward(dlogits)
+        if grad_sync is not None:
+            grad_sync()
+    optimizer.step()
+    return loss.sum()
+
+
 # FillAhead(low_priority=True): the fill's stream is created at the lowest priority the device offers, so that its
 # workgroups take the CUs the updates leave idle instead of competing with them launch by launch (one GPU, same box:
 # 704.3 -> 691.0 ms per GAN step).  Only without a gradient reduction beside it: with the layer-wise all-reduce on its

@@ -36,7 +36,7 @@ def test_top_logits_refusals(pg, call, error):
 @pytest.mark.parametrize("kw,error", [
     ({"temperature": -0.1}, ValueError), ({"temperature": float("inf")}, ValueError), ({"temperature": float("nan")}, ValueError),
     ({"top_k": -1}, ValueError), ({"top_p": 0.0}, ValueError), ({"top_p": 1.5}, ValueError), ({"top_p": float("nan")}, ValueError),
-    ({"min_p": -0.1}, ValueError), ({"min_p": 1.1}, ValueError),
+    ({"empty": -2}, ValueError), ({"min_p": -0.1}, ValueError), ({"min_p": 1.1}, ValueError),
     ({"temperature": torch.ones(3)}, ValueError), ({"temperature": torch.ones(4, dtype=torch.float64)}, TypeError),
     ({"top_k": torch.ones(4, dtype=torch.int64)}, TypeError), ({"noise": torch.ones(4, 9)}, ValueError),
     ({"noise": torch.ones(4, 10, dtype=torch.float64)}, TypeError), ({"logits": torch.zeros(2, 2, 10)}, ValueError),
@@ -88,10 +88,10 @@ def test_c_abi_refusals(pg):
     assert top(k=0) == ARG and top(k=9) == ARG and top(tau=0.0) == ARG and top(tau=float("nan")) == ARG and top(o=None) == ARG
     assert top(V=(1 << 24) + 1) == UNSUPPORTED and top(V=5000, k=1025) == UNSUPPORTED
 
-    def smp(q=p, ldq=8, T=2, V=8, temp=1.0, k=0, tp=1.0, mp=0.0, out=p):
-        return lib.pg_sample_filtered(0, p, 8, q, ldq, T, V, temp, k, tp, mp, None, None, None, None, out, p, None, 0, None)
+    def smp(q=p, ldq=8, T=2, V=8, temp=1.0, k=0, tp=1.0, mp=0.0, out=p, empty=-1):
+        return lib.pg_sample_filtered(0, p, 8, q, ldq, T, V, temp, k, tp, mp, None, None, None, None, empty, out, p, None, 0, None)
     assert smp(q=None) == ARG and smp(ldq=-1) == ARG and smp(temp=-1.0) == ARG and smp(temp=float("nan")) == ARG and smp(k=-1) == ARG
-    assert smp(tp=0.0) == ARG and smp(tp=1.01) == ARG and smp(mp=-0.1) == ARG and smp(mp=2.0) == ARG and smp(out=None) == ARG
+    assert smp(tp=0.0) == ARG and smp(tp=1.01) == ARG and smp(mp=-0.1) == ARG and smp(mp=2.0) == ARG and smp(out=None) == ARG and smp(empty=-2) == ARG
     assert smp(V=(1 << 24) + 1) == UNSUPPORTED
 
     def fwd(x=p, v=p, k=3, tau=1.0, V=8, loss=p, stash=p):
@@ -116,5 +116,23 @@ def test_c_abi_refusals(pg):
     tneed = lib.pg_top_logits_workspace_bytes(0, 2, 100000, 3)
     assert tneed > 0 and lib.pg_top_logits(0, p, 100000, 2, 100000, 3, 1.0, p, p, p, p, tneed - 1, None) == WORKSPACE
     sneed = lib.pg_sample_filtered_workspace_bytes(0, 2, 100000, 5)
-    assert sneed > 0 and lib.pg_sample_filtered(0, p, 100000, p, 100000, 2, 100000, 1.0, 5, 1.0, 0.0, None, None, None, None, p, p, None,
-                                                0, None) == WORKSPACE
+    assert sneed > 0 and lib.pg_sample_filtered(0, p, 100000, p, 100000, 2, 100000, 1.0, 5, 1.0, 0.0, None, None, None, None, -1, p, p,
+                                                None, 0, None) == WORKSPACE
+
+
+@pytest.mark.parametrize("kw", [{"top_k": -1}, {"top_p": 0.0}, {"top_p": 1.1}, {"min_p": -0.1}, {"min_p": 1.5}])
+def test_generation_refuses_bad_filters_before_the_first_pass(pg, kw):
+    from protgen_gan_amd import generate as G
+    gen = torch.nn.Identity()  # (never called)
+    with pytest.raises(ValueError):
+        G.generate_full_mode_sequences(gen, pg.ProtTokenizer(), 2, [20], device="cpu", **kw)
+    with pytest.raises(ValueError):
+        G.generate_seeded_mode_sequences(gen, pg.ProtTokenizer(), 2, ["ACDE"], device="cpu", **kw)
+
+
+def test_generation_flags(pg):
+    from protgen_gan_amd import generate as G
+    a = G._parser().parse_args(["--ckpt_id", "x"])
+    assert (a.top_k, a.top_p, a.min_p) == (0, 1.0, 0.0) and G._filters(a.top_k, a.top_p, a.min_p) == {}
+    a = G._parser().parse_args(["--ckpt_id", "x", "--top_k", "5", "--top_p", "0.9", "--min_p", "0.1"])
+    assert G._filters(a.top_k, a.top_p, a.min_p) == {"top_k": 5, "top_p": 0.9, "min_p": 0.1}
