@@ -65,7 +65,7 @@ class Generator(nn.Module):
         default): sample every position from the head of its distribution only (ops.sample_filtered, same draw of noise);
         the confidence that ranks the commits is then the token's probability among the entries kept."""
         return self._fill_step(input_ids, attention_mask, [(0, input_ids.shape[0], float(temperature))], keep_percent,
-                               current_rate, noise, packing, (top_k, top_p, min_p))
+                               current_rate, noise, packing, **self._filters(top_k, top_p, min_p))
 
     @torch.no_grad()
     def generate_groups(self, input_ids, attention_mask, groups, keep_percent=0.1, current_rate=None, noise=None,
@@ -81,18 +81,20 @@ class Generator(nn.Module):
         the kept columns only, laid back to back; tokens, confidences and commits are those of
         the full-width pass.  `top_k`, `top_p`, `min_p`: see generate."""
         return self._fill_step(input_ids, attention_mask, [(int(a), int(b), float(t)) for a, b, t in groups],
-                               keep_percent, current_rate, noise, packing, (top_k, top_p, min_p))
+                               keep_percent, current_rate, noise, packing, **self._filters(top_k, top_p, min_p))
+
+    @staticmethod
+    def _filters(top_k, top_p, min_p):
+        return {} if top_k == 0 and top_p == 1.0 and min_p == 0.0 else {"filters": {"top_k": top_k, "top_p": top_p, "min_p": min_p}}
 
     @staticmethod
     def _sample(logits, noise, temperature, filters, pred=None, conf=None):
-        top_k, top_p, min_p = filters
-        if top_k == 0 and top_p == 1.0 and min_p == 0.0:
+        if filters is None:
             return ops.sample_tokens(logits, noise, temperature, pred=pred, conf=conf)
         # (empty=0: what sample_tokens gives for a row of NaN; the commit must write ids of the vocabulary only)
-        return ops.sample_filtered(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, empty=0, pred=pred,
-                                   conf=conf)
+        return ops.sample_filtered(logits, noise, temperature=temperature, empty=0, pred=pred, conf=conf, **filters)
 
-    def _fill_step(self, input_ids, attention_mask, groups, keep_percent, current_rate, noise, packing=None, filters=(0, 1.0, 0.0)):
+    def _fill_step(self, input_ids, attention_mask, groups, keep_percent, current_rate, noise, packing=None, filters=None):
         m: ProtBertForMaskedLM = self.protbert
         ids = m._check_ids(input_ids)
         inplace = ids.data_ptr() == input_ids.data_ptr()
