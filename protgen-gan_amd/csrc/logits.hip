@@ -382,18 +382,27 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
 
 // list[0..n) in LDS, largest first; at least P = the next power of two of room
 template <int NT> __device__ __forceinline__ void sort_keys(uint64_t* list, int n) {
-  if (n <= NT && n <= 512) {  // few: each key's rank by counting, two barriers instead of one per step of a network
-    const uint64_t mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+  if (n <= 2 * NT && n <= 512) {  // few: each key's rank by counting, two barriers instead of one per step of a network
+    const int i0 = threadIdx.x, i1 = threadIdx.x + NT;
+    const uint64_t k0 = i0 < n ? list[i0] : 0, k1 = i1 < n ? list[i1] : 0;
     if ((n & 1) && threadIdx.x == 0) list[n] = 0;
     __syncthreads();
-    int rank = 0;
-    if ((int)threadIdx.x < n)
+    int r0 = 0, r1 = 0;
+    if (n <= NT) {
       for (int j = 0; j < n; j += 2) {
         const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
-        rank += (two.x > mine) + (two.y > mine);
+        r0 += (two.x > k0) + (two.y > k0);
       }
+    } else {
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
+        r0 += (two.x > k0) + (two.y > k0);
+        r1 += (two.x > k1) + (two.y > k1);
+      }
+    }
     __syncthreads();
-    if ((int)threadIdx.x < n) list[rank] = mine;
+    if (i0 < n) list[r0] = k0;
+    if (i1 < n) list[r1] = k1;
     __syncthreads();
     return;
   }
@@ -510,7 +519,7 @@ template <int NT> struct RowKeys {
   template <typename L> __device__ __forceinline__ int first(int K, int room, uint64_t* list, float c, L& l) {
     uint64_t bound = 0;
     const int used = (n + NT - 1) / NT;
-    if (n > 2 * K) {  // by the upper half of the values' bits, nearly always enough
+    if (n > 2 * K && n > 384) {  // by the upper half of the values' bits, nearly always enough (few are sorted whole)
       uint32_t hi[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) hi[r] = (uint32_t)(k[r] >> 32);
@@ -1579,12 +1588,23 @@ template <int G> struct Group {
   template <typename T> static __device__ __forceinline__ T sum(T v) { return all(v, [](T a, T b) { return a + b; }); }
 };
 
-// f(entry u's key, u) for the row's entries, keys in LDS (G per row, those past V zero: behind every entry)
-template <int G, typename F> __device__ __forceinline__ void each_key(const uint32_t* keys, int V, F f) {
-  for (int u = 0; u < V; u += 4) {
+// The number of entries before this lane's (key, v) in its row: those u < v with a key at least this one, those u > v with a larger
+// one.  Keys in LDS, G per row, those past V zero.  The lanes behind u are a constant of the unrolled step, so a step is a select, a
+// comparison and an addition of its carry.
+template <int G> __device__ __forceinline__ int rank_of(const uint32_t* keys, int V, uint32_t key) {
+  const int v = threadIdx.x & (G - 1);
+  const uint32_t next = key + 1;  // (no key is ~0)
+  int rank = 0;
+#pragma unroll
+  for (int u = 0; u < G; u += 4) {
+    if (u >= V) break;
     const uint4 k = *reinterpret_cast<const uint4*>(keys + u);
-    f(k.x, u); f(k.y, u + 1); f(k.z, u + 2); f(k.w, u + 3);
+    rank += k.x >= (v > u ? key : next);
+    rank += k.y >= (v > u + 1 ? key : next);
+    rank += k.z >= (v > u + 2 ? key : next);
+    rank += k.w >= (v > u + 3 ? key : next);
   }
+  return rank;
 }
 
 template <typename T, int G>
@@ -1597,8 +1617,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ lo
   const uint32_t key = v < V ? value_key(to_f32<T>(logits[t * ld + v])) : 0;
   keys[threadIdx.x] = key;
   __syncthreads();
-  int rank = 0;
-  each_key<G>(keys + (threadIdx.x & ~(G - 1)), V, [&](uint32_t k, int u) { rank += k > key || (k == key && u < v); });
+  const int rank = rank_of<G>(keys + (threadIdx.x & ~(G - 1)), V, key);
   const float x = key_value(key);
   const bool left = v < V && rank >= K;
   const float m = Group<G>::max(left ? x : -INFINITY);
@@ -1608,7 +1627,7 @@ __global__ __launch_bounds__(256) void top_small_kernel(const T* __restrict__ lo
     values[t * K + rank] = from_f32<T>(x);
     ids[t * K + rank] = v;
   }
-  if (v == 0) rest[t] = m == -INFINITY || m == INFINITY ? m : (float)((double)m / tau + log((double)sum));
+  if (v == 0) rest[t] = m == -INFINITY || m == INFINITY ? m : (float)((double)m * (1.0 / (double)tau) + (double)logf(sum));
 }
 
 template <typename T, int G>
@@ -1628,28 +1647,33 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
   double w = 0.0;
   if (v < V) w = x == m ? 1.0 : greedy ? 0.0 : exp2_f64(((double)x - (double)m) * (LOG2E / (double)f.temperature));
   keys[threadIdx.x] = key;
-  weights[threadIdx.x] = w;
   __syncthreads();
   bool keep = v < V && x > -INFINITY && f.above_min_p(x, m);
-  if (f.top_p < 1.f) {
-    int rank = 0;
-    double before = 0.0;
-    const double* ws = weights + first;
-    each_key<G>(keys + first, V, [&](uint32_t k, int u) {
-      const bool b = k > key || (k == key && u < v);
-      rank += b;
-      before += b ? ws[u] : 0.0;
-    });
-    const bool in_k = f.top_k <= 0 || rank < f.top_k;
-    const double mass = Group<G>::sum(in_k ? w : 0.0);
-    keep = keep && in_k && (rank == 0 || before < (double)f.top_p * mass);
-  } else if (f.top_k > 0 && f.top_k < V) {
-    int rank = 0;
-    each_key<G>(keys + first, V, [&](uint32_t k, int u) { rank += k > key || (k == key && u < v); });
-    keep = keep && rank < f.top_k;
+  double total;
+  if (f.top_p < 1.f && !greedy) {
+    // weights in the row's order, their running sum, and from it how many entries stay: an entry does while the mass before it is
+    // below the share of the first k's
+    const int rank = rank_of<G>(keys + first, V, key);
+    weights[first + rank] = w;  // (lanes past V: key 0, w 0, ranks V.. by their lane)
+    const int nk = f.top_k > 0 && f.top_k < V ? f.top_k : V;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const double mine = weights[threadIdx.x];
+    double upto = mine;
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) {
+      const double up = __shfl_up(upto, o, G);
+      upto += v >= o ? up : 0.0;
+    }
+    const double mass = __shfl(upto, nk - 1, G);
+    const uint64_t in = __ballot(v < nk && (v == 0 || upto - mine < (double)f.top_p * mass));
+    const int n = __popcll(G == 64 ? in : (threadIdx.x & 32) ? in >> 32 : in & 0xffffffffu);
+    keep = keep && rank < n;
+    total = Group<G>::sum(keep ? w : 0.0);
+  } else {
+    if (f.top_k > 0 && f.top_k < V) keep = keep && rank_of<G>(keys + first, V, key) < f.top_k;
+    if (greedy) keep = keep && x == m;
+    total = Group<G>::sum(keep ? w : 0.0);
   }
-  if (greedy) keep = keep && x == m;
-  const double total = Group<G>::sum(keep ? w : 0.0);
   // the race: in fp32 (relative error below 2^-21) to find who can win, in 64 bits where more than one can
   const float r = keep ? ((float)w > 0.f ? (float)w / q : 0.f) : -1.f;
   const float top = Group<G>::max(greedy ? (keep ? 1.f : -1.f) : r);

@@ -5,6 +5,7 @@ arithmetic step is a call into libprotgen_hip.so."""
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -237,6 +238,10 @@ def _rows(x, what="logits"):
     return T, V, (x.stride(0) if T > 1 else V)
 
 
+# (sizes of workspaces: a function of the call's sizes alone)
+_top_bytes = functools.lru_cache(maxsize=1024)(lib.pg_top_logits_workspace_bytes)
+_sample_bytes = functools.lru_cache(maxsize=1024)(lib.pg_sample_filtered_workspace_bytes)
+_distill_bytes = functools.lru_cache(maxsize=1024)(lib.pg_distill_workspace_bytes)
 # (torch.cuda.current_stream builds an object a call, 2 us of the 12 a small call takes on the host)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
@@ -291,7 +296,7 @@ def top_logits(logits, k: int, temperature: float = 1.0):
     rest = torch.empty(lead, dtype=torch.float32, device=logits.device)
     if T:
         _launch(logits, "pg_top_logits", (dt, logits.data_ptr(), ld, T, V, k, temperature, values.data_ptr(), ids.data_ptr(),
-                                          rest.data_ptr()), lib.pg_top_logits_workspace_bytes(dt, T, V, k))
+                                          rest.data_ptr()), _top_bytes(dt, T, V, k))
     return values, ids, rest
 
 
@@ -312,26 +317,28 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     dev = logits.device
     _same(logits, "noise", noise, torch.float32, (T, V))
     ld_noise = _rows(noise, "noise")[2]
-    rows = {}
-    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if torch.is_tensor(v) and v.dim():
+
+    def setting(name, v, dtype, off):  # (a number, None) or (unused, a row of numbers)
+        if isinstance(v, torch.Tensor) and v.dim():
             _same(logits, name, v, dtype, (T,))
-            rows[name] = v.contiguous()
-    num = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
-    for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
-        if name not in rows:
-            num[name] = int(v) if name == "top_k" else float(v)
-    if not 0.0 <= num["temperature"] < float("inf"):
-        raise ValueError(f"temperature must be finite and not negative, got {num['temperature']}")
-    if num["top_k"] < 0:
-        raise ValueError(f"top_k must not be negative, got {num['top_k']}")
-    if not 0.0 < num["top_p"] <= 1.0:
-        raise ValueError(f"top_p must lie in (0, 1], got {num['top_p']}")
+            return off, v.contiguous()
+        return type(off)(v), None
+
+    temperature, temps = setting("temperature", temperature, torch.float32, 1.0)
+    top_k, ks = setting("top_k", top_k, torch.int32, 0)
+    top_p, ps = setting("top_p", top_p, torch.float32, 1.0)
+    min_p, mins = setting("min_p", min_p, torch.float32, 0.0)
+    if not 0.0 <= temperature < float("inf"):
+        raise ValueError(f"temperature must be finite and not negative, got {temperature}")
+    if top_k < 0:
+        raise ValueError(f"top_k must not be negative, got {top_k}")
+    if not 0.0 < top_p <= 1.0:
+        raise ValueError(f"top_p must lie in (0, 1], got {top_p}")
+    if not 0.0 <= min_p <= 1.0:
+        raise ValueError(f"min_p must lie in [0, 1], got {min_p}")
     if empty < -1:
         raise ValueError(f"empty must be a token or -1, got {empty}")
-    if not 0.0 <= num["min_p"] <= 1.0:
-        raise ValueError(f"min_p must lie in [0, 1], got {num['min_p']}")
+    top_k = min(top_k, V)
     _need_cuda(logits)
     if pred is None:
         pred = torch.empty(T, dtype=torch.int64, device=dev)
@@ -343,9 +350,8 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError("pred and conf must be contiguous")
     if T:
         _launch(logits, "pg_sample_filtered",
-                (dt, logits.data_ptr(), ld, noise.data_ptr(), ld_noise, T, V, num["temperature"], min(num["top_k"], V), num["top_p"],
-                 num["min_p"], ptr(rows.get("temperature")), ptr(rows.get("top_k")), ptr(rows.get("top_p")),
-                 ptr(rows.get("min_p")), empty, pred.data_ptr(), conf.data_ptr()), lib.pg_sample_filtered_workspace_bytes(dt, T, V, min(num["top_k"], V)))
+                (dt, logits.data_ptr(), ld, noise.data_ptr(), ld_noise, T, V, temperature, top_k, top_p, min_p, ptr(temps), ptr(ks),
+                 ptr(ps), ptr(mins), empty, pred.data_ptr(), conf.data_ptr()), _sample_bytes(dt, T, V, top_k))
     return pred, conf
 
 
@@ -375,7 +381,7 @@ def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
     if T:
         _launch(logits, "pg_distill_fwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest),
                                            ptr(weights), temperature, loss.data_ptr(), stash.data_ptr()),
-                lib.pg_distill_workspace_bytes(dt, T, V, k, 0))
+                _distill_bytes(dt, T, V, k, 0))
     return loss, stash
 
 
@@ -400,7 +406,7 @@ def distill_loss_grad(logits, values, ids, rest=None, temperature=1.0, weights=N
     if T:
         _launch(logits, "pg_distill_loss_grad",
                 (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest), ptr(weights), temperature,
-                 loss.data_ptr(), out.data_ptr(), V), lib.pg_distill_workspace_bytes(dt, T, V, k, 1))
+                 loss.data_ptr(), out.data_ptr(), V), _distill_bytes(dt, T, V, k, 1))
     return loss, out
 
 
