@@ -151,26 +151,39 @@ __device__ __forceinline__ double exp2_f64(double t) {
 // bisection over the segment instead.
 constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
 constexpr int MAX_SEG_K = 512;
-constexpr int MAX_CAP(int nt) { return nt == 64 ? 512 : 1088; }  // keys a segment may leave
+constexpr int max_cap(int K) { return K > 128 ? 1088 : 512; }  // keys a segment may leave
 
-template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E]) {  // (NaN: passed over)
-  float m = -INFINITY;
+// The largest of three, NaN passed over.  (fmaxf costs a second instruction per operand here, which quiets signalling NaN first;
+// v_max3_f32 does that by itself.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E], float m = -INFINITY) {
+  if constexpr (E == 1) return max3(m, m, o[0]);
 #pragma unroll
-  for (int e = 0; e < E; ++e) m = fmaxf(m, o[e]);
+  for (int e = 0; e + 1 < E; e += 2) m = max3(m, o[e], o[e + 1]);
   return m;
 }
-// The exponentials of E entries of which vm is the largest, with one rescaling for all of them.  NaN as -inf, or (KEEP_NAN) kept.
+// The exponentials of E entries of which vm is the largest, with one rescaling for all of them.  NaN as -inf (looked for in the
+// sum, not entry by entry), or (KEEP_NAN) kept.
 template <int E, bool KEEP_NAN = false> __device__ __forceinline__ void exp_sum_vec(ExpSum& a, const float (&o)[E], float vm, float c) {
-  const float m = fmaxf(a.m, vm);
+  const float m = max3(a.m, a.m, vm);
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f(((KEEP_NAN ? o[e] : fmaxf(o[e], -INFINITY)) - m) * c);
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((o[e] - m) * c);
+  if (!KEEP_NAN && s != s) {
+    s = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s += o[e] == o[e] ? __builtin_amdgcn_exp2f((o[e] - m) * c) : 0.f;
+  }
   a.s = a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + s;
   a.m = m;
 }
 __device__ __forceinline__ void exp_sum_one(ExpSum& a, float x, float c) {
   const float o[1] = {x};
-  exp_sum_vec<1>(a, o, fmaxf(x, -INFINITY), c);
+  exp_sum_vec<1>(a, o, vec_max<1>(o), c);
 }
 
 // exp((x - m) / temperature) for x <= m in whole multiples of 2^-40: sums of these are the same in any order.
@@ -206,10 +219,10 @@ __device__ __forceinline__ Key kth_bound(const Key (&k)[R], int used, int K, int
   return bound;
 }
 
-template <int NT> struct SegLds {
+template <int NT, bool MANY> struct SegLds {  // MANY: for K above 128
   uint64_t wave[16];
-  static constexpr int STAGE = NT == 64 ? 256 : 512;  // vectors that may hold an entry above the bound
-  static constexpr int LIST = NT == 64 ? 512 : 2048;  // keys (a power of two of at least MAX_CAP)
+  static constexpr int STAGE = MANY ? 512 : 256;  // vectors that may hold an entry above the bound
+  static constexpr int LIST = MANY ? 2048 : 512;  // keys (a power of two of at least max_cap)
   __align__(16) uint64_t list[LIST];
   uint4 vec[STAGE];
   int at[STAGE];
@@ -272,17 +285,17 @@ template <typename T, int NT, int VPT> struct Segment {
 
 // Leaves the keys of the segment's largest entries in list (n of them, at most cap, in no order; at least K if it has as many),
 // the sum over its other entries in rest (per thread), and the level.  FINITE: entries of -inf are never listed.
-template <typename T, int NT, int VPT, bool FINITE>
-__device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, int K, int cap, float c, SegLds<NT>& l, uint64_t& level,
+template <typename T, int NT, int VPT, bool FINITE, bool MANY>
+__device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, int K, int cap, float c, SegLds<NT, MANY>& l, uint64_t& level,
                                        ExpSum& rest) {
-  constexpr int E = Segment<T, NT, VPT>::E, STAGE = SegLds<NT>::STAGE, LIST = SegLds<NT>::LIST;
+  constexpr int E = Segment<T, NT, VPT>::E, STAGE = SegLds<NT, MANY>::STAGE, LIST = SegLds<NT, MANY>::LIST;
   uint64_t* list = l.list;
   float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     float o[E];
     unpack(sg.d[j], o);
-    gm[j & 3] = fmaxf(gm[j & 3], vec_max<E>(o));
+    gm[j & 3] = vec_max<E>(o, gm[j & 3]);
   }
   gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
   uint32_t mk[4];
@@ -382,27 +395,23 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
 
 // list[0..n) in LDS, largest first; at least P = the next power of two of room
 template <int NT> __device__ __forceinline__ void sort_keys(uint64_t* list, int n) {
-  if (n <= 2 * NT && n <= 512) {  // few: each key's rank by counting, two barriers instead of one per step of a network
-    const int i0 = threadIdx.x, i1 = threadIdx.x + NT;
-    const uint64_t k0 = i0 < n ? list[i0] : 0, k1 = i1 < n ? list[i1] : 0;
-    if ((n & 1) && threadIdx.x == 0) list[n] = 0;
+  if (n <= NT && n <= 504) {  // few: each key's rank by counting, two barriers instead of one per step of a network
+    const uint64_t mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+    const int padded = (n + 7) & ~7;
+    if (n + (int)threadIdx.x < padded) list[n + threadIdx.x] = 0;
     __syncthreads();
-    int r0 = 0, r1 = 0;
-    if (n <= NT) {
-      for (int j = 0; j < n; j += 2) {
-        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
-        r0 += (two.x > k0) + (two.y > k0);
+    int rank = 0;
+    if ((int)(threadIdx.x & ~63u) < n)  // (whole waves)
+#pragma unroll 1
+      for (int j = 0; j < padded; j += 8) {  // (four reads in flight: one at a time, each step waits for LDS)
+        ulonglong2 d[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) d[u] = *reinterpret_cast<const ulonglong2*>(list + j + 2 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) rank += (d[u].x > mine) + (d[u].y > mine);
       }
-    } else {
-      for (int j = 0; j < n; j += 2) {
-        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(list + j);
-        r0 += (two.x > k0) + (two.y > k0);
-        r1 += (two.x > k1) + (two.y > k1);
-      }
-    }
     __syncthreads();
-    if (i0 < n) list[r0] = k0;
-    if (i1 < n) list[r1] = k1;
+    if ((int)threadIdx.x < n) list[rank] = mine;
     __syncthreads();
     return;
   }
@@ -439,11 +448,11 @@ __device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float t
     *rest_out = rest.m == INFINITY ? INFINITY : rest.s > 0.f ? (float)((double)rest.m / tau + log((double)rest.s)) : -INFINITY;
 }
 
-template <typename T, int NT, int VPT>
-__global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
+template <typename T, int NT, int VPT, bool MANY>
+__global__ __launch_bounds__(NT, VPT <= 8 ? 8 : 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
                                                          T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest_out,
                                                          SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
-  __shared__ SegLds<NT> l;
+  __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
   const int seg = blockIdx.y, nseg = gridDim.y;
   const float c = (float)(LOG2E / (double)tau);
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict_
   sg.load(row, V, seg, nseg);
   uint64_t level;
   ExpSum rest;
-  const int n = collect<T, NT, VPT, false>(sg, row, K, cap, c, l, level, rest);
+  const int n = collect<T, NT, VPT, false, MANY>(sg, row, K, cap, c, l, level, rest);
   if (nseg == 1) {
     top_finish<T, NT>(l.list, n, K, tau, c, rest, l.red, values + t * K, ids + t * K, rest_out + t);
     return;
@@ -506,7 +515,7 @@ template <int NT> struct RowKeys {
     for (int r = 0; r < R; ++r) {
       const int i = r * NT + threadIdx.x;
       k[r] = 0;
-      if (i < n) {
+      if (r * NT < n && i < n) {
         int s = 0;
         while ((int)ends[s] <= i) ++s;
         k[r] = lists[(t * nseg + s) * cap + i - (s ? (int)ends[s - 1] : 0)];
@@ -519,7 +528,7 @@ template <int NT> struct RowKeys {
   template <typename L> __device__ __forceinline__ int first(int K, int room, uint64_t* list, float c, L& l) {
     uint64_t bound = 0;
     const int used = (n + NT - 1) / NT;
-    if (n > 2 * K && n > 384) {  // by the upper half of the values' bits, nearly always enough (few are sorted whole)
+    if (n > 2 * K) {  // by the upper half of the values' bits, nearly always enough
       uint32_t hi[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) hi[r] = (uint32_t)(k[r] >> 32);
@@ -530,6 +539,7 @@ template <int NT> struct RowKeys {
       uint64_t most = 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
+        if (r >= used) break;
         m += k[r] != 0 && k[r] >= bound;
         if (k[r] < bound && k[r] > most) most = k[r];
       }
@@ -543,8 +553,10 @@ template <int NT> struct RowKeys {
         const float x0 = key_value((uint32_t)(most >> 32));
         uint64_t sum = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+          if (r >= used) break;
           if (k[r] != 0 && k[r] < bound) sum += fixed_weight(key_value((uint32_t)(k[r] >> 32)), x0, c);
+        }
         sum = block_all<NT>(sum, l.wave, [](uint64_t a, uint64_t b) { return a + b; });
         if (threadIdx.x == 0 && most && x0 > -INFINITY) rest = exp_sum_join(rest, {x0, (float)sum * 0x1p-40f}, c);
       }
@@ -552,8 +564,10 @@ template <int NT> struct RowKeys {
       if (threadIdx.x == 0) l.n = 0;
       __syncthreads();
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        if (r >= used) break;
         if (k[r] != 0 && k[r] >= bound) list[atomicAdd(&l.n, 1u)] = k[r];
+      }
       __syncthreads();
       level = bound > level ? bound : level;
       return m;
@@ -581,13 +595,14 @@ __global__ __launch_bounds__(NT) void top_merge_kernel(int nseg, int K, int cap,
   top_finish<T, NT>(l.list, n, K, tau, c, rk.rest, l.red, values + t * K, ids + t * K, rest_out + t);
 }
 
-// How a call is cut: threads and vectors per thread of a segment, segments per row, keys a segment may leave.
-struct Cut { int nt, vpt, nseg, cap; };
+// How a call is cut: threads and vectors per thread of a segment, segments per row, keys a segment may leave, K above 128.
+struct Cut { int nt, vpt, nseg, cap; bool many; };
 Cut cut_rows(int dtype, int T, int V, int K) {
-  if (K > MAX_SEG_K || V <= 64) return {0, 0, 0, 0};
+  if (K > MAX_SEG_K || V <= 64) return {0, 0, 0, 0, false};
+  const bool many = K > 128;
   const int vecs = V / (dtype == PG_F32 ? 4 : 8);
-  const int shapes[3][2] = {{64, 4}, {256, 4}, {256, 16}};
-  for (int i = K <= 128 ? 0 : 1; i < 3; ++i) {
+  const int shapes[3][2] = {{64, 4}, {256, 4}, {256, many ? 16 : 8}};
+  for (int i = many ? 1 : 0; i < 3; ++i) {
     const int per = shapes[i][0] * shapes[i][1], nseg = vecs <= per ? 1 : (vecs + per - 1) / per;
     if (nseg > 1 && i < 2) {
       // few rows: small segments, to spread them over the chip; many: the next larger ones
@@ -595,11 +610,20 @@ Cut cut_rows(int dtype, int T, int V, int K) {
     }
     if (nseg > MAX_SEGS) continue;
     int cap = 2 * K + 64;
-    if (cap > MAX_CAP(shapes[i][0])) cap = MAX_CAP(shapes[i][0]);
+    if (cap > max_cap(K)) cap = max_cap(K);
     if (cap > MERGE / nseg) cap = MERGE / nseg;
-    if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap};
+    if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap, many};
   }
-  return {0, 0, 0, 0};
+  return {0, 0, 0, 0, false};
+}
+template <int N> struct Int { static constexpr int value = N; };
+template <bool B> struct Bool { static constexpr bool value = B; };
+template <typename F> void by_cut(const Cut& c, F f) {
+  if (c.nt == 64) f(Int<64>(), Int<4>(), Bool<false>());
+  else if (c.vpt == 4 && c.many) f(Int<256>(), Int<4>(), Bool<true>());
+  else if (c.vpt == 4) f(Int<256>(), Int<4>(), Bool<false>());
+  else if (c.many) f(Int<256>(), Int<16>(), Bool<true>());
+  else f(Int<256>(), Int<8>(), Bool<false>());
 }
 
 // ------------------------------------------------------------------ sampling
@@ -1090,10 +1114,10 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
   finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
 }
 
-template <typename T, int NT, int VPT>
-__global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
+template <typename T, int NT, int VPT, bool MANY>
+__global__ __launch_bounds__(NT, VPT <= 8 ? 8 : 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
                                                                int cap, SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
-  __shared__ SegLds<NT> l;
+  __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
   const int seg = blockIdx.y, nseg = gridDim.y;
   const float temp = args.temps ? args.temps[t] : args.temperature;
@@ -1103,7 +1127,7 @@ __global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restri
   sg.load(row, V, seg, nseg);
   uint64_t level;
   ExpSum rest;
-  const int n = collect<T, NT, VPT, true>(sg, row, K, cap, c, l, level, rest);
+  const int n = collect<T, NT, VPT, true, MANY>(sg, row, K, cap, c, l, level, rest);
   rest = block_exp_sum<NT>(rest, c, l.red);
   const int64_t at = t * nseg + seg;
   for (int i = threadIdx.x; i < n; i += NT) lists[at * cap + i] = l.list[i];
@@ -1808,12 +1832,11 @@ int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, 
     SegHead* heads = (SegHead*)ws;
     uint64_t* lists = (uint64_t*)(heads + (int64_t)n * cut.nseg);
     const dim3 grid(n, cut.nseg);
-    if (cut.nt == 64)
-      hipLaunchKernelGGL((top_segment_kernel<T, 64, 4>), grid, dim3(64), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
-    else if (cut.vpt == 4)
-      hipLaunchKernelGGL((top_segment_kernel<T, 256, 4>), grid, dim3(256), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
-    else
-      hipLaunchKernelGGL((top_segment_kernel<T, 256, 16>), grid, dim3(256), 0, s, x, ld, V, k, cut.cap, tau, values, ids, rest, heads, lists);
+    by_cut(cut, [&](auto nt, auto vpt, auto many) {
+      constexpr int NT = decltype(nt)::value;
+      hipLaunchKernelGGL((top_segment_kernel<T, NT, decltype(vpt)::value, decltype(many)::value>), grid, dim3(NT), 0, s, x, ld, V, k, cut.cap,
+                         tau, values, ids, rest, heads, lists);
+    });
     if (cut.nseg > 1)
       hipLaunchKernelGGL((top_merge_kernel<T, 256>), dim3(n), dim3(256), 0, s, cut.nseg, k, cut.cap, tau, values, ids, rest, heads, lists);
     return check_launch();
@@ -1834,7 +1857,7 @@ Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
   const bool rows = a.temps || a.ks || a.ps || a.mins;
   const bool by_k = a.top_k > 0 && a.top_k <= MAX_SEG_K && a.top_k < V, large_k = a.top_k > MAX_SEG_K && a.top_k < V;
   const bool ends = by_k || (!large_k && a.top_p < 1.f) || a.min_p > 0.f || a.temperature == 0.f;
-  if (!rows && !ends) return {0, 0, 0, 0};
+  if (!rows && !ends) return {0, 0, 0, 0, false};
   return cut_rows(dtype, T, V, sample_k(a.ks ? 0 : a.top_k));
 }
 
@@ -1851,12 +1874,12 @@ int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int 
     uint64_t* lists = (uint64_t*)(heads + (int64_t)n * cut.nseg);
     const dim3 grid(n, cut.nseg);
     const int K = sample_k(a.ks ? 0 : a.top_k);
-    if (cut.nt == 64)
-      hipLaunchKernelGGL((sample_segment_kernel<T, 64, 4>), grid, dim3(64), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
-    else if (cut.nt && cut.vpt == 4)
-      hipLaunchKernelGGL((sample_segment_kernel<T, 256, 4>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
-    else if (cut.nt)
-      hipLaunchKernelGGL((sample_segment_kernel<T, 256, 16>), grid, dim3(256), 0, s, x, ld, V, a, K, cut.cap, heads, lists);
+    if (cut.nt)
+      by_cut(cut, [&](auto nt, auto vpt, auto many) {
+        constexpr int NT = decltype(nt)::value;
+        hipLaunchKernelGGL((sample_segment_kernel<T, NT, decltype(vpt)::value, decltype(many)::value>), grid, dim3(NT), 0, s, x, ld, V, a, K,
+                           cut.cap, heads, lists);
+      });
     if (cut.nt)
       hipLaunchKernelGGL((sample_list_kernel<T, 256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
     const bool settled = cut.nt && !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K;  // the lists hold the first k
