@@ -144,9 +144,9 @@ __device__ __forceinline__ double exp2_f64(double t) {
 
 // ------------------------------------------------------------------ the largest entries of a segment of a row, kept in registers
 // A row is cut into segments of NT * VPT 16-byte vectors; a workgroup loads one whole segment into registers (all its loads in
-// flight at once) and reads it once.  Each thread's vectors form four groups; the K-th largest of the NT * 4 group maxima is a
-// lower bound of the segment's K-th largest entry and not far below it (64 of 1024 maxima leave about 70 entries above the
-// bound), found by eight rounds of counting on the upper 16 bits of their keys.  Vectors with an entry above the bound go to
+// flight at once) and reads it once.  The K-th largest of the threads' maxima is a lower bound of the segment's K-th largest entry
+// and not far below it (64 of 256 maxima leave about 75 entries above the bound, 128 about 180; above that each thread's vectors
+// form four groups), found by eight rounds of counting on the upper 16 bits of their keys.  Vectors with an entry above the bound go to
 // LDS, all others into the sum of exponentials.  Where too many entries tie at the bound, the exact K-th key is found by
 // bisection over the segment instead.
 constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
@@ -180,6 +180,27 @@ template <int E, bool KEEP_NAN = false> __device__ __forceinline__ void exp_sum_
   }
   a.s = a.s * __builtin_amdgcn_exp2f((a.m - m) * c) + s;
   a.m = m;
+}
+// The same sum for entries of one set with a fixed reference m, an entry of the set: one multiply-add, one exponential and one
+// addition per entry.  m c is rounded once (mc) and the sum corrected by the difference at the end.  Entries far above m overflow
+// it: then ok() is false and the caller takes the way above, as where there is no usable m.
+struct FixedSum {
+  float m, mc, s, c;
+  __device__ __forceinline__ FixedSum(float reference, float scale) : m(reference), mc(reference * scale), s(0.f), c(scale) {}
+  __device__ __forceinline__ bool ok() const { return fabsf(mc) < 1e30f && s < INFINITY; }  // (false for NaN)
+  template <int E> __device__ __forceinline__ void add(const float (&o)[E]) {
+    float t[2] = {0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) t[e & 1] += __builtin_amdgcn_exp2f(fmaf(o[e], c, -mc));
+    s += t[0] + t[1];
+  }
+  __device__ __forceinline__ ExpSum end() const { return {m, s * __builtin_amdgcn_exp2f(-fmaf(m, c, -mc))}; }
+};
+// 16 bytes of a row that is read once: past the caches (6.4 TB/s against 5.6 of ordinary loads, 256 MB).
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+  const u4 v = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ void exp_sum_one(ExpSum& a, float x, float c) {
   const float o[1] = {x};
@@ -256,7 +277,7 @@ template <typename T, int NT, int VPT> struct Segment {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       d[j] = make_uint4(none, none, none, none);
-      if (has(j)) d[j] = *reinterpret_cast<const uint4*>(row + index(j));
+      if (has(j)) d[j] = load_once(row + index(j));
     }
     end_at[0] = seg == 0 && (int)threadIdx.x < head ? (int)threadIdx.x : -1;
     end_at[1] = seg == nseg - 1 && (int)threadIdx.x < V - tail ? tail + (int)threadIdx.x : -1;
@@ -290,23 +311,29 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
                                        ExpSum& rest) {
   constexpr int E = Segment<T, NT, VPT>::E, STAGE = SegLds<NT, MANY>::STAGE, LIST = SegLds<NT, MANY>::LIST;
   uint64_t* list = l.list;
-  float gm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  constexpr int GROUPS = MANY ? 4 : 1;  // of a thread's vectors
+  float gm[GROUPS], low = INFINITY;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) gm[g] = -INFINITY;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     float o[E];
     unpack(sg.d[j], o);
-    gm[j & 3] = vec_max<E>(o, gm[j & 3]);
+    const float vm = vec_max<E>(o);
+    gm[j % GROUPS] = max3(gm[j % GROUPS], gm[j % GROUPS], vm);
+    low = sg.has(j) && vm < low ? vm : low;
   }
   gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
-  uint32_t mk[4];
+  uint32_t mk[GROUPS];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
+  for (int g = 0; g < GROUPS; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
   if (threadIdx.x == 0) l.n_vec = 0, l.n = 0;
-  const uint32_t bound = kth_bound<NT>(mk, 4, K, 30, 16, l.counts);
+  const uint32_t bound = kth_bound<NT>(mk, GROUPS, K, 30, 16, l.counts);
   const float thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
-  rest = {-FLT_MAX, 0.f};
   __syncthreads();
   sg.fresh();
+  // the sum over vectors without an entry above the bound: against the smallest of the vectors' maxima if that is one of them
+  FixedSum sum(low < thr && low > -INFINITY ? low : INFINITY, c);
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     float o[E];
@@ -319,7 +346,19 @@ __device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, in
         l.at[p] = sg.index(j);
       }
     } else {
-      exp_sum_vec<E>(rest, o, vm, c);
+      sum.template add<E>(o);
+    }
+  }
+  rest = sum.end();
+  if (!sum.ok()) {  // (vectors without an entry above -inf or all with one above the bound, entries far apart, NaN)
+    rest = {-FLT_MAX, 0.f};
+    sg.fresh();
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      float o[E];
+      unpack(sg.d[j], o);
+      const float vm = vec_max<E>(o);
+      if (!(vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j))) exp_sum_vec<E>(rest, o, vm, c);
     }
   }
   auto take = [&](float x, int i) {
@@ -449,7 +488,7 @@ __device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float t
 }
 
 template <typename T, int NT, int VPT, bool MANY>
-__global__ __launch_bounds__(NT, VPT <= 8 ? 8 : 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
+__global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
                                                          T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest_out,
                                                          SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
   __shared__ SegLds<NT, MANY> l;
@@ -601,7 +640,7 @@ Cut cut_rows(int dtype, int T, int V, int K) {
   if (K > MAX_SEG_K || V <= 64) return {0, 0, 0, 0, false};
   const bool many = K > 128;
   const int vecs = V / (dtype == PG_F32 ? 4 : 8);
-  const int shapes[3][2] = {{64, 4}, {256, 4}, {256, many ? 16 : 8}};
+  const int shapes[3][2] = {{64, 4}, {256, 4}, {256, 16}};
   for (int i = many ? 1 : 0; i < 3; ++i) {
     const int per = shapes[i][0] * shapes[i][1], nseg = vecs <= per ? 1 : (vecs + per - 1) / per;
     if (nseg > 1 && i < 2) {
@@ -623,7 +662,7 @@ template <typename F> void by_cut(const Cut& c, F f) {
   else if (c.vpt == 4 && c.many) f(Int<256>(), Int<4>(), Bool<true>());
   else if (c.vpt == 4) f(Int<256>(), Int<4>(), Bool<false>());
   else if (c.many) f(Int<256>(), Int<16>(), Bool<true>());
-  else f(Int<256>(), Int<8>(), Bool<false>());
+  else f(Int<256>(), Int<16>(), Bool<false>());
 }
 
 // ------------------------------------------------------------------ sampling
@@ -1115,7 +1154,7 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
 }
 
 template <typename T, int NT, int VPT, bool MANY>
-__global__ __launch_bounds__(NT, VPT <= 8 ? 8 : 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
+__global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
                                                                int cap, SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
   __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
@@ -1204,24 +1243,45 @@ template <typename T> struct Span {
   __device__ __forceinline__ bool owns(int i) const {
     return i < head ? first : i >= tail ? last : i >= head + v0 * E && i < head + v1 * E;
   }
-  // vec(o, v) over the vectors, four in flight per thread (begin() sends the first off); one(i) over the odd elements
-  template <int NT> __device__ __forceinline__ void begin(const T* row, uint4 (&d)[4]) const {
+  // vec(o, v) over the vectors, one(i) over the odd elements.  A wave takes 4 KB at a time, four vectors a lane from one address;
+  // the next four are on their way while these are worked on (begin() sends the first off).
+  static constexpr int U = 4;
+  __device__ __forceinline__ int vector(int tile, int u) const { return v0 + tile * U + (int)(threadIdx.x & ~63u) * U + u * 64 + (int)(threadIdx.x & 63); }
+  template <bool ONCE> static __device__ __forceinline__ uint4 get(const uint4* p) { return ONCE ? load_once(p) : *p; }
+  template <int NT, bool ONCE> __device__ __forceinline__ void begin(const T* row, uint4 (&d)[U]) const {
     const uint4* p = reinterpret_cast<const uint4*>(row + head);
-    if (v0 + (int)threadIdx.x < v1)
+    if ((v1 - v0) >= NT * U)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) d[u] = p[min(v0 + (int)threadIdx.x + u * NT, v1 - 1)];
+      for (int u = 0; u < U; ++u) d[u] = get<ONCE>(p + vector(0, u));
   }
-  template <int NT, typename F, typename G> __device__ __forceinline__ void each(const T* row, int V, uint4 (&d)[4], F vec, G one) const {
+  template <int NT, bool ONCE, typename F, typename G> __device__ __forceinline__ void each(const T* row, int V, uint4 (&d)[U], F vec, G one) const {
     const uint4* p = reinterpret_cast<const uint4*>(row + head);
-    if (v0 + (int)threadIdx.x < v1) {
-#pragma unroll 1
-      for (int v = v0 + threadIdx.x; v < v1; v += NT) {
+    const int tiles = (v1 - v0) / (NT * U);
+    uint4 n[U];
+    auto work = [&](const uint4 (&x)[U], int tile) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
         float o[E];
-        unpack(d[0], o);
-        d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
-        d[3] = p[min(v + 4 * NT, v1 - 1)];
-        vec(o, v);
+        unpack(x[u], o);
+        vec(o, vector(tile, u));
       }
+    };
+#pragma unroll 1
+    for (int i = 0; i < tiles; i += 2) {
+      if (i + 1 < tiles)
+#pragma unroll
+        for (int u = 0; u < U; ++u) n[u] = get<ONCE>(p + vector((i + 1) * NT, u));
+      work(d, i * NT);
+      if (i + 2 < tiles)
+#pragma unroll
+        for (int u = 0; u < U; ++u) d[u] = get<ONCE>(p + vector((i + 2) * NT, u));
+      if (i + 1 < tiles) work(n, (i + 1) * NT);
+    }
+#pragma unroll 1
+    for (int v = v0 + tiles * NT * U + threadIdx.x; v < v1; v += NT) {
+      float o[E];
+      unpack(get<ONCE>(p + v), o);
+      vec(o, v);
     }
     if (first && (int)threadIdx.x < head) one((int)threadIdx.x);
     if (last && tail + (int)threadIdx.x < V) one(tail + (int)threadIdx.x);
@@ -1236,8 +1296,8 @@ template <typename T, int NT>
 __device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>& sp, const T* values, const int32_t* ids, int K, bool tail,
                                               float c, uint32_t* member, int* repeated) {
   constexpr int E = Span<T>::E;
-  uint4 d[4];
-  sp.template begin<NT>(row, d);
+  uint4 d[Span<T>::U];
+  sp.template begin<NT, false>(row, d);
   const int start = sp.head + sp.v0 * E - E;  // element of bit 0: a vector's worth before the segment, for the odd elements in front
   if (tail) {
     const int bits = (sp.v1 - sp.v0 + 2) * E;
@@ -1252,23 +1312,45 @@ __device__ __forceinline__ ExpSum distill_sum(const T* row, int V, const Span<T>
     __syncthreads();
   }
   const uint8_t* bytes = reinterpret_cast<const uint8_t*>(member);
-  ExpSum o = {-FLT_MAX, 0.f};
-  sp.template each<NT>(row, V, d, [&](const float (&x)[E], int v) {
+  auto outside = [&](const float (&x)[E], int v, float (&y)[E]) {  // the vector without the list's tokens
     const int at = v - sp.v0 + 1;
     const uint32_t in = tail ? (E == 8 ? bytes[at] : bytes[at >> 1] >> (at & 1) * 4 & 15) : 0;
-    if (in == 0) {
-      exp_sum_vec<E, true>(o, x, vec_max<E>(x), c);
-    } else {
-      float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = x[e];
+    if (in)
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] = in >> e & 1 ? -INFINITY : x[e];
-      exp_sum_vec<E, true>(o, y, vec_max<E>(y), c);
-    }
-  }, [&](int i) {
+  };
+  // the reference of the thread's sum: its first vector's largest entry outside the list
+  float m = INFINITY;
+  if (sp.v1 - sp.v0 >= NT * Span<T>::U) {
+    float x[E], y[E];
+    unpack(d[0], x);
+    outside(x, sp.vector(0, 0), y);
+    m = vec_max<E>(y);
+  }
+  FixedSum sum(m, c);
+  ExpSum ends = {-FLT_MAX, 0.f};
+  auto one = [&](int i) {
     const int b = i - start;
-    if (!tail || !(member[b >> 5] >> (b & 31) & 1)) exp_sum_add(o, to_f32<T>(row[i]), c);
-  });
-  return o;
+    if (!tail || !(member[b >> 5] >> (b & 31) & 1)) exp_sum_add(ends, to_f32<T>(row[i]), c);
+  };
+  sp.template each<NT, false>(row, V, d, [&](const float (&x)[E], int v) {
+    float y[E];
+    outside(x, v, y);
+    sum.template add<E>(y);
+  }, one);
+  ExpSum o = sum.end();
+  if (!sum.ok()) {  // short segments, entries far apart, NaN
+    o = {-FLT_MAX, 0.f};
+    sp.template begin<NT, false>(row, d);
+    sp.template each<NT, false>(row, V, d, [&](const float (&x)[E], int v) {
+      float y[E];
+      outside(x, v, y);
+      exp_sum_vec<E, true>(o, y, vec_max<E>(y), c);
+    }, [](int) {});
+  }
+  return ends.s == 0.f ? o : exp_sum_join(o, ends, c);
 }
 
 // One entry of the teacher's list per thread, loaded before the pass over the row (longer lists: the rest in loops).
@@ -1358,9 +1440,9 @@ __device__ __forceinline__ void distill_grad(const T* row, int V, const Span<T>&
     return;
   }
   auto grad = [&](float x) { return __builtin_amdgcn_exp2f((x - mo) * c) * co; };
-  uint4 d[4];
-  sp.template begin<NT>(row, d);
-  sp.template each<NT>(row, V, d, [&](const float (&x)[E], int v) {
+  uint4 d[Span<T>::U];
+  sp.template begin<NT, true>(row, d);
+  sp.template each<NT, true>(row, V, d, [&](const float (&x)[E], int v) {
     float g[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) g[e] = grad(x[e]);

@@ -139,19 +139,20 @@ def compute_gradient_penalty(critic, real_data, fake_data, real_mask, fake_mask,
 
 class _DistillFn(torch.autograd.Function):
     """Forward: row losses and eight numbers per row (pg_distill_fwd); backward: one pass that reads the logits again and writes
-    their gradient (pg_distill_bwd)."""
+    their gradient (pg_distill_bwd), on the arguments the forward has checked."""
 
     @staticmethod
     def forward(ctx, logits, values, ids, rest, weights, temperature):
-        loss, stash = ops.distill_fwd(logits, values, ids, rest, weights, temperature)
-        ctx.save_for_backward(logits, values, ids, weights, stash)
-        ctx.temperature = temperature
+        call = ops._distill_args(logits, values, ids, rest, weights, temperature)
+        loss, stash = ops._distill_fwd(logits, call)
+        ctx.save_for_backward(logits, call[5], call[6], call[8], stash)
+        ctx.call = call[:5] + call[9:]
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
         logits, values, ids, weights, stash = ctx.saved_tensors
-        grad = ops.distill_bwd(logits, values, ids, stash, dloss, weights, ctx.temperature)
+        grad = ops._distill_bwd(logits, ctx.call, values, ids, weights, stash, dloss)
         if torch.is_grad_enabled():  # (create_graph)
             grad = _NoSecondDerivative.apply(grad, logits, dloss)
         return grad, None, None, None, None, None

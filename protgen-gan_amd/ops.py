@@ -242,6 +242,7 @@ def _rows(x, what="logits"):
 _top_bytes = functools.lru_cache(maxsize=1024)(lib.pg_top_logits_workspace_bytes)
 _sample_bytes = functools.lru_cache(maxsize=1024)(lib.pg_sample_filtered_workspace_bytes)
 _distill_bytes = functools.lru_cache(maxsize=1024)(lib.pg_distill_workspace_bytes)
+_STASH = lib.pg_distill_stash_floats()
 # (torch.cuda.current_stream builds an object a call, 2 us of the 12 a small call takes on the host)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
@@ -373,11 +374,10 @@ def _distill_args(logits, values, ids, rest, weights, temperature):
     return dt, T, V, ld, k, values, ids, rest, weights, temperature
 
 
-def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
-    """Row losses of loss.distillation_loss (fp32 [...]) and the stash distill_bwd needs."""
-    dt, T, V, ld, k, values, ids, rest, weights, temperature = _distill_args(logits, values, ids, rest, weights, temperature)
+def _distill_fwd(logits, call):
+    dt, T, V, ld, k, values, ids, rest, weights, temperature = call
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
-    stash = torch.empty(T * lib.pg_distill_stash_floats(), dtype=torch.float32, device=logits.device)
+    stash = torch.empty(T * _STASH, dtype=torch.float32, device=logits.device)
     if T:
         _launch(logits, "pg_distill_fwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(rest),
                                            ptr(weights), temperature, loss.data_ptr(), stash.data_ptr()),
@@ -385,16 +385,27 @@ def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
     return loss, stash
 
 
-def distill_bwd(logits, values, ids, stash, dloss, weights=None, temperature=1.0):
-    """d sum(dloss * loss) / d logits, contiguous, in the logits' type.  `stash` from distill_fwd on the same arguments."""
-    dt, T, V, ld, k, values, ids, _, weights, temperature = _distill_args(logits, values, ids, None, weights, temperature)
-    _same(logits, "dloss", dloss, torch.float32, logits.shape[:-1])
+def _distill_bwd(logits, call, values, ids, weights, stash, dloss):
+    dt, T, V, ld, k, temperature = call
     dloss = dloss.contiguous()
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if T:
         _launch(logits, "pg_distill_bwd", (dt, logits.data_ptr(), ld, T, V, values.data_ptr(), ids.data_ptr(), k, ptr(weights),
                                            temperature, dloss.data_ptr(), stash.data_ptr(), out.data_ptr(), V), None)
     return out
+
+
+def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
+    """Row losses of loss.distillation_loss (fp32 [...]) and the stash distill_bwd needs."""
+    return _distill_fwd(logits, _distill_args(logits, values, ids, rest, weights, temperature))
+
+
+def distill_bwd(logits, values, ids, stash, dloss, weights=None, temperature=1.0):
+    """d sum(dloss * loss) / d logits, contiguous, in the logits' type.  `stash` from distill_fwd on the same arguments."""
+    call = _distill_args(logits, values, ids, None, weights, temperature)
+    _same(logits, "dloss", dloss, torch.float32, logits.shape[:-1])
+    _same(logits, "stash", stash, torch.float32, (call[1] * _STASH,))
+    return _distill_bwd(logits, call[:5] + call[9:], call[5], call[6], call[8], stash, dloss)
 
 
 def distill_loss_grad(logits, values, ids, rest=None, temperature=1.0, weights=None):
