@@ -139,11 +139,10 @@ def compute_gradient_penalty(critic, real_data, fake_data, real_mask, fake_mask,
 
 class _DistillFn(torch.autograd.Function):
     """Forward: row losses and eight numbers per row (pg_distill_fwd); backward: one pass that reads the logits again and writes
-    their gradient (pg_distill_bwd), on the arguments the forward has checked."""
+    their gradient (pg_distill_bwd).  `call`: the checked arguments (a tuple: apply() looks at every tensor it is given)."""
 
     @staticmethod
-    def forward(ctx, logits, values, ids, rest, weights, temperature):
-        call = ops._distill_args(logits, values, ids, rest, weights, temperature)
+    def forward(ctx, logits, call):
         loss, stash = ops._distill_fwd(logits, call)
         ctx.save_for_backward(logits, call[5], call[6], call[8], stash)
         ctx.call = call[:5] + call[9:]
@@ -155,7 +154,7 @@ class _DistillFn(torch.autograd.Function):
         grad = ops._distill_bwd(logits, ctx.call, values, ids, weights, stash, dloss)
         if torch.is_grad_enabled():  # (create_graph)
             grad = _NoSecondDerivative.apply(grad, logits, dloss)
-        return grad, None, None, None, None, None
+        return grad, None
 
 
 class _NoSecondDerivative(torch.autograd.Function):
@@ -181,4 +180,4 @@ def distillation_loss(student_logits, top_values, top_ids, rest=None, temperatur
     gradient, whatever they hold.  Differentiable in student_logits, once; ids outside the vocabulary (-1) mark absent entries."""
     if top_values.requires_grad or (rest is not None and rest.requires_grad) or (weights is not None and weights.requires_grad):
         raise ValueError("top_values, rest and weights must not require a gradient: the loss is differentiable in the student's logits")
-    return _DistillFn.apply(student_logits, top_values, top_ids, rest, weights, float(temperature))
+    return _DistillFn.apply(student_logits, ops._distill_args(student_logits, top_values, top_ids, rest, weights, temperature))
