@@ -266,21 +266,24 @@ template <typename T, int NT, int VPT> struct Segment {
 
   __device__ __forceinline__ int index(int j) const { return base + (j * NT + (int)threadIdx.x) * E; }
   __device__ __forceinline__ bool has(int j) const { return j * NT + (int)threadIdx.x < nv; }
-  __device__ __forceinline__ void load(const T* row, int V, int seg, int nseg) {
+  __device__ __forceinline__ void place(const T* row, int V, int seg, int nseg) {
     int head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
     if (head > V) head = V;
     const int all = (V - head) / E, tail = head + all * E;
     base = head + seg * VECS * E;
     nv = all - seg * VECS;
     nv = nv < 0 ? 0 : nv > VECS ? VECS : nv;
+    end_at[0] = seg == 0 && (int)threadIdx.x < head ? (int)threadIdx.x : -1;
+    end_at[1] = seg == nseg - 1 && (int)threadIdx.x < V - tail ? tail + (int)threadIdx.x : -1;
+  }
+  __device__ __forceinline__ void load(const T* row, int V, int seg, int nseg) {
+    place(row, V, seg, nseg);
     const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       d[j] = make_uint4(none, none, none, none);
       if (has(j)) d[j] = load_once(row + index(j));
     }
-    end_at[0] = seg == 0 && (int)threadIdx.x < head ? (int)threadIdx.x : -1;
-    end_at[1] = seg == nseg - 1 && (int)threadIdx.x < V - tail ? tail + (int)threadIdx.x : -1;
 #pragma unroll
     for (int i = 0; i < 2; ++i) ends[i] = end_at[i] >= 0 ? to_f32<T>(row[end_at[i]]) : -INFINITY;
   }
@@ -289,139 +292,160 @@ template <typename T, int NT, int VPT> struct Segment {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) asm volatile("" : "+v"(d[j].x), "+v"(d[j].y), "+v"(d[j].z), "+v"(d[j].w));
   }
-  // f(value, index) over this thread's entries, read again from memory (a loop over the registers would have to be unrolled)
-  template <typename F> __device__ __forceinline__ void entries(const T* row, F f) const {
+  // f(value, index) over this thread's entries of segments seg .. seg + count - 1, read again from memory
+  template <typename F> static __device__ __forceinline__ void entries(const T* row, int V, int seg, int count, int nseg, F f) {
 #pragma unroll 1
-    for (int j = 0; j < VPT && has(j); ++j) {
-      float o[E];
-      unpack(*reinterpret_cast<const uint4*>(row + index(j)), o);
+    for (int s = seg; s < seg + count; ++s) {
+      Segment at;
+      at.place(row, V, s, nseg);
+#pragma unroll 1
+      for (int j = 0; j < VPT && at.has(j); ++j) {
+        float o[E];
+        unpack(*reinterpret_cast<const uint4*>(row + at.index(j)), o);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(o[e], index(j) + e);
+        for (int e = 0; e < E; ++e) f(o[e], at.index(j) + e);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (at.end_at[i] >= 0) f(to_f32<T>(row[at.end_at[i]]), at.end_at[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (end_at[i] >= 0) f(ends[i], end_at[i]);
   }
 };
 
-// Leaves the keys of the segment's largest entries in list (n of them, at most cap, in no order; at least K if it has as many),
-// the sum over its other entries in rest (per thread), and the level.  FINITE: entries of -inf are never listed.
+// Leaves the keys of the largest entries of segments seg .. seg + count - 1 (of nseg in the row) in l.list (n of them, at most cap,
+// in no order; at least K if there are as many), the sum over the other entries in rest (per thread), and the level.  FINITE:
+// entries of -inf are never listed.  Over several segments the threads' maxima, and with them the bound, run on.
 template <typename T, int NT, int VPT, bool FINITE, bool MANY>
-__device__ __forceinline__ int collect(Segment<T, NT, VPT>& sg, const T* row, int K, int cap, float c, SegLds<NT, MANY>& l, uint64_t& level,
-                                       ExpSum& rest) {
-  constexpr int E = Segment<T, NT, VPT>::E, STAGE = SegLds<NT, MANY>::STAGE, LIST = SegLds<NT, MANY>::LIST;
+__device__ __forceinline__ int collect(const T* row, int V, int seg, int count, int nseg, int K, int cap, float c, SegLds<NT, MANY>& l,
+                                       uint64_t& level, ExpSum& rest) {
+  typedef Segment<T, NT, VPT> Seg;
+  constexpr int E = Seg::E, STAGE = SegLds<NT, MANY>::STAGE, LIST = SegLds<NT, MANY>::LIST;
   uint64_t* list = l.list;
   constexpr int GROUPS = MANY ? 4 : 1;  // of a thread's vectors
-  float gm[GROUPS], low = INFINITY;
+  Seg sg;
+  sg.load(row, V, seg, nseg);
+  float gm[GROUPS], thr = -INFINITY;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) gm[g] = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    float o[E];
-    unpack(sg.d[j], o);
-    const float vm = vec_max<E>(o);
-    gm[j % GROUPS] = max3(gm[j % GROUPS], gm[j % GROUPS], vm);
-    low = sg.has(j) && vm < low ? vm : low;
-  }
-  gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
-  uint32_t mk[GROUPS];
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
-  if (threadIdx.x == 0) l.n_vec = 0, l.n = 0;
-  const uint32_t bound = kth_bound<NT>(mk, GROUPS, K, 30, 16, l.counts);
-  const float thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
-  __syncthreads();
-  sg.fresh();
-  // the sum over vectors without an entry above the bound: against the smallest of the vectors' maxima if that is one of them
-  FixedSum sum(low < thr && low > -INFINITY ? low : INFINITY, c);
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    float o[E];
-    unpack(sg.d[j], o);
-    const float vm = vec_max<E>(o);
-    if (vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j)) {
-      const uint32_t p = atomicAdd(&l.n_vec, 1u);
-      if (p < STAGE) {
-        l.vec[p] = sg.d[j];
-        l.at[p] = sg.index(j);
-      }
-    } else {
-      sum.template add<E>(o);
-    }
-  }
-  rest = sum.end();
-  if (!sum.ok()) {  // (vectors without an entry above -inf or all with one above the bound, entries far apart, NaN)
-    rest = {-FLT_MAX, 0.f};
+  rest = {-FLT_MAX, 0.f};
+  bool over = false;
+  if (threadIdx.x == 0) l.n = 0;
+#pragma unroll 1
+  for (int s = 0;; ++s) {
+    float low = INFINITY;
     sg.fresh();
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       float o[E];
       unpack(sg.d[j], o);
       const float vm = vec_max<E>(o);
-      if (!(vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j))) exp_sum_vec<E>(rest, o, vm, c);
+      gm[j % GROUPS] = max3(gm[j % GROUPS], gm[j % GROUPS], vm);
+      low = sg.has(j) && vm < low ? vm : low;
     }
-  }
-  auto take = [&](float x, int i) {
-    x = fmaxf(x, -INFINITY);
-    const bool in = x >= thr && (!FINITE || x > -INFINITY);
-    if (in) {
-      const uint32_t p = atomicAdd(&l.n, 1u);
-      if (p < LIST) list[p] = entry_key(x, i);
+    gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
+    uint32_t mk[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
+    if (threadIdx.x == 0) l.n_vec = 0;
+    const uint32_t bound = kth_bound<NT>(mk, GROUPS, K, 30, 16, l.counts);
+    thr = bound > 0x007fffffu ? key_value(bound) : -INFINITY;
+    __syncthreads();
+    sg.fresh();
+    // the sum over vectors without an entry above the bound: against the smallest of the vectors' maxima if that is one of them
+    FixedSum sum(low < thr && low > -INFINITY ? low : INFINITY, c);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      float o[E];
+      unpack(sg.d[j], o);
+      const float vm = vec_max<E>(o);
+      if (vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j)) {
+        const uint32_t p = atomicAdd(&l.n_vec, 1u);
+        if (p < STAGE) {
+          l.vec[p] = sg.d[j];
+          l.at[p] = sg.index(j);
+        }
+      } else {
+        sum.template add<E>(o);
+      }
     }
-    return in;
-  };
+    ExpSum part = sum.end();
+    if (!sum.ok()) {  // (vectors without an entry above -inf or all with one above the bound, entries far apart, NaN)
+      part = {-FLT_MAX, 0.f};
+      sg.fresh();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (sg.end_at[i] >= 0 && !take(sg.ends[i], sg.end_at[i])) exp_sum_one(rest, sg.ends[i], c);
-  __syncthreads();
-  const int n_vec = l.n_vec, staged = n_vec < STAGE ? n_vec : STAGE;
-  float most = -INFINITY;  // the largest entry that a vector with a listed one brings along
-  for (int i = threadIdx.x; i < staged; i += NT) {
-    float o[E];
-    unpack(l.vec[i], o);
+      for (int j = 0; j < VPT; ++j) {
+        float o[E];
+        unpack(sg.d[j], o);
+        const float vm = vec_max<E>(o);
+        if (!(vm >= thr && (!FINITE || vm > -INFINITY) && sg.has(j))) exp_sum_vec<E>(part, o, vm, c);
+      }
+    }
+    rest = s == 0 ? part : exp_sum_join(rest, part, c);
+    auto take = [&](float x, int i) {
+      x = fmaxf(x, -INFINITY);
+      const bool in = x >= thr && (!FINITE || x > -INFINITY);
+      if (in) {
+        const uint32_t p = atomicAdd(&l.n, 1u);
+        if (p < LIST) list[p] = entry_key(x, i);
+      }
+      return in;
+    };
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (!take(o[e], l.at[i] + e)) most = fmaxf(most, o[e]);
-  }
-  most = block_max<NT>(most, l.red);
-  if (most > -INFINITY) {  // the staged vectors are in no fixed order: their sum is one of whole multiples of 2^-40 of the largest
-    uint64_t sum = 0;
+    for (int i = 0; i < 2; ++i)
+      if (sg.end_at[i] >= 0 && !take(sg.ends[i], sg.end_at[i])) exp_sum_one(rest, sg.ends[i], c);
+    if (s + 1 < count) sg.load(row, V, seg + s + 1, nseg);  // (on its way while the staged vectors are looked through)
+    __syncthreads();
+    const int n_vec = l.n_vec, staged = n_vec < STAGE ? n_vec : STAGE;
+    float most = -INFINITY;  // the largest entry that a vector with a listed one brings along
     for (int i = threadIdx.x; i < staged; i += NT) {
       float o[E];
       unpack(l.vec[i], o);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (o[e] < thr) sum += fixed_weight(o[e], most, c);
+        if (!take(o[e], l.at[i] + e)) most = fmaxf(most, o[e]);
     }
-    sum = block_all<NT>(sum, l.wave, [](uint64_t a, uint64_t b) { return a + b; });
-    if (threadIdx.x == 0) rest = exp_sum_join(rest, {most, (float)sum * 0x1p-40f}, c);
+    most = block_max<NT>(most, l.red);
+    if (most > -INFINITY) {  // the staged vectors are in no fixed order: their sum is one of whole multiples of 2^-40 of the largest
+      uint64_t sum = 0;
+      for (int i = threadIdx.x; i < staged; i += NT) {
+        float o[E];
+        unpack(l.vec[i], o);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (o[e] < thr) sum += fixed_weight(o[e], most, c);
+      }
+      sum = block_all<NT>(sum, l.wave, [](uint64_t a, uint64_t b) { return a + b; });
+      if (threadIdx.x == 0) rest = exp_sum_join(rest, {most, (float)sum * 0x1p-40f}, c);
+    }
+    __syncthreads();
+    over = over || n_vec > STAGE;
+    if (s + 1 == count) break;
   }
-  __syncthreads();
   int n = l.n;
   level = thr > -INFINITY ? (uint64_t)value_key(thr) << 32 : 0;
-  if (n_vec > STAGE || n > cap) {  // too many at the bound: the K-th key itself, bit by bit
-    auto count = [&](auto in) {
+  if (over || n > cap) {  // too many at the bound: the K-th key itself, bit by bit
+    auto number = [&](auto in) {
       int k = 0;
-      sg.entries(row, [&](float x, int i) { k += in(x, i); });
+      Seg::entries(row, V, seg, count, nseg, [&](float x, int i) { k += in(x, i); });
       return block_all<NT>(k, reinterpret_cast<int*>(l.red), [](int a, int b) { return a + b; });
     };
     uint32_t vk = 0;
     for (int b = 31; b >= 0; --b) {
       const uint32_t trial = vk | (1u << b);
-      if (count([&](float x, int) { return value_key(x) >= trial; }) >= K) vk = trial;
+      if (number([&](float x, int) { return value_key(x) >= trial; }) >= K) vk = trial;
     }
-    const int above = count([&](float x, int) { return value_key(x) > vk; });
+    const int above = number([&](float x, int) { return value_key(x) > vk; });
     uint32_t low = 0;  // of the entries at the K-th value, the K - above lowest indexes: the largest bound on ~index that keeps them
     for (int b = 31; b >= 0; --b) {
       const uint32_t trial = low | (1u << b);
-      if (count([&](float x, int i) { return value_key(x) == vk && (uint32_t)~i >= trial; }) >= K - above) low = trial;
+      if (number([&](float x, int i) { return value_key(x) == vk && (uint32_t)~i >= trial; }) >= K - above) low = trial;
     }
     level = ((uint64_t)vk << 32) | low;
     rest = {-FLT_MAX, 0.f};
     __syncthreads();
     if (threadIdx.x == 0) l.n = 0;
     __syncthreads();
-    sg.entries(row, [&](float x, int i) {
+    Seg::entries(row, V, seg, count, nseg, [&](float x, int i) {
       const uint64_t k = entry_key(x, i);
       if (k >= level && (!FINITE || x > -INFINITY)) list[atomicAdd(&l.n, 1u)] = k;
       else exp_sum_one(rest, x, c);
@@ -488,19 +512,17 @@ __device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float t
 }
 
 template <typename T, int NT, int VPT, bool MANY>
-__global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, float tau,
+__global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, int count, float tau,
                                                          T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest_out,
                                                          SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
   __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
   const int seg = blockIdx.y, nseg = gridDim.y;
   const float c = (float)(LOG2E / (double)tau);
-  Segment<T, NT, VPT> sg;
   const T* row = logits + t * ld;
-  sg.load(row, V, seg, nseg);
   uint64_t level;
   ExpSum rest;
-  const int n = collect<T, NT, VPT, false, MANY>(sg, row, K, cap, c, l, level, rest);
+  const int n = collect<T, NT, VPT, false, MANY>(row, V, seg * count, count, nseg * count, K, cap, c, l, level, rest);
   if (nseg == 1) {
     top_finish<T, NT>(l.list, n, K, tau, c, rest, l.red, values + t * K, ids + t * K, rest_out + t);
     return;
@@ -634,10 +656,12 @@ __global__ __launch_bounds__(NT) void top_merge_kernel(int nseg, int K, int cap,
   top_finish<T, NT>(l.list, n, K, tau, c, rk.rest, l.red, values + t * K, ids + t * K, rest_out + t);
 }
 
-// How a call is cut: threads and vectors per thread of a segment, segments per row, keys a segment may leave, K above 128.
-struct Cut { int nt, vpt, nseg, cap; bool many; };
+// How a call is cut: threads and vectors per thread of a segment, workgroups per row, keys a workgroup may leave, K above 128,
+// segments a workgroup takes one after the other.
+struct Cut { int nt, vpt, nseg, cap; bool many; int count; };
 Cut cut_rows(int dtype, int T, int V, int K) {
-  if (K > MAX_SEG_K || V <= 64) return {0, 0, 0, 0, false};
+  const Cut none = {0, 0, 0, 0, false, 1};
+  if (K > MAX_SEG_K || V <= 64) return none;
   const bool many = K > 128;
   const int vecs = V / (dtype == PG_F32 ? 4 : 8);
   const int shapes[3][2] = {{64, 4}, {256, 4}, {256, 16}};
@@ -647,13 +671,17 @@ Cut cut_rows(int dtype, int T, int V, int K) {
       // few rows: small segments, to spread them over the chip; many: the next larger ones
       if (i == 0 || (int64_t)T * nseg > 1024) continue;
     }
+    // rows enough for four workgroups a CU: one takes the whole row and joins nothing (1024 x 131072 bf16, k 64: 87 us,
+    // against 105 with four workgroups a row and a launch that joins their lists).  Its
+    // list grows by about 1.2 K / s in segment s
+    if (nseg > 1 && i == 2 && T >= 1024 && 1.4 * K * (1.0 + log((double)nseg)) <= 400.0) return {256, 16, 1, max_cap(K), many, nseg};
     if (nseg > MAX_SEGS) continue;
     int cap = 2 * K + 64;
     if (cap > max_cap(K)) cap = max_cap(K);
     if (cap > MERGE / nseg) cap = MERGE / nseg;
-    if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap, many};
+    if (nseg == 1 || cap >= K + K / 2 + 32) return {shapes[i][0], shapes[i][1], nseg, cap, many, 1};
   }
-  return {0, 0, 0, 0, false};
+  return none;
 }
 template <int N> struct Int { static constexpr int value = N; };
 template <bool B> struct Bool { static constexpr bool value = B; };
@@ -1155,18 +1183,16 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
 
 template <typename T, int NT, int VPT, bool MANY>
 __global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args, int K,
-                                                               int cap, SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
+                                                               int cap, int count, SegHead* __restrict__ heads, uint64_t* __restrict__ lists) {
   __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
   const int seg = blockIdx.y, nseg = gridDim.y;
   const float temp = args.temps ? args.temps[t] : args.temperature;
   const float c = temp > 0.f ? (float)(LOG2E / (double)temp) : 0.f;
   const T* row = logits + t * ld;
-  Segment<T, NT, VPT> sg;
-  sg.load(row, V, seg, nseg);
   uint64_t level;
   ExpSum rest;
-  const int n = collect<T, NT, VPT, true, MANY>(sg, row, K, cap, c, l, level, rest);
+  const int n = collect<T, NT, VPT, true, MANY>(row, V, seg * count, count, nseg * count, K, cap, c, l, level, rest);
   rest = block_exp_sum<NT>(rest, c, l.red);
   const int64_t at = t * nseg + seg;
   for (int i = threadIdx.x; i < n; i += NT) lists[at * cap + i] = l.list[i];
@@ -1917,7 +1943,7 @@ int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, 
     by_cut(cut, [&](auto nt, auto vpt, auto many) {
       constexpr int NT = decltype(nt)::value;
       hipLaunchKernelGGL((top_segment_kernel<T, NT, decltype(vpt)::value, decltype(many)::value>), grid, dim3(NT), 0, s, x, ld, V, k, cut.cap,
-                         tau, values, ids, rest, heads, lists);
+                         cut.count, tau, values, ids, rest, heads, lists);
     });
     if (cut.nseg > 1)
       hipLaunchKernelGGL((top_merge_kernel<T, 256>), dim3(n), dim3(256), 0, s, cut.nseg, k, cut.cap, tau, values, ids, rest, heads, lists);
@@ -1939,7 +1965,7 @@ Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
   const bool rows = a.temps || a.ks || a.ps || a.mins;
   const bool by_k = a.top_k > 0 && a.top_k <= MAX_SEG_K && a.top_k < V, large_k = a.top_k > MAX_SEG_K && a.top_k < V;
   const bool ends = by_k || (!large_k && a.top_p < 1.f) || a.min_p > 0.f || a.temperature == 0.f;
-  if (!rows && !ends) return {0, 0, 0, 0, false};
+  if (!rows && !ends) return {0, 0, 0, 0, false, 1};
   return cut_rows(dtype, T, V, sample_k(a.ks ? 0 : a.top_k));
 }
 
@@ -1960,7 +1986,7 @@ int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int 
       by_cut(cut, [&](auto nt, auto vpt, auto many) {
         constexpr int NT = decltype(nt)::value;
         hipLaunchKernelGGL((sample_segment_kernel<T, NT, decltype(vpt)::value, decltype(many)::value>), grid, dim3(NT), 0, s, x, ld, V, a, K,
-                           cut.cap, heads, lists);
+                           cut.cap, cut.count, heads, lists);
       });
     if (cut.nt)
       hipLaunchKernelGGL((sample_list_kernel<T, 256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
