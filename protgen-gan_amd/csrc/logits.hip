@@ -936,7 +936,7 @@ template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict__ noise, int64_t ld_noise, int V, SampleArgs args,
                                                          int nseg, int cap, const SegHead* __restrict__ heads,
                                                          const uint64_t* __restrict__ lists, int64_t* __restrict__ pred,
-                                                         float* __restrict__ conf) {
+                                                         float* __restrict__ conf, uint64_t* __restrict__ split, int64_t split_words) {
   __shared__ ListLds l;
   const int64_t t = blockIdx.x;
   const float* q = noise + t * ld_noise;
@@ -1031,6 +1031,8 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict
   if (f.min_p > 0.f && (na < nv || whole)) keep = min(keep, na);
   if (!sure || keep > nv) {
     if (threadIdx.x == 0) pred[t] = -2 - (int64_t)arg, conf[t] = m;
+    if (split)
+      for (int i = threadIdx.x; i < split_words; i += NT) split[t * split_words + i] = 0;
     return;
   }
   const double kept_mass = (double)l.mass[keep - 1] * 0x1p-40;
@@ -1045,6 +1047,84 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict
   } else {
     finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
   }
+}
+
+// min_p as the smallest value it leaves; -inf and NaN never race
+__device__ __forceinline__ float least_value(const RowFilter& f, float m) {
+  if (!(f.min_p > 0.f)) return -FLT_MAX;
+  const double x = (double)m + (double)f.temperature * log((double)fminf(f.min_p, 1.f));
+  float least = fmaxf((float)x, -FLT_MAX);
+  if ((double)least < x) least = key_value(value_key(least) + 1);
+  return fminf(least, m);
+}
+__device__ __forceinline__ Bins row_bins(const RowFilter& f, float m) { return Bins(m, (float)BINS / fminf(40.f * f.temperature, 32.f)); }
+
+// The n entries at p, the first of them entry i0 of its row: those before the border race, those at it go to push(key).  A wave
+// first packs a vector's racing entries (each wave its own part of `packs`), so that a few among many do not take the 64-bit work
+// of all; four vectors per thread are on their way meanwhile, and noise is read for the racing entries alone.
+template <typename T, int NT, typename P>
+__device__ __forceinline__ void sweep(const T* p, int n, int i0, const float* q, uint64_t floor, const Border& at, float least, const Weight& weight,
+                                      Race& race, PackedEntry* packs, P push) {
+  constexpr int E = 16 / (int)sizeof(T);
+  PackedEntry* pack = packs + (threadIdx.x >> 6) * 512;
+  int packed = 0;
+  auto look = [&](float x, int i) {  // (by whole waves)
+    bool go = x >= least;
+    if (!(x > at.hi)) {
+      const bool near = x >= at.lo;
+      go = go && near;
+      if (near) {
+        const uint64_t k = entry_key(x, i), digits = k & at.mask;
+        go = go && k >= floor && digits > at.prefix;
+        if (k >= floor && digits == at.prefix) push(k);
+      }
+    }
+    const uint64_t lanes = __ballot(go);
+    if (go) pack[packed + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = {x, i};
+    packed += __popcll(lanes);
+  };
+  auto run = [&]() {
+    if (packed == 0) return;
+    race.screen = wave_max(race.screen);  // (alone, some lane of a wave nearly always has a new best of its own to divide for)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int j = threadIdx.x & 63; j < packed; j += 256) {
+      PackedEntry e[4];
+      float z[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        e[u] = pack[min(j + 64 * u, packed - 1)];
+        z[u] = q[e[u].i];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (j + 64 * u < packed) race.add(weight(e[u].x), e[u].x, z[u], e[u].i);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    packed = 0;
+  };
+  int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
+  if (head > n) head = n;
+  const int nv = (n - head) / E, tail = head + nv * E;
+  const uint4* vec = reinterpret_cast<const uint4*>(p + head);
+  uint4 d[4] = {};
+  if (nv)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) d[u] = vec[min((int)threadIdx.x + u * NT, nv - 1)];
+#pragma unroll 1
+  for (int r0 = 0; r0 < nv; r0 += NT) {
+    const int v = r0 + threadIdx.x;
+    float o[E];
+    unpack(d[0], o);
+    d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
+    d[3] = vec[min(v + 4 * NT, nv - 1)];
+#pragma unroll
+    for (int e = 0; e < E; ++e) look(v < nv ? o[e] : NAN, i0 + head + v * E + e);
+    run();
+  }
+  const int end = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;  // (both ends: less than 2 E entries)
+  look(end < n && (int)threadIdx.x < head + n - tail ? to_f32<T>(p[end]) : NAN, i0 + end);
+  run();
 }
 
 // From the whole row: every row (all), or those sample_list_kernel left.  The border of top-k, then of top-p among those, then
@@ -1082,93 +1162,24 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
     __syncthreads();
   }
   const Weight weight = {m, LOG2E / (double)f.temperature};
-  const Bins bins(m, (float)BINS / fminf(40.f * f.temperature, 32.f));
+  const Bins bins = row_bins(f, m);
   const bool by_k = f.top_k > 0 && f.top_k < V, by_p = f.top_p < 1.f;
-  // min_p as the smallest value it leaves; -inf and NaN never race
-  float least = -FLT_MAX;
-  if (f.min_p > 0.f) {
-    const double x = (double)m + (double)f.temperature * log((double)fminf(f.min_p, 1.f));
-    least = fmaxf((float)x, -FLT_MAX);
-    if ((double)least < x) least = key_value(value_key(least) + 1);
-    least = fminf(least, m);
-  }
+  const float least = least_value(f, m);
   Race race;
-  // The entries before the border race, those at it go to the list.  A wave first packs a vector's racing entries (each wave its
-  // own part of l.pack), so that a few among many do not take the 64-bit work of all; four vectors per thread are on their way
-  // meanwhile, and noise is read for the racing entries alone.
-  auto sweep = [&](uint64_t floor, const Border& at) {
-    constexpr int E = 16 / (int)sizeof(T);
-    PackedEntry* pack = l.pack + (threadIdx.x >> 6) * 512;
-    race = Race();
-    int n = 0;
-    auto look = [&](float x, int i) {  // (by whole waves)
-      bool go = x >= least;
-      if (!(x > at.hi)) {
-        const bool near = x >= at.lo;
-        go = go && near;
-        if (near) {
-          const uint64_t k = entry_key(x, i), digits = k & at.mask;
-          go = go && k >= floor && digits > at.prefix;
-          if (k >= floor && digits == at.prefix) {
-            const uint32_t p = atomicAdd(&l.n, 1u);
-            if (p < POOL) l.list[p] = k;
-          }
-        }
-      }
-      const uint64_t lanes = __ballot(go);
-      if (go) pack[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = {x, i};
-      n += __popcll(lanes);
-    };
-    auto run = [&]() {
-      if (n == 0) return;
-      race.screen = wave_max(race.screen);  // (alone, some lane of a wave nearly always has a new best of its own to divide for)
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-      for (int j = threadIdx.x & 63; j < n; j += 256) {
-        PackedEntry e[4];
-        float z[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          e[u] = pack[min(j + 64 * u, n - 1)];
-          z[u] = q[e[u].i];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (j + 64 * u < n) race.add(weight(e[u].x), e[u].x, z[u], e[u].i);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      n = 0;
-    };
-    int head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
-    if (head > V) head = V;
-    const int nv = (V - head) / E, tail = head + nv * E;
-    const uint4* vec = reinterpret_cast<const uint4*>(row + head);
-    uint4 d[4] = {};
-    if (nv)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) d[u] = vec[min((int)threadIdx.x + u * NT, nv - 1)];
-#pragma unroll 1
-    for (int r0 = 0; r0 < nv; r0 += NT) {
-      const int v = r0 + threadIdx.x;
-      float o[E];
-      unpack(d[0], o);
-      d[0] = d[1]; d[1] = d[2]; d[2] = d[3];
-      d[3] = vec[min(v + 4 * NT, nv - 1)];
-#pragma unroll
-      for (int e = 0; e < E; ++e) look(v < nv ? o[e] : NAN, head + v * E + e);
-      run();
-    }
-    const int end = (int)threadIdx.x < head ? (int)threadIdx.x : tail + (int)threadIdx.x - head;  // (both ends: less than 2 E entries)
-    look(end < V && (int)threadIdx.x < head + V - tail ? to_f32<T>(row[end]) : NAN, end);
-    run();
-  };
   Border at = {BINS, 0, 0, INFINITY, -INFINITY, 0, 0, 0};
 #pragma unroll 1
   for (int last = by_k && by_p ? 0 : 1; last < 2; ++last) {  // one copy of the code for both filters
     const uint64_t floor = at.B;
     auto gather = [&](const Border& a) {
-      if (last) sweep(floor, a);
-      else gather_bin<T, NT>(row, V, floor, a, l);
+      if (last) {
+        race = Race();
+        sweep<T, NT>(row, V, 0, q, floor, a, least, weight, race, l.pack, [&](uint64_t k) {
+          const uint32_t p = atomicAdd(&l.n, 1u);
+          if (p < POOL) l.list[p] = k;
+        });
+      } else {
+        gather_bin<T, NT>(row, V, floor, a, l);
+      }
     };
     at = border<T, NT>(row, V, bins, floor, last && by_p, by_k || by_p ? f.top_k : -1, (double)f.top_p, weight, l, gather);
   }
@@ -1178,6 +1189,140 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
     if (x >= least) race.add(weight(x), x, q[j], j);
   }
   const double kept_mass = block_sum<NT>(race.total, l.redd);
+  finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
+}
+
+// The rows sample_list_kernel left, where there are few rows: each cut into parts for several CUs, in three launches (bins of the
+// parts added up; the race of the parts, the border's entries listed; the border and the race joined).  For rows with one border or
+// none; a row with both filters open, or with more entries in the border's bin than the list holds, stays for sample_row_kernel.
+struct SplitPart { double best, total; uint64_t at; float x; int pad; };
+struct SplitRow {  // one per row, in the workspace
+  uint64_t mass[BINS], list[POOL];
+  uint64_t need;   // of the border's bin
+  uint32_t n, pad;
+  SplitPart part[16];
+};
+__device__ __forceinline__ bool split_row(const SampleArgs& args, int64_t t, int V, const int64_t* pred, RowFilter& f, bool& by_k, bool& by_p) {
+  if (pred[t] > -2) return false;
+  f = args.row(t);
+  by_k = f.top_k > 0 && f.top_k < V;
+  by_p = f.top_p < 1.f;
+  return !(by_k && by_p);
+}
+struct PartOf { int i0, n; };
+__device__ __forceinline__ PartOf part_of(int V, int part, int parts) {
+  const int per = (V + parts - 1) / parts, i0 = min(part * per, V);
+  return {i0, min(per, V - i0)};
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_bins_kernel(const T* __restrict__ logits, int64_t ld, int V, SampleArgs args,
+                                                         const int64_t* __restrict__ pred, const float* __restrict__ conf,
+                                                         SplitRow* __restrict__ split) {
+  __shared__ uint64_t mass[BINS];
+  const int64_t t = blockIdx.x;
+  RowFilter f;
+  bool by_k, by_p;
+  if (!split_row(args, t, V, pred, f, by_k, by_p) || !(by_k || by_p)) return;
+  const float m = conf[t];
+  const Weight weight = {m, LOG2E / (double)f.temperature};
+  const Bins bins = row_bins(f, m);
+  const PartOf at = part_of(V, blockIdx.y, gridDim.y);
+  for (int i = threadIdx.x; i < BINS; i += NT) mass[i] = 0;
+  __syncthreads();
+  each<T, NT>(logits + t * ld + at.i0, at.n, [&](int, float x) {
+    x = fmaxf(x, -INFINITY);
+    atomicAdd((unsigned long long*)&mass[bins.of(x)], by_p ? (unsigned long long)fixed(weight(x)) : 1ull);
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += NT)
+    if (mass[i]) atomicAdd((unsigned long long*)&split[t].mass[i], (unsigned long long)mass[i]);
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(NT, 2) void sample_part_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
+                                                         int64_t ld_noise, int V, SampleArgs args, const int64_t* __restrict__ pred,
+                                                         const float* __restrict__ conf, SplitRow* __restrict__ split) {
+  __shared__ RowLds<NT> l;
+  const int64_t t = blockIdx.x;
+  RowFilter f;
+  bool by_k, by_p;
+  if (!split_row(args, t, V, pred, f, by_k, by_p)) return;
+  const float m = conf[t];
+  const Weight weight = {m, LOG2E / (double)f.temperature};
+  const Bins bins = row_bins(f, m);
+  SplitRow& w = split[t];
+  Border at = {BINS, 0, 0, INFINITY, -INFINITY, 0, 0, 0};
+  if (by_k || by_p) {
+    for (int i = threadIdx.x; i < BINS; i += NT) l.mass[i] = w.mass[i];
+    __syncthreads();
+    auto get = [&](int i) { return l.mass[i]; };
+    uint64_t need = f.top_k;
+    if (by_p) {
+      const double all = (double)find_cut<NT>(BINS, ~0ull, l, get).before;
+      need = (uint64_t)fmin(fmax(ceil((double)f.top_p * all), 1.0), all);
+    }
+    const CutAt c = find_cut<NT>(BINS, need, l, get);
+    at.bin = min(c.i, BINS - 1);
+    at.lo = lowest_of(bins, at.bin);
+    const float next = lowest_of(bins, at.bin - 1);
+    at.hi = at.bin > 0 ? key_value(value_key(next) - 1) : INFINITY;
+    if (blockIdx.y == 0 && threadIdx.x == 0) w.need = c.i < BINS ? need - c.before : ~0ull;
+    __syncthreads();
+  }
+  const PartOf part = part_of(V, blockIdx.y, gridDim.y);
+  Race race;
+  sweep<T, NT>(logits + t * ld + part.i0, part.n, part.i0, noise + t * ld_noise, 0, at, least_value(f, m), weight, race, l.pack, [&](uint64_t k) {
+    const uint32_t p = atomicAdd(&w.n, 1u);
+    if (p < POOL) w.list[p] = k;
+  });
+  const double total = block_sum<NT>(race.total, l.redd);
+  const double best = block_all<NT>(race.best, l.redd, [](double a, double b) { return fmax(a, b); });
+  const uint64_t mine = race.best == best ? race.at : (uint64_t)~0ull;
+  const uint64_t first = block_all<NT>(mine, l.wave, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+  if (first == ~0ull ? threadIdx.x == 0 : mine == first) w.part[blockIdx.y] = {best, total, first, race.x, 0};
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT) void sample_join_kernel(const float* __restrict__ noise, int64_t ld_noise, int V, SampleArgs args, int parts,
+                                                         int64_t* __restrict__ pred, float* __restrict__ conf,
+                                                         const SplitRow* __restrict__ split) {
+  __shared__ RowLds<NT> l;
+  const int64_t t = blockIdx.x;
+  RowFilter f;
+  bool by_k, by_p;
+  if (!split_row(args, t, V, pred, f, by_k, by_p)) return;
+  const SplitRow& w = split[t];
+  const int n = (int)w.n;
+  if (n > POOL) return;
+  const uint32_t arg = (uint32_t)(-2 - pred[t]);
+  const float m = conf[t], least = least_value(f, m);
+  const Weight weight = {m, LOG2E / (double)f.temperature};
+  int kept = 0;
+  if (n) {
+    for (int i = threadIdx.x; i < n; i += NT) l.list[i] = w.list[i];
+    __syncthreads();
+    sort_keys<NT>(l.list, n);
+    const CutAt c = find_cut<NT>(n, w.need, l, [&](int i) { return by_p ? fixed(weight(key_value((uint32_t)(l.list[i] >> 32)))) : (uint64_t)1; });
+    kept = min(c.i + 1, n);
+  }
+  Race race;
+  for (int i = threadIdx.x; i < kept; i += NT) {
+    const float x = key_value((uint32_t)(l.list[i] >> 32));
+    const uint32_t j = ~(uint32_t)l.list[i];
+    if (x >= least) race.add(weight(x), x, noise[t * ld_noise + j], j);
+  }
+  double kept_mass = block_sum<NT>(race.total, l.redd);
+  for (int p = 0; p < parts; ++p) kept_mass += w.part[p].total;
+  if ((int)threadIdx.x < parts) {
+    const SplitPart s = w.part[threadIdx.x];
+    if (s.at != ~0ull && (s.best > race.best || (s.best == race.best && s.at < race.at))) {
+      race.best = s.best;
+      race.at = s.at;
+      race.x = s.x;
+    }
+  }
+  __syncthreads();  // (pred and conf are read by all before one writes)
   finish<NT>(race, kept_mass, arg, weight, l, pred + t, conf + t);
 }
 
@@ -1960,13 +2105,23 @@ int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, 
 
 // The entries the segments look for: k itself where it is one number up to 512, else 128, the end of most nucleus and min-p
 // sets.  No segments where they could not end the kept set: no filter at all, or a larger k that only top_p or nothing can undercut.
+bool few_long_rows(int T, int V) { return T <= 256 && V >= 16384; }  // (more rows fill the chip whole)
 int sample_k(int top_k) { return top_k > 0 && top_k <= MAX_SEG_K ? (top_k < 16 ? 16 : top_k) : 128; }
 Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
   const bool rows = a.temps || a.ks || a.ps || a.mins;
   const bool by_k = a.top_k > 0 && a.top_k <= MAX_SEG_K && a.top_k < V, large_k = a.top_k > MAX_SEG_K && a.top_k < V;
   const bool ends = by_k || (!large_k && a.top_p < 1.f) || a.min_p > 0.f || a.temperature == 0.f;
-  if (!rows && !ends) return {0, 0, 0, 0, false, 1};
+  // (few rows are cut into parts behind the lists, whatever the filters)
+  if (!rows && !ends && !few_long_rows(T, V)) return {0, 0, 0, 0, false, 1};
   return cut_rows(dtype, T, V, sample_k(a.ks ? 0 : a.top_k));
+}
+// Parts of a row that the lists do not settle, 0: whole rows only.
+int split_parts(int dtype, int T, int V, const SampleArgs& a) {
+  const bool settled = !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K, both = !a.ks && a.top_k > MAX_SEG_K && a.top_k < V && !a.ps && a.top_p < 1.f;
+  if (settled || both || !few_long_rows(T, V) || sample_cut(dtype, T, V, a).nt == 0) return 0;
+  int parts = 1024 / T;
+  if (parts > V / 8192) parts = V / 8192;
+  return parts > 16 ? 16 : parts < 2 ? 2 : parts;
 }
 
 template <typename T>
@@ -1988,8 +2143,16 @@ int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int 
         hipLaunchKernelGGL((sample_segment_kernel<T, NT, decltype(vpt)::value, decltype(many)::value>), grid, dim3(NT), 0, s, x, ld, V, a, K,
                            cut.cap, cut.count, heads, lists);
       });
+    const int parts = split_parts(sizeof(T) == 4 ? PG_F32 : PG_BF16, n, V, a);
+    SplitRow* split = parts ? (SplitRow*)(lists + (int64_t)n * cut.nseg * cut.cap) : nullptr;
     if (cut.nt)
-      hipLaunchKernelGGL((sample_list_kernel<T, 256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf);
+      hipLaunchKernelGGL((sample_list_kernel<T, 256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, cut.nseg, cut.cap, heads, lists, pred, conf,
+                         (uint64_t*)split, (int64_t)(sizeof(SplitRow) / 8));
+    if (parts) {
+      hipLaunchKernelGGL((sample_bins_kernel<T, 512>), dim3(n, parts), dim3(512), 0, s, x, ld, V, a, pred, conf, split);
+      hipLaunchKernelGGL((sample_part_kernel<T, 512>), dim3(n, parts), dim3(512), 0, s, x, ld, q, ldq, V, a, pred, conf, split);
+      hipLaunchKernelGGL((sample_join_kernel<256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, parts, pred, conf, split);
+    }
     const bool settled = cut.nt && !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K;  // the lists hold the first k
     if (!settled)
       hipLaunchKernelGGL((sample_row_kernel<T, 512>), dim3(n), dim3(512), 0, s, x, ld, q, ldq, V, a, cut.nt == 0, pred, conf);
@@ -2089,7 +2252,7 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
 
 extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, int top_k) {
   const Cut cut = cut_rows(dtype, T, V, sample_k(top_k));
-  return (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8);
+  return (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8) + (few_long_rows(T, V) ? (int64_t)T * sizeof(SplitRow) : 0);
 }
 
 extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* noise, int64_t ld_noise, int T, int V,
