@@ -125,7 +125,7 @@ template <int NT> __device__ __forceinline__ ExpSum block_exp_sum(ExpSum a, floa
   return {m, s};
 }
 
-// 2^t in 64 bits for t <= 0: 2^t = 2^n 2^f, |f| <= 1/2, the Taylor series of 2^f to degree 9 (remainder below 8e-12).
+// 2^t in 64 bits, 2^-1022 for every t below: 2^t = 2^n 2^f, |f| <= 1/2, the Taylor series of 2^f to degree 9 (remainder below 8e-12).
 __device__ __forceinline__ double exp2_f64(double t) {
   t = fmax(t, -1022.0);
   const double n = rint(t), f = t - n;
@@ -140,6 +140,13 @@ __device__ __forceinline__ double exp2_f64(double t) {
   p = fma(p, f, 6.93147180559945286227e-1);
   p = fma(p, f, 1.0);
   return ldexp(p, (int)n);
+}
+
+// log s in 64 bits for s > 0: the fp32 logarithm y and what is left, s e^-y - 1 (below 2^-20: its own logarithm to 2^-40).
+__device__ __forceinline__ double log_f64(double s) {
+  const double y = (double)logf((float)s);
+  const double e = s * exp2_f64(-y * LOG2E) - 1.0;
+  return s > 0.0 && s < (double)INFINITY ? y + e : y;  // (0, infinite, NaN: as logf)
 }
 
 // ------------------------------------------------------------------ the largest entries of a segment of a row, kept in registers
@@ -1532,7 +1539,7 @@ template <typename T> __device__ __forceinline__ ListEntry list_entry(const T* r
 }
 struct DistillLds {
   float2 sums[16 * 3];
-  float red[16];
+  double redd[16];
   int repeated;
 };
 
@@ -1541,7 +1548,7 @@ struct DistillLds {
 template <typename T, int NT>
 __device__ __forceinline__ void distill_row(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
                                             ListEntry mine, ExpSum own, bool repeated, DistillLds& l, float (&st)[STASH], float* loss) {
-  const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
+  const float c = (float)(LOG2E / (double)a.tau);
   const bool tail = a.rest != nullptr;
   const float rest = tail ? a.rest[t] : -INFINITY;  // in units of x / tau
   ExpSum sums[3] = {own, {-FLT_MAX, 0.f}, {-FLT_MAX, 0.f}};  // outside, inside the list; the teacher's
@@ -1558,36 +1565,38 @@ __device__ __forceinline__ void distill_row(const T* row, int V, const T* values
   });
   block_exp_sums<NT, 3>(sums, c, l.sums);
   const ExpSum o = sums[0], all = tail ? exp_sum_join(o, sums[1], c) : o;
-  ExpSum te = sums[2];
-  const bool entries = te.s > 0.f, has_rest = rest > -INFINITY;
-  float tr = 0.f, log_tr = 0.f;
-  if (has_rest) {
-    const ExpSum r = {rest * a.tau, 1.f};
-    te = entries ? exp_sum_join(te, r, c) : r;
-    tr = __builtin_amdgcn_exp2f((r.m - te.m) * c) / te.s;
-    log_tr = (r.m - te.m) * inv_tau - logf(te.s);
-  }
+  const bool entries = sums[2].s > 0.f, has_rest = rest > -INFINITY;
+  const float tm = has_rest ? fmaxf(sums[2].m, rest * a.tau) : sums[2].m;  // the reference of the teacher's weights
   const bool live = entries && all.s != 0.f;  // (NaN lives)
-  float part = 0.f;
-  const float shift = logf(all.s) - logf(te.s);
+  // The loss is a small difference of large terms where student and teacher agree (it falls with tau^2 before it is scaled by it):
+  // the teacher's weights, the terms and their sums in 64 bits; the row's sum is fp32 as it comes.
+  const double per = 1.0 / (double)a.tau, scale = per * LOG2E;
+  double weight = 0.0, part = 0.0;
   if (live)
     entries_of([&](ListEntry n, int) {
-      const float p = __builtin_amdgcn_exp2f((n.v - te.m) * c) / te.s;
-      if (p > 0.f) part += p * (((n.v - te.m) - (n.x - all.m)) * inv_tau + shift);
+      const double v = (double)n.v - (double)tm, p = exp2_f64(v * scale);
+      weight += p;
+      if (p > 1e-300) part += p * (v - ((double)n.x - (double)all.m)) * per;
     });
-  part = block_all<NT>(part, l.red, [](float x, float y) { return x + y; });
-  float coef = 0.f;
+  weight = block_sum<NT>(weight, l.redd);
+  part = block_sum<NT>(part, l.redd);
+  float tr = 0.f, coef = 0.f;
   if (live) {
-    if (tr > 0.f) part += tr * (log_tr - ((o.m - all.m) * inv_tau + logf(o.s) - logf(all.s)));
+    const double v = (double)rest - (double)tm * per, p = has_rest ? exp2_f64(v * LOG2E) : 0.0;
+    weight += p;
+    if (p > 1e-300) part += p * (v - ((double)o.m - (double)all.m) * per - log_f64((double)o.s));
+    part = part / weight + (log_f64((double)all.s) - log_f64(weight));
+    tr = (float)(p / weight);
     const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
     coef = o.s != 0.f ? (sr - tr) / o.s : 0.f;
   }
+  const ExpSum te = {tm, (float)weight};
   st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
   st[2] = o.m; st[3] = coef;
   st[4] = te.m; st[5] = live ? 1.f / te.s : 0.f;
   st[6] = live ? 1.f : 0.f;
   st[7] = !tail || repeated ? 1.f : 0.f;  // (without the tail nobody looked)
-  if (threadIdx.x == 0) *loss = live ? w * a.tau * a.tau * part : 0.f;
+  if (threadIdx.x == 0) *loss = live ? (float)((double)w * a.tau * a.tau * part) : 0.f;
 }
 
 // The gradient of one segment: the tokens outside the list in one pass of 16-byte loads and stores, then those in the list.
@@ -1972,6 +1981,12 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
   }
 }
 
+// exp((x - m) / temperature) in 64 bits, 0 for -inf; NaN stays NaN (an infinite x makes one).
+__device__ __forceinline__ double weight_f64(float x, float m, double scale) {
+  const float d = x - m;
+  return d != d ? (double)NAN : x == -INFINITY ? 0.0 : exp2_f64(((double)x - (double)m) * scale);
+}
+
 // Distillation, V and K <= G: the row, its entries and every sum in one group's registers; an entry's teacher probability reaches
 // its token's lane through LDS, added up over the list in order (an id that occurs twice adds twice).
 // LOSS: forward (loss, stash); GRAD: the gradient, from this pass's own numbers (LOSS) or from the stash.
@@ -1985,7 +2000,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
   __shared__ __align__(16) float list_p[256];
   const int v = threadIdx.x & (G - 1), first = threadIdx.x & ~(G - 1);
   const int64_t t0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, t = t0 < rows ? t0 : rows - 1;
-  const float c = (float)(LOG2E / (double)a.tau), inv_tau = 1.f / a.tau;
+  const float c = (float)(LOG2E / (double)a.tau);
   const float w = a.weights ? a.weights[t] : 1.f;
   const bool on = w != 0.f;  // (a row of weight 0 is not read)
   const float x = on && v < V ? to_f32<T>(logits[t * ld + v]) : -INFINITY;
@@ -2009,32 +2024,34 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     const bool out = v < V && !(tail && member);
     o_m = Group<G>::max(out ? x : -INFINITY);
     o_m = o_m == -INFINITY ? 0.f : o_m;
-    const float o_s = Group<G>::sum(out ? __builtin_amdgcn_exp2f((x - o_m) * c) : 0.f);
-    const float in_s = Group<G>::sum(tail && member && v < V ? __builtin_amdgcn_exp2f((x - all_m) * c) : 0.f);
-    const float o_all = o_s * __builtin_amdgcn_exp2f((o_m - all_m) * c);
-    all_s = (o_s == 0.f ? 0.f : o_all) + in_s;
-    float rest = tail ? a.rest[t] : -INFINITY;
+    // In 64 bits, as where the rows are long (distill_row): weights, sums and the terms of the loss.
+    const double per = 1.0 / (double)a.tau, scale = per * LOG2E;
+    const double o_s = Group<G>::sum(out ? weight_f64(x, o_m, scale) : 0.0);
+    const double in_s = Group<G>::sum(tail && member && v < V ? weight_f64(x, all_m, scale) : 0.0);
+    const double o_all = o_s == 0.0 ? 0.0 : o_s * exp2_f64(((double)o_m - (double)all_m) * scale), sum = o_all + in_s;
+    const float rest = tail ? a.rest[t] : -INFINITY;
     const bool has_rest = on && rest > -INFINITY;
     te_m = Group<G>::max(entry ? val : -INFINITY);
     const bool entries = te_m > -INFINITY;
-    const float rest_x = rest * a.tau;
-    if (has_rest) te_m = fmaxf(te_m, rest_x);
+    if (has_rest) te_m = fmaxf(te_m, rest * a.tau);
     if (te_m == -INFINITY) te_m = 0.f;
-    float te_s = Group<G>::sum(entry ? __builtin_amdgcn_exp2f((val - te_m) * c) : 0.f);
-    const float rest_e = has_rest ? __builtin_amdgcn_exp2f((rest_x - te_m) * c) : 0.f;
-    te_s += rest_e;
-    const bool counts = entries && all_s != 0.f;  // (NaN counts)
-    te_inv = 1.f / te_s;
-    const float tr = rest_e * te_inv, log_all = logf(all_s), log_te = logf(te_s);
-    p = entry ? __builtin_amdgcn_exp2f((val - te_m) * c) * te_inv : 0.f;
-    float part = 0.f;
-    if (p > 0.f) part = p * (((val - te_m) - (xs[first + id] - all_m)) * inv_tau + (log_all - log_te));
+    const double rest_v = (double)rest - (double)te_m * per, rest_e = has_rest ? exp2_f64(rest_v * LOG2E) : 0.0;
+    const double mine = entry ? exp2_f64(((double)val - (double)te_m) * scale) : 0.0;
+    const double te_s = Group<G>::sum(mine) + rest_e;
+    const bool counts = entries && sum != 0.0;  // (NaN counts)
+    double part = 0.0;
+    if (mine > 1e-300) part = mine * (((double)val - (double)te_m) - ((double)xs[first + id] - (double)all_m)) * per;
     part = Group<G>::sum(part);
-    if (tr > 0.f) part += tr * (((rest_x - te_m) * inv_tau - log_te) - ((o_m - all_m) * inv_tau + logf(o_s) - log_all));
-    coef = o_s != 0.f ? ((tail ? o_all / all_s : 1.f) - tr) / o_s : 0.f;
+    if (rest_e > 1e-300) part += rest_e * (rest_v - ((double)o_m - (double)all_m) * per - log_f64(o_s));
+    part = part / te_s + (log_f64(sum) - log_f64(te_s));
+    const float tr = (float)(rest_e / te_s);
+    te_inv = (float)(1.0 / te_s);
+    p = (float)(mine / te_s);
+    all_s = (float)sum;
+    coef = o_s != 0.0 ? (float)(((tail ? o_all / sum : 1.0) - tr) / o_s) : 0.f;
     live = counts ? 1.f : 0.f;
     if (v == 0 && t0 < rows) {
-      loss[t] = counts ? w * a.tau * a.tau * part : 0.f;
+      loss[t] = counts ? (float)((double)w * a.tau * a.tau * part) : 0.f;
       if (!GRAD) {
         float* st = stash + t * STASH;
         *reinterpret_cast<float4*>(st) = make_float4(all_m, counts ? 1.f / all_s : 0.f, o_m, counts ? coef : 0.f);
