@@ -324,7 +324,7 @@ int pg_commit_topk(int64_t* ids, const int64_t* pred, const float* conf, int B, 
  * logits: T rows of V <= 2^24 entries (dtype PG_F32 or PG_BF16), row t at logits + t*ld elements; any alignment of the element
  * type.  Entries of a row are ordered by value, ties by the lower index; NaN counts as -inf, -0 as +0.  Workspaces: the
  * *_workspace_bytes functions (may be 0; then NULL will do); a workspace is 16-byte aligned and serves one
- * call at a time.
+ * call at a time.  temperature lies in 1e-30 .. 1e30 (pg_sample_filtered: or is 0; finite ones outside count as the nearer end).
  *
  * pg_top_logits: a teacher's record of each row, for pg_distill_*: the first k <= min(V, 1024) entries (values [T][k] in the
  * activation type, ids [T][k], in order) and rest[t] = log sum over the other entries of exp(x / temperature) (-inf if there is

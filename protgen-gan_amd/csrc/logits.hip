@@ -13,6 +13,7 @@ namespace {
 
 constexpr int MAX_K = 1024;
 constexpr int MAX_VOCAB = 1 << 24;  // 2^24 weights of at most 2^40 each fit the 64-bit fixed-point sums
+constexpr float MIN_TAU = 1e-30f, MAX_TAU = 1e30f;
 constexpr double LOG2E = 1.4426950408889634074;
 constexpr double LN2 = 0.69314718055994530942;
 
@@ -190,11 +191,12 @@ template <int E, bool KEEP_NAN = false> __device__ __forceinline__ void exp_sum_
 }
 // The same sum for entries of one set with a fixed reference m, an entry of the set: one multiply-add, one exponential and one
 // addition per entry.  m c is rounded once (mc) and the sum corrected by the difference at the end.  Entries far above m overflow
-// it: then ok() is false and the caller takes the way above, as where there is no usable m.
+// it, and past 2^29 the rounding of m c (half an ulp: above 16) could do so in either direction: then ok() is false and the caller
+// takes the way above, as where there is no usable m.
 struct FixedSum {
   float m, mc, s, c;
   __device__ __forceinline__ FixedSum(float reference, float scale) : m(reference), mc(reference * scale), s(0.f), c(scale) {}
-  __device__ __forceinline__ bool ok() const { return fabsf(mc) < 1e30f && s < INFINITY; }  // (false for NaN)
+  __device__ __forceinline__ bool ok() const { return fabsf(mc) < 0x1p29f && s < INFINITY; }  // (false for NaN)
   template <int E> __device__ __forceinline__ void add(const float (&o)[E]) {
     float t[2] = {0.f, 0.f};
 #pragma unroll
@@ -714,8 +716,10 @@ struct SampleArgs {
   float temperature, top_p, min_p;
   int top_k, empty;  // empty: the token of a row with nothing above -inf
   const float* temps; const int32_t* ks; const float* ps; const float* mins;
+  // (positive temperatures within MIN_TAU .. MAX_TAU, where no scale or product of a scale leaves fp32's range)
   __device__ __forceinline__ RowFilter row(int64_t t) const {
-    return {temps ? temps[t] : temperature, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
+    const float given = temps ? temps[t] : temperature;
+    return {given > 0.f ? fminf(fmaxf(given, MIN_TAU), MAX_TAU) : 0.f, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
   }
 };
 // ------------------------------------------------------------------ one row by a whole workgroup, any boundary
@@ -1339,7 +1343,7 @@ __global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restri
   __shared__ SegLds<NT, MANY> l;
   const int64_t t = blockIdx.x;
   const int seg = blockIdx.y, nseg = gridDim.y;
-  const float temp = args.temps ? args.temps[t] : args.temperature;
+  const float temp = args.row(t).temperature;
   const float c = temp > 0.f ? (float)(LOG2E / (double)temp) : 0.f;
   const T* row = logits + t * ld;
   uint64_t level;
@@ -2011,7 +2015,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     val = to_f32<T>(((const T*)a.values)[t * a.K + v]);
   }
   const bool entry = (uint32_t)id < (uint32_t)V && val > -INFINITY;
-  float all_m, all_s, o_m, coef, te_m, te_inv, p, live;
+  float all_m, all_s, o_m, coef, te_m, te_inv, live;
   xs[threadIdx.x] = x;
   list_id[threadIdx.x] = entry ? id : -1;
   if (LOSS) {
@@ -2046,7 +2050,6 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     part = part / te_s + (log_f64(sum) - log_f64(te_s));
     const float tr = (float)(rest_e / te_s);
     te_inv = (float)(1.0 / te_s);
-    p = (float)(mine / te_s);
     all_s = (float)sum;
     coef = o_s != 0.0 ? (float)(((tail ? o_all / sum : 1.0) - tr) / o_s) : 0.f;
     live = counts ? 1.f : 0.f;
@@ -2062,10 +2065,9 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
   } else {
     const float4 s0 = *reinterpret_cast<const float4*>(stash + t * STASH), s1 = *reinterpret_cast<const float4*>(stash + t * STASH + 4);
     all_m = s0.x; all_s = s0.y; o_m = s0.z; coef = s0.w; te_m = s1.x; te_inv = s1.y; live = s1.z;
-    p = entry ? __builtin_amdgcn_exp2f((val - te_m) * c) * te_inv : 0.f;
   }
   if (!GRAD) return;
-  list_p[threadIdx.x] = p;
+  list_p[threadIdx.x] = entry ? __builtin_amdgcn_exp2f((val - te_m) * c) * te_inv : 0.f;  // (one expression, so one result, for both ways)
   __syncthreads();
   bool member = false;
   float tv = 0.f;
@@ -2091,7 +2093,7 @@ int check_distill(int dtype, const void* logits, int64_t ld, int T, int V, const
                   float tau) {
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
-  if (!values || !ids || k <= 0 || !(tau > 0.f) || !(tau <= FLT_MAX)) return PG_ERR_ARG;
+  if (!values || !ids || k <= 0 || !(tau >= MIN_TAU && tau <= MAX_TAU)) return PG_ERR_ARG;
   return k > MAX_K ? PG_ERR_UNSUPPORTED : PG_OK;
 }
 
@@ -2258,7 +2260,7 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
                              int32_t* ids, float* rest, void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
-  if (!values || !ids || !rest || k <= 0 || k > V || !(temperature > 0.f) || !(temperature <= FLT_MAX)) return PG_ERR_ARG;
+  if (!values || !ids || !rest || k <= 0 || k > V || !(temperature >= MIN_TAU && temperature <= MAX_TAU)) return PG_ERR_ARG;
   if (k > MAX_K) return PG_ERR_UNSUPPORTED;
   const int64_t need = pg_top_logits_workspace_bytes(dtype, T, V, k);
   if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;

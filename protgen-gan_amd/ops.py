@@ -276,8 +276,8 @@ def _same(like, name, t, dtype, shape):
 
 def _positive(temperature):
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be positive and finite (1e-30 to 1e30), got {temperature}")
     return temperature
 
 
@@ -309,7 +309,7 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     entries (0: all), of those to the smallest leading set that holds `top_p` of their mass, and to the entries of at least
     `min_p` times the largest probability.  `noise` fp32 [T, V] ~ Exp(1): the token is the argmax of p / noise, as in
     sample_tokens; only the kept entries' noise is read.  Every setting is a number or a tensor [T] on the device (fp32; top_k:
-    int32), read per row without a check.  temperature 0: the largest entry.  Returns (pred int64 [T], conf fp32 [T]), conf the
+    int32), read per row without a check.  temperature 0: the largest entry; 1e-30 is the least above it.  Returns (pred int64 [T], conf fp32 [T]), conf the
     token's probability among the kept entries; a row with nothing above -inf gives (`empty`, 0)."""
     if logits.dim() != 2:
         raise ValueError(f"logits: expected [T, V], got {tuple(logits.shape)}")

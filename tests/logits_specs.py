@@ -95,6 +95,8 @@ def distill(x, values, ids, rest, tau, w):
         lse = log_sum(z)
         s = np.exp(z - lse)
         r = -np.inf if rest is None else float(rest[t])
+        most = max(v.max(), r if r < np.inf else -np.inf)  # (as z: at temperature 2^-40 an entry of 11 is 1.2e13, spaced by 2^-9)
+        v, r = v - most, r - most
         lt = log_sum(np.append(v, r))
         te, tr = np.exp(v - lt), math.exp(r - lt) if r > -np.inf else 0.0
         out = np.ones(V, bool)

@@ -177,6 +177,22 @@ def test_sample_filtered_per_row_settings(pg, dtype, V):
     check_sample(pg, x, top_p=p)
 
 
+@pytest.mark.parametrize("V", [30, 900, 33000])
+def test_extreme_temperatures(pg, V):
+    """Near 0 only the ties of the largest entry race; far up, and infinite in a row's own setting, all entries weigh the same."""
+    temp = torch.tensor([1e-45, 1e-40, 1e-30, 1e-20, 1e20, 1e30, 3e38, float("inf")], device=DEV)
+    x = rows(8, V, torch.bfloat16, 12)
+    x[:, V // 3] = x[:, V // 2] = 50.0
+    x[:, V // 4] = float("-inf")
+    for f in ({}, {"top_p": 0.6}, {"top_k": 7}, {"min_p": 0.3}, {"top_k": 600, "top_p": 0.9}):
+        check_sample(pg, x, temperature=temp, **f)
+        for t in (1e-40, 3e38):
+            check_sample(pg, x, temperature=t, **f)
+    for tau in (2.0 ** -99, 2.0 ** 99):  # (numbers of fp32)
+        check_top(pg, x, 1, tau)
+        check_top(pg, x, 20, tau)
+
+
 def test_sample_filtered_strided_inputs_and_outputs(pg):
     x = rows(8, 333, torch.bfloat16, 2, pad=7, shift=5)
     q = torch.empty(8, 400, device=DEV).exponential_(1.0)[:, 3:336]
@@ -312,6 +328,15 @@ def test_distill_gradient_against_differences(pg, V):
         diff = ((f(h) - f(-h)) / (2 * h)).cpu().numpy()
         along = (grad.double() * d.double()).sum(1).cpu().numpy()
         assert (np.abs(diff - along) <= 5e-5 * tau + (ADDS(V) + 64) * U * ls / h).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [30, 900, 33000])
+@pytest.mark.parametrize("tau", [2.0 ** -40, 2.0 ** -10, 2.0 ** 10])
+def test_distill_extreme_temperatures(pg, dtype, V, tau):
+    x, v, i, r = record(pg, 5, V, 9, dtype, V, tau, True)
+    check_distill(pg, x, v, i, r, tau, None)
+    check_distill(pg, x, v, i, None, tau, None)
 
 
 def test_distill_strides_and_leading_dims(pg):

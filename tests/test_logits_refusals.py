@@ -20,6 +20,8 @@ X = torch.zeros(4, 10)
     (lambda o: o.top_logits(X, 3, temperature=0.0), ValueError),
     (lambda o: o.top_logits(X, 3, temperature=float("nan")), ValueError),
     (lambda o: o.top_logits(X, 3, temperature=float("inf")), ValueError),
+    (lambda o: o.top_logits(X, 3, temperature=1e-31), ValueError),
+    (lambda o: o.top_logits(X, 3, temperature=1e31), ValueError),
     (lambda o: o.top_logits(X.half(), 3), TypeError),
     (lambda o: o.top_logits(X.double(), 3), TypeError),
     (lambda o: o.top_logits(torch.zeros(()), 1), ValueError),
@@ -57,6 +59,7 @@ def test_sample_filtered_refusals(pg, kw, error):
     ({"rest": torch.zeros(3)}, ValueError), ({"rest": torch.zeros(4, dtype=torch.float64)}, TypeError),
     ({"weights": torch.zeros(4, 1)}, ValueError), ({"weights": torch.zeros(4, dtype=torch.int64)}, TypeError),
     ({"temperature": 0.0}, ValueError), ({"temperature": -1.0}, ValueError), ({"logits": X.half()}, TypeError), ({}, ValueError),
+    ({"temperature": 1e-31}, ValueError), ({"temperature": 1e31}, ValueError),
 ])
 def test_distill_refusals(pg, kw, error):
     args = {"logits": X, "values": torch.zeros(4, 3), "ids": torch.zeros(4, 3, dtype=torch.int32), "rest": None, "weights": None}
