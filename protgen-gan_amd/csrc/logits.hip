@@ -2004,7 +2004,8 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
   __shared__ __align__(16) float list_p[256];
   const int v = threadIdx.x & (G - 1), first = threadIdx.x & ~(G - 1);
   const int64_t t0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, t = t0 < rows ? t0 : rows - 1;
-  const float c = (float)(LOG2E / (double)a.tau);
+  const double per = 1.0 / (double)a.tau, scale = per * LOG2E;
+  const float c = (float)scale;
   const float w = a.weights ? a.weights[t] : 1.f;
   const bool on = w != 0.f;  // (a row of weight 0 is not read)
   const float x = on && v < V ? to_f32<T>(logits[t * ld + v]) : -INFINITY;
@@ -2029,9 +2030,8 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     o_m = Group<G>::max(out ? x : -INFINITY);
     o_m = o_m == -INFINITY ? 0.f : o_m;
     // In 64 bits, as where the rows are long (distill_row): weights, sums and the terms of the loss.
-    const double per = 1.0 / (double)a.tau, scale = per * LOG2E;
-    const double o_s = Group<G>::sum(out ? weight_f64(x, o_m, scale) : 0.0);
-    const double in_s = Group<G>::sum(tail && member && v < V ? weight_f64(x, all_m, scale) : 0.0);
+    const double mass = v < V ? weight_f64(x, out ? o_m : all_m, scale) : 0.0;
+    const double o_s = Group<G>::sum(out ? mass : 0.0), in_s = Group<G>::sum(out ? 0.0 : mass);
     const double o_all = o_s == 0.0 ? 0.0 : o_s * exp2_f64(((double)o_m - (double)all_m) * scale), sum = o_all + in_s;
     const float rest = tail ? a.rest[t] : -INFINITY;
     const bool has_rest = on && rest > -INFINITY;
@@ -2048,20 +2048,18 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     part = Group<G>::sum(part);
     if (rest_e > 1e-300) part += rest_e * (rest_v - ((double)o_m - (double)all_m) * per - log_f64(o_s));
     part = part / te_s + (log_f64(sum) - log_f64(te_s));
-    const float tr = (float)(rest_e / te_s);
-    te_inv = (float)(1.0 / te_s);
-    all_s = (float)sum;
-    coef = o_s != 0.0 ? (float)(((tail ? o_all / sum : 1.0) - tr) / o_s) : 0.f;
+    te_inv = 1.f / (float)te_s;
+    all_s = 1.f / (float)sum;
+    coef = o_s != 0.0 ? ((tail ? (float)o_all * all_s : 1.f) - (float)rest_e * te_inv) / (float)o_s : 0.f;
     live = counts ? 1.f : 0.f;
     if (v == 0 && t0 < rows) {
       loss[t] = counts ? (float)((double)w * a.tau * a.tau * part) : 0.f;
       if (!GRAD) {
         float* st = stash + t * STASH;
-        *reinterpret_cast<float4*>(st) = make_float4(all_m, counts ? 1.f / all_s : 0.f, o_m, counts ? coef : 0.f);
+        *reinterpret_cast<float4*>(st) = make_float4(all_m, counts ? all_s : 0.f, o_m, counts ? coef : 0.f);
         *reinterpret_cast<float4*>(st + 4) = make_float4(te_m, counts ? te_inv : 0.f, live, 0.f);
       }
     }
-    all_s = 1.f / all_s;
   } else {
     const float4 s0 = *reinterpret_cast<const float4*>(stash + t * STASH), s1 = *reinterpret_cast<const float4*>(stash + t * STASH + 4);
     all_m = s0.x; all_s = s0.y; o_m = s0.z; coef = s0.w; te_m = s1.x; te_inv = s1.y; live = s1.z;
