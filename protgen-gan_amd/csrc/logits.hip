@@ -155,8 +155,8 @@ __device__ __forceinline__ double log_f64(double s) {
 // flight at once) and reads it once.  The K-th largest of the threads' maxima is a lower bound of the segment's K-th largest entry
 // and not far below it (64 of 256 maxima leave about 75 entries above the bound, 128 about 180; above that each thread's vectors
 // form four groups), found by eight rounds of counting on the upper 16 bits of their keys.  Vectors with an entry above the bound go to
-// LDS, all others into the sum of exponentials.  Where too many entries tie at the bound, the exact K-th key is found by
-// bisection over the segment instead.
+// LDS, all others into the sum of exponentials.  Where too many entries tie at the bound, the K-th key's digits are found by
+// counting over the segment instead.
 constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
 constexpr int MAX_SEG_K = 512;
 constexpr int max_cap(int K) { return K > 128 ? 1088 : 512; }  // keys a segment may leave
@@ -190,13 +190,14 @@ template <int E, bool KEEP_NAN = false> __device__ __forceinline__ void exp_sum_
   a.m = m;
 }
 // The same sum for entries of one set with a fixed reference m, an entry of the set: one multiply-add, one exponential and one
-// addition per entry.  m c is rounded once (mc) and the sum corrected by the difference at the end.  Entries far above m overflow
-// it, and past 2^29 the rounding of m c (half an ulp: above 16) could do so in either direction: then ok() is false and the caller
-// takes the way above, as where there is no usable m.
+// addition per entry.  m c is rounded once (mc) and the sum corrected by the difference at the end.  Entries far above m make it
+// large: past 2^90 a join with a sum whose m is 2^126 larger would flush its factor, and lose more than 2^-36 of the whole.  Past
+// 2^29 the rounding of m c (half an ulp: above 16) could do as much.  Then ok() is false and the caller takes the way above, as
+// where there is no usable m.
 struct FixedSum {
   float m, mc, s, c;
   __device__ __forceinline__ FixedSum(float reference, float scale) : m(reference), mc(reference * scale), s(0.f), c(scale) {}
-  __device__ __forceinline__ bool ok() const { return fabsf(mc) < 0x1p29f && s < INFINITY; }  // (false for NaN)
+  __device__ __forceinline__ bool ok() const { return fabsf(mc) < 0x1p29f && s < 0x1p90f; }  // (false for NaN)
   template <int E> __device__ __forceinline__ void add(const float (&o)[E]) {
     float t[2] = {0.f, 0.f};
 #pragma unroll
@@ -249,15 +250,51 @@ __device__ __forceinline__ Key kth_bound(const Key (&k)[R], int used, int K, int
   return bound;
 }
 
+// The first i < n at which get(0) + ... + get(i) reaches need, and the sum before it; i = n, the sum of all, if none does.
+struct CutAt { int i; uint64_t before; };
+template <int NT, typename L, typename F> __device__ __forceinline__ CutAt find_cut(int n, uint64_t need, L& l, F get) {
+  const int per = (n + NT - 1) / NT, a = min((int)threadIdx.x * per, n), b = min(a + per, n);
+  uint64_t sum = 0;
+  for (int i = a; i < b; ++i) sum += get(i);
+  uint64_t upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t v = __shfl_up(upto, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) upto += v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x >> 6] = upto;
+  if (threadIdx.x == 0) l.cut = n;
+  __syncthreads();
+  uint64_t all = 0, off = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < (int)(threadIdx.x >> 6)) off += l.wave[w];
+    all += l.wave[w];
+  }
+  upto += off;
+  uint64_t before = upto - sum;
+  if (before < need && upto >= need) {
+    int i = a;
+    for (uint64_t g; i < b && before + (g = get(i)) < need; ++i) before += g;
+    l.cut = i;
+    l.cut_before = before;
+  }
+  __syncthreads();
+  return l.cut < n ? CutAt{l.cut, l.cut_before} : CutAt{n, all};
+}
+
 template <int NT, bool MANY> struct SegLds {  // MANY: for K above 128
   uint64_t wave[16];
-  static constexpr int STAGE = MANY ? 512 : 256;  // vectors that may hold an entry above the bound
+  static constexpr int STAGE = MANY ? 1024 : 256;  // vectors that may hold an entry above the bound (k 512: about 700)
   static constexpr int LIST = MANY ? 2048 : 512;  // keys (a power of two of at least max_cap)
   __align__(16) uint64_t list[LIST];
   uint4 vec[STAGE];
   int at[STAGE];
   uint32_t n_vec, n;
   uint64_t counts[2][16];
+  uint64_t cut_before;
+  int cut;
   float red[16];
 };
 struct SegHead {      // what a segment leaves for the merge
@@ -432,24 +469,28 @@ __device__ __forceinline__ int collect(const T* row, int V, int seg, int count, 
   }
   int n = l.n;
   level = thr > -INFINITY ? (uint64_t)value_key(thr) << 32 : 0;
-  if (over || n > cap) {  // too many at the bound: the K-th key itself, bit by bit
-    auto number = [&](auto in) {
-      int k = 0;
-      Seg::entries(row, V, seg, count, nseg, [&](float x, int i) { k += in(x, i); });
-      return block_all<NT>(k, reinterpret_cast<int*>(l.red), [](int a, int b) { return a + b; });
-    };
-    uint32_t vk = 0;
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t trial = vk | (1u << b);
-      if (number([&](float x, int) { return value_key(x) >= trial; }) >= K) vk = trial;
+  if (over || n > cap) {  // too many at the bound: the K-th key by its digits, ten bits at a time, until at most cap keys are left
+    uint32_t* bins = reinterpret_cast<uint32_t*>(l.vec);
+    uint64_t prefix = 0;
+    int above = 0;
+    for (int shift = 54, last = 64;; last = shift, shift = shift > 10 ? shift - 10 : 0) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 1024; i += NT) bins[i] = 0;
+      __syncthreads();
+      Seg::entries(row, V, seg, count, nseg, [&](float x, int i) {
+        const uint64_t k = entry_key(x, i);
+        if ((last == 64 || k >> last == prefix) && (!FINITE || x > -INFINITY))
+          atomicAdd(&bins[(int)(k >> shift) & ((1 << (last - shift)) - 1)], 1u);
+      });
+      __syncthreads();
+      const int digits = 1 << (last - shift);
+      const CutAt at = find_cut<NT>(digits, K - above, l, [&](int i) { return (uint64_t)bins[digits - 1 - i]; });
+      const int digit = digits - 1 - min(at.i, digits - 1);
+      above += (int)at.before;
+      prefix = prefix << (last - shift) | digit;
+      level = prefix << shift;
+      if (above + (int)bins[digit] <= cap || shift == 0) break;
     }
-    const int above = number([&](float x, int) { return value_key(x) > vk; });
-    uint32_t low = 0;  // of the entries at the K-th value, the K - above lowest indexes: the largest bound on ~index that keeps them
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t trial = low | (1u << b);
-      if (number([&](float x, int i) { return value_key(x) == vk && (uint32_t)~i >= trial; }) >= K - above) low = trial;
-    }
-    level = ((uint64_t)vk << 32) | low;
     rest = {-FLT_MAX, 0.f};
     __syncthreads();
     if (threadIdx.x == 0) l.n = 0;
@@ -744,40 +785,6 @@ template <int NT> struct RowLds {
   uint32_t n, ends[66];
 };
 
-// The first i < n at which get(0) + ... + get(i) reaches need, and the sum before it; i = n, the sum of all, if none does.
-struct CutAt { int i; uint64_t before; };
-template <int NT, typename L, typename F> __device__ __forceinline__ CutAt find_cut(int n, uint64_t need, L& l, F get) {
-  const int per = (n + NT - 1) / NT, a = min((int)threadIdx.x * per, n), b = min(a + per, n);
-  uint64_t sum = 0;
-  for (int i = a; i < b; ++i) sum += get(i);
-  uint64_t upto = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t v = __shfl_up(upto, o, 64);
-    if ((int)(threadIdx.x & 63) >= o) upto += v;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) l.wave[threadIdx.x >> 6] = upto;
-  if (threadIdx.x == 0) l.cut = n;
-  __syncthreads();
-  uint64_t all = 0, off = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) off += l.wave[w];
-    all += l.wave[w];
-  }
-  upto += off;
-  uint64_t before = upto - sum;
-  if (before < need && upto >= need) {
-    int i = a;
-    for (uint64_t g; i < b && before + (g = get(i)) < need; ++i) before += g;
-    l.cut = i;
-    l.cut_before = before;
-  }
-  __syncthreads();
-  return l.cut < n ? CutAt{l.cut, l.cut_before} : CutAt{n, all};
-}
-
 // Bins of equal width in m - x, m the largest entry: an entry's bin never decreases with m - x, so bins are ranges of the order.
 struct Bins {
   float m, per;
@@ -957,7 +964,7 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict
   const float c = greedy ? 0.f : (float)scale;
   RowKeys<NT> rk;
   rk.load(heads, lists, t, nseg, cap, l.ends);
-  const int want = f.top_k > 0 && f.top_k < POOL / 4 ? f.top_k : 192;  // (what 256 threads sort by counting)
+  const int want = f.top_k > 0 && f.top_k <= MAX_SEG_K ? f.top_k : 192;  // (what 256 threads sort by counting)
   const int n = rk.first(want, POOL, l.list, c, l);
   if (n == 0) {
     if (threadIdx.x == 0) pred[t] = args.empty, conf[t] = 0.f;

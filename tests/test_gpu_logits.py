@@ -92,6 +92,22 @@ def test_top_logits_odd_rows(pg, dtype, V, k):
     check_top(pg, odd_values(V, dtype), k, tau=0.5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(900, 100), (8192, 512), (8192, 300), (40000, 64), (131072, 128), (131072, 512)])
+def test_top_logits_few_values(pg, dtype, V, k):
+    """Rows of a few distinct values, masks of the type's lowest and of -inf among them: the border lies inside long ties."""
+    g = torch.Generator().manual_seed(V + k)
+    x = torch.stack([torch.randint(0, n, (V,), generator=g).float() for n in (1, 2, 40, 300, 2, 2)])
+    x[4] = torch.where(x[4] > 0, torch.finfo(dtype).min, float("-inf"))
+    x[5] = float("-inf")
+    x[4, V // 2: V // 2 + 20] = 3.0
+    x[5, 7:7 + k // 2] = 1.0
+    x = x.to(dtype).to(DEV)
+    check_top(pg, x, k)
+    check_sample(pg, x, top_k=k)
+    check_sample(pg, x, top_p=0.4)
+
+
 def test_top_logits_leading_dims_and_empty(pg):
     x = rows(6, 40, torch.float32, 1).contiguous().view(2, 3, 40)
     v, i, r = pg.ops.top_logits(x, 5)
@@ -328,6 +344,28 @@ def test_distill_gradient_against_differences(pg, V):
         diff = ((f(h) - f(-h)) / (2 * h)).cpu().numpy()
         along = (grad.double() * d.double()).sum(1).cpu().numpy()
         assert (np.abs(diff - along) <= 5e-5 * tau + (ADDS(V) + 64) * U * ls / h).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V", [(5, 900), (5, 8192), (5, 33000), (1030, 9000), (1030, 33000), (1025, 140001)])
+def test_steep_rows(pg, dtype, T, V):
+    """Entries spread over hundreds of units of temperature: a thread's sum may start at the least of them."""
+    x = (40 * torch.randn(T, V, device=DEV, generator=torch.Generator(DEV).manual_seed(V))).to(dtype)
+    few = slice(0, T, max(1, T // 5))
+    v, i, r = pg.ops.top_logits(x, 40, temperature=0.5)
+    for a, b in zip((v[few], i[few], r[few]), pg.ops.top_logits(x[few].contiguous(), 40, temperature=0.5)):
+        assert a.dtype == torch.float32 and torch.allclose(a, b, rtol=2 * U, atol=ADDS(V) * U) or torch.equal(a, b)
+    check_top(pg, x[few], 40, 0.5)
+    check_sample(pg, x[few], top_p=0.9, temperature=3.0)
+    student = (x.float() * 0.9).to(dtype)
+    both = pg.ops.distill_loss_grad(student, v, i, rest=r, temperature=0.5)
+    loss, stash = pg.ops.distill_fwd(student, v, i, rest=r, temperature=0.5)
+    for t in range(0, T, max(1, T // 5)):
+        want, grad, ls, gs = spec.distill(student[t:t + 1], v[t:t + 1], i[t:t + 1], r[t:t + 1], 0.5, None)
+        a = (ADDS(V) + 64) * U
+        assert abs(float(both[0][t]) - want[0]) <= a * ls[0] and abs(float(loss[t]) - want[0]) <= a * ls[0]
+        err = np.abs(both[1][t].double().cpu().numpy() - grad[0])
+        assert (err <= a * gs[0] + torch.finfo(dtype).eps / 2 * np.abs(grad[0]) * 1.01 + 1e-38).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
