@@ -336,8 +336,8 @@ int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k
  * w_v = exp((x_v - max) / temperature), the row keeps its first min(k, n_p, n_m) entries: n_p = those before which less than
  * top_p of the first k entries' mass lies, n_m = those with w >= min_p.  pred = argmax w_v / noise_v over them (ties: lowest
  * index; noise ~ Exp(1), row t at noise + t*ld_noise), conf = w_pred / their mass.  top_k 0, top_p 1, min_p 0 switch a filter
- * off; temperature 0 takes the first entry (conf 1).  A row without an entry above -inf: pred = empty (>= -1),
- * conf 0.  temps / ks / ps / mins
+ * off; temperature 0 takes the first entry (conf 1).  For top_p an entry's mass counts in multiples of 2^-40 of the largest's, so
+ * that sums are the same in any order.  A row without an entry above -inf: pred = empty (>= -1), conf 0.  temps / ks / ps / mins
  * (nullable): settings per row; there out-of-range values mean: temperature <= 0 or NaN 0, k <= 0 off, top_p >= 1 or NaN off,
  * top_p <= 0 the first entry, min_p <= 0 or NaN off, min_p > 1 as 1. */
 int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, int top_k /* 0: none, or per row */);

@@ -1162,7 +1162,7 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
     float most = -INFINITY;
     int first = -1;
     each<T, NT>(row, V, [&](int i, float x) {
-      if (x > most || (first < 0 && x == most)) most = x, first = i;
+      if (x > most || (x == most && (uint32_t)i < (uint32_t)first)) most = x, first = i;  // (the row's odd ends come last)
     });
     uint64_t top = first < 0 ? entry_key(-INFINITY, ~0u) : entry_key(most, first);
     top = block_all<NT>(top, l.wave, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
@@ -1554,60 +1554,90 @@ struct DistillLds {
   int repeated;
 };
 
-// The row's loss and stash from each thread's sum over the tokens outside the list (tail) or over all of them.  Every thread of the
-// workgroup returns with the stash's numbers in st.
+// The entries of the teacher's list, this thread's: f(entry, its place).
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void own_entries(const T* row, int V, const T* values, const int32_t* ids, int K, ListEntry mine, F f) {
+  if (mine.id >= 0) f(mine, (int)threadIdx.x);
+  for (int e = threadIdx.x + NT; e < K; e += NT) {
+    const ListEntry n = list_entry(row, V, values, ids, e, K);
+    if (n.id >= 0) f(n, e);
+  }
+}
+// The teacher's weights are taken relative to the largest of the list's entries and the rest, in 64 bits: the rest is in units of
+// x / tau, and in fp32 its conversion would move it by whole probabilities where logits are far from 0.
+struct Teacher {
+  double per, scale, rest_x, m;  // 1 / tau, log2(e) / tau, rest tau, the reference
+  bool has_rest;
+  __device__ __forceinline__ Teacher(float list_max, const DistillArgs& a, int64_t t) {
+    const float rest = a.rest ? a.rest[t] : -INFINITY;
+    per = 1.0 / (double)a.tau;
+    scale = per * LOG2E;
+    rest_x = (double)rest * (double)a.tau;
+    has_rest = rest > -INFINITY;
+    m = has_rest ? fmax((double)list_max, rest_x) : (double)list_max;
+  }
+};
+struct RowSums {
+  ExpSum out, all, list;  // student: outside the list, all tokens; teacher: the list's entries
+  bool live;
+};
+
+// The row's sums and stash from each thread's sum over the tokens outside the list (tail) or over all of them.  Every thread of the
+// workgroup returns with them.
 template <typename T, int NT>
-__device__ __forceinline__ void distill_row(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
-                                            ListEntry mine, ExpSum own, bool repeated, DistillLds& l, float (&st)[STASH], float* loss) {
+__device__ __forceinline__ RowSums distill_sums(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t,
+                                                ListEntry mine, ExpSum own, bool repeated, DistillLds& l, float (&st)[STASH]) {
   const float c = (float)(LOG2E / (double)a.tau);
   const bool tail = a.rest != nullptr;
-  const float rest = tail ? a.rest[t] : -INFINITY;  // in units of x / tau
   ExpSum sums[3] = {own, {-FLT_MAX, 0.f}, {-FLT_MAX, 0.f}};  // outside, inside the list; the teacher's
-  auto entries_of = [&](auto f) {
-    if (mine.id >= 0) f(mine, (int)threadIdx.x);
-    for (int e = threadIdx.x + NT; e < a.K; e += NT) {
-      const ListEntry n = list_entry(row, V, values, ids, e, a.K);
-      if (n.id >= 0) f(n, e);
-    }
-  };
-  entries_of([&](ListEntry n, int e) {
+  own_entries<T, NT>(row, V, values, ids, a.K, mine, [&](ListEntry n, int e) {
     exp_sum_add(sums[2], n.v, c);
     if (tail && (!repeated || first_of_id(values, ids, e, V))) exp_sum_add(sums[1], n.x, c);
   });
   block_exp_sums<NT, 3>(sums, c, l.sums);
   const ExpSum o = sums[0], all = tail ? exp_sum_join(o, sums[1], c) : o;
-  const bool entries = sums[2].s > 0.f, has_rest = rest > -INFINITY;
-  const float tm = has_rest ? fmaxf(sums[2].m, rest * a.tau) : sums[2].m;  // the reference of the teacher's weights
-  const bool live = entries && all.s != 0.f;  // (NaN lives)
-  // The loss is a small difference of large terms where student and teacher agree (it falls with tau^2 before it is scaled by it):
-  // the teacher's weights, the terms and their sums in 64 bits; the row's sum is fp32 as it comes.
-  const double per = 1.0 / (double)a.tau, scale = per * LOG2E;
+  const bool live = sums[2].s > 0.f && all.s != 0.f;  // (NaN lives)
+  const Teacher te(sums[2].m, a, t);
+  const float share = __builtin_amdgcn_exp2f((float)(((double)sums[2].m - te.m) * te.scale));
+  const float rest = te.has_rest ? __builtin_amdgcn_exp2f((float)((te.rest_x - te.m) * te.scale)) : 0.f;
+  const float weight = sums[2].s * share + rest;
+  const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
+  st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
+  st[2] = o.m; st[3] = live && o.s != 0.f ? (sr - rest / weight) / o.s : 0.f;
+  st[4] = sums[2].m; st[5] = live ? share / weight : 0.f;
+  st[6] = live ? 1.f : 0.f;
+  st[7] = !tail || repeated ? 1.f : 0.f;  // (without the tail nobody looked)
+  return {o, all, sums[2], live};
+}
+// Its loss, a small difference of large terms where student and teacher agree (it falls with tau^2 before it is scaled by it): the
+// teacher's weights, the terms and their sums in 64 bits; the student's sums are fp32 as they come.
+template <typename T, int NT>
+__device__ __forceinline__ void distill_loss(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
+                                             ListEntry mine, const RowSums& r, DistillLds& l, float* loss) {
+  const Teacher te(r.list.m, a, t);
   double weight = 0.0, part = 0.0;
-  if (live)
-    entries_of([&](ListEntry n, int) {
-      const double v = (double)n.v - (double)tm, p = exp2_f64(v * scale);
+  if (r.live)
+    own_entries<T, NT>(row, V, values, ids, a.K, mine, [&](ListEntry n, int) {
+      const double v = (double)n.v - te.m, p = exp2_f64(v * te.scale);
       weight += p;
-      if (p > 1e-300) part += p * (v - ((double)n.x - (double)all.m)) * per;
+      if (p > 1e-300) part += p * (v - ((double)n.x - (double)r.all.m)) * te.per;
     });
   weight = block_sum<NT>(weight, l.redd);
   part = block_sum<NT>(part, l.redd);
-  float tr = 0.f, coef = 0.f;
-  if (live) {
-    const double v = (double)rest - (double)tm * per, p = has_rest ? exp2_f64(v * LOG2E) : 0.0;
+  if (threadIdx.x != 0) return;
+  if (r.live) {
+    const double v = te.rest_x - te.m, p = te.has_rest ? exp2_f64(v * te.scale) : 0.0;
     weight += p;
-    if (p > 1e-300) part += p * (v - ((double)o.m - (double)all.m) * per - log_f64((double)o.s));
-    part = part / weight + (log_f64((double)all.s) - log_f64(weight));
-    tr = (float)(p / weight);
-    const float sr = tail ? o.s * __builtin_amdgcn_exp2f((o.m - all.m) * c) / all.s : 1.f;
-    coef = o.s != 0.f ? (sr - tr) / o.s : 0.f;
+    if (p > 1e-300) part += p * ((v - ((double)r.out.m - (double)r.all.m)) * te.per - log_f64((double)r.out.s));
+    part = part / weight + (log_f64((double)r.all.s) - log_f64(weight));
   }
-  const ExpSum te = {tm, (float)weight};
-  st[0] = all.m; st[1] = live ? 1.f / all.s : 0.f;
-  st[2] = o.m; st[3] = coef;
-  st[4] = te.m; st[5] = live ? 1.f / te.s : 0.f;
-  st[6] = live ? 1.f : 0.f;
-  st[7] = !tail || repeated ? 1.f : 0.f;  // (without the tail nobody looked)
-  if (threadIdx.x == 0) *loss = live ? (float)((double)w * a.tau * a.tau * part) : 0.f;
+  *loss = r.live ? (float)((double)w * a.tau * a.tau * part) : 0.f;
+}
+template <typename T, int NT>
+__device__ __forceinline__ void distill_row(const T* row, int V, const T* values, const int32_t* ids, const DistillArgs& a, int64_t t, float w,
+                                            ListEntry mine, ExpSum own, bool repeated, DistillLds& l, float (&st)[STASH], float* loss) {
+  const RowSums r = distill_sums<T, NT>(row, V, values, ids, a, t, mine, own, repeated, l, st);
+  distill_loss<T, NT>(row, V, values, ids, a, t, w, mine, r, l, loss);
 }
 
 // The gradient of one segment: the tokens outside the list in one pass of 16-byte loads and stores, then those in the list.
@@ -1766,7 +1796,7 @@ __global__ __launch_bounds__(NT, 4) void distill_resident_kernel(const T* __rest
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (sg.end_at[i] >= 0 && !(tail && is_member(sg.end_at[i]))) exp_sum_add(o, sg.ends[i], c);
-  distill_row<T, NT>(row, V, values, ids, a, t, w, mine, o, l.repeated != 0, l, st, loss + t);
+  const RowSums sums = distill_sums<T, NT>(row, V, values, ids, a, t, mine, o, l.repeated != 0, l, st);
   const float f = w * a.tau, mo = st[2], co = st[3] * f;
   const bool together = (((uintptr_t)out ^ (uintptr_t)row) & 15) == 0, live = st[6] != 0.f;
   auto g_of = [&](float x) { return live ? __builtin_amdgcn_exp2f((x - mo) * c) * co : 0.f; };
@@ -1788,6 +1818,8 @@ __global__ __launch_bounds__(NT, 4) void distill_resident_kernel(const T* __rest
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (sg.end_at[i] >= 0) out[sg.end_at[i]] = from_f32<T>(g_of(sg.ends[i]));
+  // (only now: in 64 bits it would not fit the registers beside the row)
+  distill_loss<T, NT>(row, V, values, ids, a, t, w, mine, sums, l, loss + t);
   if (!live) return;
   __threadfence_block();  // (the list's tokens are written again, by other threads)
   __syncthreads();
@@ -2044,20 +2076,21 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     const bool has_rest = on && rest > -INFINITY;
     te_m = Group<G>::max(entry ? val : -INFINITY);
     const bool entries = te_m > -INFINITY;
-    if (has_rest) te_m = fmaxf(te_m, rest * a.tau);
     if (te_m == -INFINITY) te_m = 0.f;
-    const double rest_v = (double)rest - (double)te_m * per, rest_e = has_rest ? exp2_f64(rest_v * LOG2E) : 0.0;
-    const double mine = entry ? exp2_f64(((double)val - (double)te_m) * scale) : 0.0;
+    const double rest_x = (double)rest * (double)a.tau, tm = has_rest ? fmax((double)te_m, rest_x) : (double)te_m;
+    const double rest_e = has_rest ? exp2_f64((rest_x - tm) * scale) : 0.0;
+    const double mine = entry ? exp2_f64(((double)val - tm) * scale) : 0.0;
     const double te_s = Group<G>::sum(mine) + rest_e;
     const bool counts = entries && sum != 0.0;  // (NaN counts)
     double part = 0.0;
-    if (mine > 1e-300) part = mine * (((double)val - (double)te_m) - ((double)xs[first + id] - (double)all_m)) * per;
+    if (mine > 1e-300) part = mine * (((double)val - tm) - ((double)xs[first + id] - (double)all_m)) * per;
     part = Group<G>::sum(part);
-    if (rest_e > 1e-300) part += rest_e * (rest_v - ((double)o_m - (double)all_m) * per - log_f64(o_s));
+    if (rest_e > 1e-300) part += rest_e * ((rest_x - tm - ((double)o_m - (double)all_m)) * per - log_f64(o_s));
     part = part / te_s + (log_f64(sum) - log_f64(te_s));
-    te_inv = 1.f / (float)te_s;
+    const float t_s = 1.f / (float)te_s;
+    te_inv = (float)exp2_f64(((double)te_m - tm) * scale) * t_s;
     all_s = 1.f / (float)sum;
-    coef = o_s != 0.0 ? ((tail ? (float)o_all * all_s : 1.f) - (float)rest_e * te_inv) / (float)o_s : 0.f;
+    coef = o_s != 0.0 ? ((tail ? (float)o_all * all_s : 1.f) - (float)rest_e * t_s) / (float)o_s : 0.f;
     live = counts ? 1.f : 0.f;
     if (v == 0 && t0 < rows) {
       loss[t] = counts ? (float)((double)w * a.tau * a.tau * part) : 0.f;

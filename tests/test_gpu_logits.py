@@ -209,6 +209,17 @@ def test_extreme_temperatures(pg, V):
         check_top(pg, x, 20, tau)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_sample_filtered_ties_in_unaligned_rows(pg, dtype, shift):
+    """Of equal largest entries the first index, wherever the row's 16-byte vectors begin."""
+    for V, k in ((133842, 512), (5003, 0), (40001, 700)):
+        x = torch.zeros(4 * (V + 1) + shift, dtype=dtype, device=DEV)[shift:].view(4, V + 1)[:, :V]
+        x[1, 0], x[2, :2], x[3, -1] = 1.0, -1.0, 1.0
+        check_sample(pg, x, temperature=0.0, top_k=k)
+        check_sample(pg, x, top_k=k, q=torch.full((4, V), float("inf"), device=DEV))
+
+
 def test_sample_filtered_strided_inputs_and_outputs(pg):
     x = rows(8, 333, torch.bfloat16, 2, pad=7, shift=5)
     q = torch.empty(8, 400, device=DEV).exponential_(1.0)[:, 3:336]
@@ -300,6 +311,26 @@ def test_distill_odd_rows(pg, dtype, tail, V):
     w[5] = w[6] = w[7] = 0.0
     w[10] = -0.5
     check_distill(pg, x, v.to(DEV), i.to(DEV), r.to(DEV) if tail else None, 1.5, w.to(DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [30, 700, 20011])
+def test_distill_of_masked_teacher_rows(pg, dtype, V):
+    """Teachers' rows at the type's lowest value, wholly or but for fewer entries than the record holds; rows far from 0: the
+    rest's fp32 steps are as large as whole probabilities there, but it is one number."""
+    k, tau = 4, 8.0
+    low = torch.finfo(dtype).min
+    x = rows(6, V, dtype, V)
+    x[0] = low
+    x[1, 3:] = low
+    x[2] += 10000.0
+    x[3] -= 10000.0
+    x[4] = float("-inf")
+    x[4, 5] = low
+    v, i, r = pg.ops.top_logits(x, k, temperature=tau)
+    check_distill(pg, rows(6, V, dtype, V + 1), v, i, r, tau, None)
+    check_distill(pg, x, v, i, r, tau, None)
+    check_distill(pg, x[:4], v[:4], i[:4], None, tau, None)
 
 
 @pytest.mark.parametrize("V,k", [(5, 20), (30, 33), (30, 64), (30, 200), (64, 65), (70, 1024)])
