@@ -561,7 +561,7 @@ __device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float t
     *rest_out = rest.m == INFINITY ? INFINITY : rest.s > 0.f ? (float)((double)rest.m / tau + log((double)rest.s)) : -INFINITY;
 }
 
-// 1024 rows of 131072 bf16, k 64: 88 us (268 MB; reading alone 45), whole rows by one workgroup of 256, four a CU.  A segment's load, the
+// 1024 rows of 131072 bf16, k 64: 88-92 us (268 MB; reading alone 45), whole rows by one workgroup of 256, four a CU.  A segment's load, the
 // rounds that count for the bound, and the sum follow one another, and four workgroups overlap them only in part; a fifth does
 // not fit beside 128 registers a thread.  16 rows of 50021 fp32, k 100, in 13 segments each: 8.9 us.
 template <typename T, int NT, int VPT, bool MANY>
