@@ -762,10 +762,12 @@ struct SampleArgs {
   float temperature, top_p, min_p;
   int top_k, empty;  // empty: the token of a row with nothing above -inf
   const float* temps; const int32_t* ks; const float* ps; const float* mins;
-  // (positive temperatures within MIN_TAU .. MAX_TAU, where no scale or product of a scale leaves fp32's range)
+  // (positive temperatures within MIN_TAU .. MAX_TAU, where no scale or product of a scale leaves fp32's range; a row's negative
+  // top_k is 0, off)
   __device__ __forceinline__ RowFilter row(int64_t t) const {
     const float given = temps ? temps[t] : temperature;
-    return {given > 0.f ? fminf(fmaxf(given, MIN_TAU), MAX_TAU) : 0.f, ps ? ps[t] : top_p, mins ? mins[t] : min_p, ks ? ks[t] : top_k};
+    return {given > 0.f ? fminf(fmaxf(given, MIN_TAU), MAX_TAU) : 0.f, ps ? ps[t] : top_p, mins ? mins[t] : min_p,
+            ks ? max(ks[t], 0) : top_k};
   }
 };
 // ------------------------------------------------------------------ one row by a whole workgroup, any boundary
