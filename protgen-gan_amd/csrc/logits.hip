@@ -17,6 +17,7 @@ constexpr float MIN_TAU = 1e-30f, MAX_TAU = 1e30f;
 constexpr double LOG2E = 1.4426950408889634074;
 constexpr double LN2 = 0.69314718055994530942;
 
+__device__ __forceinline__ float no_nan(float x) { return x == x ? x : -INFINITY; }
 __device__ __forceinline__ uint32_t value_key(float x) {
   x = x + 0.0f;  // -0 -> +0
   if (x != x) x = -INFINITY;
@@ -161,17 +162,26 @@ constexpr int MERGE = 4096;  // keys of all segments of one row in LDS
 constexpr int MAX_SEG_K = 512;
 constexpr int max_cap(int K) { return K > 128 ? 1088 : 512; }  // keys a segment may leave
 
-// The largest of three, NaN passed over.  (fmaxf costs a second instruction per operand here, which quiets signalling NaN first;
-// v_max3_f32 does that by itself.)
+// The largest of three.  Quiet NaN is passed over, but a signalling one makes its first maximum a quiet NaN, with which the other
+// operand is lost: only for operands that are none, or where a NaN decides the result anyway.  The compiler forms the same
+// instruction from two fmaxf, so raw entries do not go through those either.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
-template <int E> __device__ __forceinline__ float vec_max(const float (&o)[E], float m = -INFINITY) {
-  if constexpr (E == 1) return max3(m, m, o[0]);
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float maximum3(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// The largest entry of a vector.  STICKY: NaN if one is NaN; else for vectors without NaN, and for sums that keep NaN, where any
+// largest will do beside one.
+template <int E, bool STICKY = false> __device__ __forceinline__ float vec_max(const float (&o)[E]) {
+  float m = -INFINITY;
 #pragma unroll
-  for (int e = 0; e + 1 < E; e += 2) m = max3(m, o[e], o[e + 1]);
+  for (int e = 0; e + 1 < E; e += 2) m = STICKY ? maximum3(m, o[e], o[e + 1]) : max3(m, o[e], o[e + 1]);
   return m;
 }
 // The exponentials of E entries of which vm is the largest, with one rescaling for all of them.  NaN as -inf (looked for in the
@@ -214,7 +224,7 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
 }
 __device__ __forceinline__ void exp_sum_one(ExpSum& a, float x, float c) {
   const float o[1] = {x};
-  exp_sum_vec<1>(a, o, vec_max<1>(o), c);
+  exp_sum_vec<1>(a, o, no_nan(x), c);
 }
 
 // exp((x - m) / temperature) for x <= m in whole multiples of 2^-40: sums of these are the same in any order.
@@ -303,6 +313,13 @@ struct SegHead {      // what a segment leaves for the merge
   uint32_t n, pad[3];
 };
 
+// A word of one or two entries, those marked in `in` replaced by -inf.
+template <typename T> __device__ __forceinline__ uint32_t without(uint32_t d, uint32_t in) {
+  if (sizeof(T) == 4) return in & 1 ? 0xff800000u : d;
+  d = in & 1 ? (d & 0xffff0000u) | 0xff80u : d;
+  return in & 2 ? (d & 0xffffu) | 0xff800000u : d;
+}
+
 template <typename T, int NT, int VPT> struct Segment {
   static constexpr int E = 16 / (int)sizeof(T), VECS = NT * VPT;
   uint4 d[VPT];
@@ -337,6 +354,13 @@ template <typename T, int NT, int VPT> struct Segment {
   __device__ __forceinline__ void fresh() {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) asm volatile("" : "+v"(d[j].x), "+v"(d[j].y), "+v"(d[j].z), "+v"(d[j].w));
+  }
+  // Vector j without the entries marked in `in`, one bit each.
+  __device__ __forceinline__ void remove(int j, uint32_t in) {
+    d[j].x = without<T>(d[j].x, in);
+    d[j].y = without<T>(d[j].y, in >> E / 4);
+    d[j].z = without<T>(d[j].z, in >> E / 2);
+    d[j].w = without<T>(d[j].w, in >> E * 3 / 4);
   }
   // f(value, index) over this thread's entries of segments seg .. seg + count - 1, read again from memory
   template <typename F> static __device__ __forceinline__ void entries(const T* row, int V, int seg, int count, int nseg, F f) {
@@ -378,17 +402,46 @@ __device__ __forceinline__ int collect(const T* row, int V, int seg, int count, 
   if (threadIdx.x == 0) l.n = 0;
 #pragma unroll 1
   for (int s = 0;; ++s) {
-    float low = INFINITY;
+    float low = INFINITY, sm[GROUPS], nan = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) sm[g] = -INFINITY;
     sg.fresh();
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       float o[E];
       unpack(sg.d[j], o);
-      const float vm = vec_max<E>(o);
-      gm[j % GROUPS] = max3(gm[j % GROUPS], gm[j % GROUPS], vm);
+      const float vm = vec_max<E, true>(o);
+      sm[j % GROUPS] = maximum3(sm[j % GROUPS], sm[j % GROUPS], vm);
       low = sg.has(j) && vm < low ? vm : low;
     }
-    gm[0] = fmaxf(gm[0], fmaxf(sg.ends[0], sg.ends[1]));
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) nan = maximum3(nan, nan, sm[g]);
+    if (nan != nan) {  // a NaN among this thread's entries: -inf from here on
+      sg.fresh();
+      low = INFINITY;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) sm[g] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        float o[E];
+        unpack(sg.d[j], o);
+        uint32_t in = 0;
+        float vm = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          in |= (o[e] != o[e]) << e;
+          vm = o[e] > vm ? o[e] : vm;
+        }
+        sg.remove(j, in);
+        sm[j % GROUPS] = vm > sm[j % GROUPS] ? vm : sm[j % GROUPS];
+        low = sg.has(j) && vm < low ? vm : low;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) gm[g] = fmaxf(gm[g], sm[g]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) gm[0] = sg.ends[i] > gm[0] ? sg.ends[i] : gm[0];
     uint32_t mk[GROUPS];
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) mk[g] = gm[g] > -INFINITY ? value_key(gm[g]) : 0;
@@ -415,7 +468,7 @@ __device__ __forceinline__ int collect(const T* row, int V, int seg, int count, 
       }
     }
     ExpSum part = sum.end();
-    if (!sum.ok()) {  // (vectors without an entry above -inf or all with one above the bound, entries far apart, NaN)
+    if (!sum.ok()) {  // (vectors without an entry above -inf or all with one above the bound, entries far apart)
       part = {-FLT_MAX, 0.f};
       sg.fresh();
 #pragma unroll
@@ -428,7 +481,7 @@ __device__ __forceinline__ int collect(const T* row, int V, int seg, int count, 
     }
     rest = s == 0 ? part : exp_sum_join(rest, part, c);
     auto take = [&](float x, int i) {
-      x = fmaxf(x, -INFINITY);
+      x = no_nan(x);
       const bool in = x >= thr && (!FINITE || x > -INFINITY);
       if (in) {
         const uint32_t p = atomicAdd(&l.n, 1u);
@@ -448,7 +501,7 @@ __device__ __forceinline__ int collect(const T* row, int V, int seg, int count, 
       unpack(l.vec[i], o);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (!take(o[e], l.at[i] + e)) most = fmaxf(most, o[e]);
+        if (!take(o[e], l.at[i] + e) && o[e] > most) most = o[e];
     }
     most = block_max<NT>(most, l.red);
     if (most > -INFINITY) {  // the staged vectors are in no fixed order: their sum is one of whole multiples of 2^-40 of the largest
@@ -845,12 +898,12 @@ __device__ __forceinline__ Border border(const T* row, int V, Bins bins, uint64_
       };
       if (d < 0)
         each<T, NT>(row, V, [&](int i, float x) {
-          x = fmaxf(x, -INFINITY);
+          x = no_nan(x);
           if (!below(x, i)) put(bins.of(x), x);
         });
       else
         for (int i = threadIdx.x; i < V; i += NT) {
-          const float x = fmaxf(to_f32<T>(row[i]), -INFINITY);
+          const float x = no_nan(to_f32<T>(row[i]));
           const uint64_t k = entry_key(x, i);
           if (k >= floor && bins.of(x) == at.bin && (k & at.mask) == at.prefix) put(n_bins - 1 - ((int)(k >> shift) & (n_bins - 1)), x);
         }
@@ -902,7 +955,7 @@ struct Weight {
 template <typename T, int NT>
 __device__ __forceinline__ void gather_bin(const T* row, int V, uint64_t floor, const Border& at, RowLds<NT>& l) {
   each<T, NT>(row, V, [&](int i, float x) {
-    x = fmaxf(x, -INFINITY);
+    x = no_nan(x);
     if (x < at.lo || x > at.hi) return;
     const uint64_t k = entry_key(x, i);
     if (k < floor || (k & at.mask) != at.prefix) return;
@@ -1259,7 +1312,7 @@ __global__ __launch_bounds__(NT) void sample_bins_kernel(const T* __restrict__ l
   for (int i = threadIdx.x; i < BINS; i += NT) mass[i] = 0;
   __syncthreads();
   each<T, NT>(logits + t * ld + at.i0, at.n, [&](int, float x) {
-    x = fmaxf(x, -INFINITY);
+    x = no_nan(x);
     atomicAdd((unsigned long long*)&mass[bins.of(x)], by_p ? (unsigned long long)fixed(weight(x)) : 1ull);
   });
   __syncthreads();
@@ -1384,7 +1437,7 @@ __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, i
   const T* row = logits + t * ld;
   const float c = (float)(LOG2E / (double)tau);
   float m = -INFINITY;
-  each<T, NT>(row, V, [&](int, float x) { m = fmaxf(m, x); });
+  each<T, NT>(row, V, [&](int, float x) { m = x > m ? x : m; });
   m = block_max<NT>(m, l.red);
   const Bins bins(m, BINS / 32.f);
   const uint64_t B = border<T, NT>(row, V, bins, 0, false, K, 0.0, [](float) { return 0.0; }, l,
@@ -1739,13 +1792,6 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logit
   if (GRAD) distill_grad<T, NT>(row, V, sp, values, ids, a, st, w * a.tau * (upstream ? upstream[t] : 1.f), grad + t * ld_grad);
 }
 
-// A word of one or two entries, those marked in `in` replaced by -inf.
-template <typename T> __device__ __forceinline__ uint32_t without(uint32_t d, uint32_t in) {
-  if (sizeof(T) == 4) return in & 1 ? 0xff800000u : d;
-  d = in & 1 ? (d & 0xffff0000u) | 0xff80u : d;
-  return in & 2 ? (d & 0xffffu) | 0xff800000u : d;
-}
-
 // Loss and gradient with the row in registers, read once: NT * 16 vectors of 16 bytes.  4096 x 32768 bf16, k 32: 130 us, against the
 // 105 of reading and writing it once at the rate of a copy; two passes, the second from the memory-side cache, took 168.  2048 x 65536
 // by 512 threads: 141 us.
@@ -1793,10 +1839,7 @@ __global__ __launch_bounds__(NT, 4) void distill_resident_kernel(const T* __rest
       const int at = j * NT + (int)threadIdx.x + 1;
       const uint32_t in = sg.has(j) ? (uint32_t)(E == 8 ? bytes[at] : bytes[at >> 1] >> (at & 1) * 4 & 15) : 0;
       if (in) {
-        sg.d[j].x = without<T>(sg.d[j].x, in);
-        sg.d[j].y = without<T>(sg.d[j].y, in >> E / 4);
-        sg.d[j].z = without<T>(sg.d[j].z, in >> E / 2);
-        sg.d[j].w = without<T>(sg.d[j].w, in >> E * 3 / 4);
+        sg.remove(j, in);
       }
       __builtin_amdgcn_sched_barrier(0);
     }

@@ -1,8 +1,10 @@
 """Corners of the operators over rows of vocabulary logits that documented arguments reach.  Bounds as in test_gpu_logits."""
+import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_logits import DEV, TYPES, check_sample, rows
+from tests import logits_specs as spec
+from tests.test_gpu_logits import DEV, TYPES, check_distill, check_sample, check_top, record, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +35,56 @@ def test_a_negative_top_k_of_a_row_is_off(pg, dtype, T, V):
     check_sample(pg, x, top_k=k, top_p=p)
     check_sample(pg, x, top_k=k, top_p=p, min_p=least)
     check_sample(pg, rows(T, V, dtype, V + 1), top_k=k, top_p=p, min_p=least)
+
+
+def signalling(x):
+    """x with signalling NaN (quiet bit clear) in every third place and on both sides of each row's largest entries."""
+    bits = x.view(torch.int16 if x.dtype == torch.bfloat16 else torch.int32)
+    bad = 0x7f81 if x.dtype == torch.bfloat16 else 0x7f810000
+    V = x.shape[1]
+    at = torch.arange(V, device=x.device)
+    top = x.float().topk(min(V, 9), dim=1).indices
+    near = torch.zeros_like(bits, dtype=torch.bool)
+    for o in (-1, 1):
+        near.scatter_(1, (top + o).clamp(0, V - 1), True)
+    near |= at % 3 == 0
+    near.scatter_(1, top, False)
+    bits[near] = bad
+    assert not torch.isnan(x.gather(1, top).float()).any() and torch.isnan(x.float()).any()
+    return x
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,k", [(30, 4), (64, 9), (700, 33), (1003, 100), (5001, 64), (40000, 200), (131072, 64)])
+def test_signalling_nan_counts_as_any_other(pg, dtype, V, k):
+    x = signalling(rows(12, V, dtype, V))
+    check_top(pg, x, k)
+    for n, f in enumerate([{}, {"top_k": 5}, {"top_p": 0.8}, {"min_p": 0.05}, {"temperature": 0.0}, {"top_k": min(V, 600), "top_p": 0.9}]):
+        check_sample(pg, x, seed=n, **f)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [9000, 40003])
+def test_signalling_nan_in_many_rows(pg, dtype, V):
+    """The cuts of calls with rows enough to fill the chip."""
+    T = 1030
+    x = torch.zeros(T, V, dtype=dtype, device=DEV)
+    few = signalling(rows(4, V, dtype, V))
+    at = torch.tensor([0, 1, T // 2, T - 1], device=DEV)
+    bits = torch.int16 if dtype == torch.bfloat16 else torch.int32
+    x.view(bits)[at] = few.view(bits)
+    v, i, r = pg.ops.top_logits(x, 33, temperature=2.0)
+    wv, wi, wr = spec.top_logits(few, 33, 2.0)
+    assert np.array_equal(i[at].cpu().numpy(), wi) and np.array_equal(v[at].double().cpu().numpy(), wv)
+    q = torch.empty(T, V, device=DEV).exponential_(1.0, generator=torch.Generator(DEV).manual_seed(2))
+    pred, _ = pg.ops.sample_filtered(x, q, top_k=40, top_p=0.9)
+    assert np.array_equal(pred[at].cpu().numpy(), spec.sample(few, q[at], 1.0, 40, 0.9, 0.0)[0])
+
+
+@pytest.mark.parametrize("V", [30, 700, 9001])
+def test_signalling_nan_in_a_students_row(pg, V):
+    x, v, i, r = record(pg, 4, V, 6, torch.bfloat16, V, 1.0, True)
+    x[:2] = 0
+    x = torch.cat([signalling(rows(2, V, torch.bfloat16, V)), x[2:]])
+    check_distill(pg, x, v, i, r, 1.0, None)
+    check_distill(pg, x, v, i, None, 1.0, torch.tensor([0.0, 1.0, 1.0, 2.0], device=DEV))
