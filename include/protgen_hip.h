@@ -349,6 +349,7 @@ int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* n
  * or a value of -inf or NaN is absent).  With t = softmax of values / temperature (and of rest, when given, for the event "any
  * other token"), s = softmax(logits / temperature):
  *   loss[t] = weight temperature^2 [ sum_e t_e log(t_e / s_id(e)) + t_rest log(t_rest / s_rest) ].
+ * A row with an entry or a rest of +inf, or a rest of NaN, has no such t: its loss and gradient are NaN.
  * An id that occurs twice counts as two entries and once in the set that s_rest leaves out.  weights [T] (NULL = 1): a row with
  * weight 0 is not read and gives loss 0 and gradient 0, and so does a row with no entry or with no logit above -inf.
  * pg_distill_fwd leaves pg_distill_stash_floats() floats per row (16-byte aligned) for pg_distill_bwd, which writes

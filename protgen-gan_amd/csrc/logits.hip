@@ -144,6 +144,9 @@ __device__ __forceinline__ double exp2_f64(double t) {
   return ldexp(p, (int)n);
 }
 
+// NaN kept (exp2_f64 takes it for -1022)
+__device__ __forceinline__ double exp2_or_nan(double t) { return t == t ? exp2_f64(t) : t; }
+
 // log s in 64 bits for s > 0: the fp32 logarithm y and what is left, s e^-y - 1 (below 2^-20: its own logarithm to 2^-40).
 __device__ __forceinline__ double log_f64(double s) {
   const double y = (double)logf((float)s);
@@ -1630,7 +1633,8 @@ __device__ __forceinline__ void own_entries(const T* row, int V, const T* values
   }
 }
 // The teacher's weights are taken relative to the largest of the list's entries and the rest, in 64 bits: the rest is in units of
-// x / tau, and in fp32 its conversion would move it by whole probabilities where logits are far from 0.
+// x / tau, and in fp32 its conversion would move it by whole probabilities where logits are far from 0.  An infinite entry or rest,
+// or a rest of NaN, makes the sum of the weights NaN, and with it the row's loss and gradient.
 struct Teacher {
   double per, scale, rest_x, m;  // 1 / tau, log2(e) / tau, rest tau, the reference
   bool has_rest;
@@ -1639,7 +1643,7 @@ struct Teacher {
     per = 1.0 / (double)a.tau;
     scale = per * LOG2E;
     rest_x = (double)rest * (double)a.tau;
-    has_rest = rest > -INFINITY;
+    has_rest = !(rest == -INFINITY);
     m = has_rest ? fmax((double)list_max, rest_x) : (double)list_max;
   }
 };
@@ -1662,7 +1666,7 @@ __device__ __forceinline__ RowSums distill_sums(const T* row, int V, const T* va
   });
   block_exp_sums<NT, 3>(sums, c, l.sums);
   const ExpSum o = sums[0], all = tail ? exp_sum_join(o, sums[1], c) : o;
-  const bool live = sums[2].s > 0.f && all.s != 0.f;  // (NaN lives)
+  const bool live = sums[2].s != 0.f && all.s != 0.f;  // (NaN lives)
   const Teacher te(sums[2].m, a, t);
   const float share = __builtin_amdgcn_exp2f((float)(((double)sums[2].m - te.m) * te.scale));
   const float rest = te.has_rest ? __builtin_amdgcn_exp2f((float)((te.rest_x - te.m) * te.scale)) : 0.f;
@@ -1684,7 +1688,7 @@ __device__ __forceinline__ void distill_loss(const T* row, int V, const T* value
   double weight = 0.0, part = 0.0;
   if (r.live)
     own_entries<T, NT>(row, V, values, ids, a.K, mine, [&](ListEntry n, int) {
-      const double v = (double)n.v - te.m, p = exp2_f64(v * te.scale);
+      const double v = (double)n.v - te.m, p = exp2_or_nan(v * te.scale);
       weight += p;
       if (p > 1e-300) part += p * (v - ((double)n.x - (double)r.all.m)) * te.per;
     });
@@ -1692,7 +1696,7 @@ __device__ __forceinline__ void distill_loss(const T* row, int V, const T* value
   part = block_sum<NT>(part, l.redd);
   if (threadIdx.x != 0) return;
   if (r.live) {
-    const double v = te.rest_x - te.m, p = te.has_rest ? exp2_f64(v * te.scale) : 0.0;
+    const double v = te.rest_x - te.m, p = te.has_rest ? exp2_or_nan(v * te.scale) : 0.0;
     weight += p;
     if (p > 1e-300) part += p * ((v - ((double)r.out.m - (double)r.all.m)) * te.per - log_f64((double)r.out.s));
     part = part / weight + (log_f64((double)r.all.s) - log_f64(weight));
@@ -2133,13 +2137,13 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
     const double o_s = Group<G>::sum(out ? mass : 0.0), in_s = Group<G>::sum(out ? 0.0 : mass);
     const double o_all = o_s == 0.0 ? 0.0 : o_s * exp2_f64(((double)o_m - (double)all_m) * scale), sum = o_all + in_s;
     const float rest = tail ? a.rest[t] : -INFINITY;
-    const bool has_rest = on && rest > -INFINITY;
+    const bool has_rest = on && !(rest == -INFINITY);
     te_m = Group<G>::max(entry ? val : -INFINITY);
     const bool entries = te_m > -INFINITY;
     if (te_m == -INFINITY) te_m = 0.f;
     const double rest_x = (double)rest * (double)a.tau, tm = has_rest ? fmax((double)te_m, rest_x) : (double)te_m;
-    const double rest_e = has_rest ? exp2_f64((rest_x - tm) * scale) : 0.0;
-    const double mine = entry ? exp2_f64(((double)val - tm) * scale) : 0.0;
+    const double rest_e = has_rest ? exp2_or_nan((rest_x - tm) * scale) : 0.0;
+    const double mine = entry ? exp2_or_nan(((double)val - tm) * scale) : 0.0;
     const double te_s = Group<G>::sum(mine) + rest_e;
     const bool counts = entries && sum != 0.0;  // (NaN counts)
     double part = 0.0;

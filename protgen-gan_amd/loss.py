@@ -177,7 +177,8 @@ def distillation_loss(student_logits, top_values, top_ids, rest=None, temperatur
 
     over the record's entries e and, with `rest`, the event "any other token" (without it the teacher is renormalised over its
     entries).  `weights` fp32 [...]: rows with weight 0 (padding, positions that are not scored) are not read and get no
-    gradient, whatever they hold.  Differentiable in student_logits, once; ids outside the vocabulary (-1) mark absent entries."""
+    gradient, whatever they hold.  Differentiable in student_logits, once; ids outside the vocabulary (-1) mark absent entries.
+    A record that is not finite (an overflowing teacher: +inf among the values or in the rest) gives a NaN loss and gradient."""
     if top_values.requires_grad or (rest is not None and rest.requires_grad) or (weights is not None and weights.requires_grad):
         raise ValueError("top_values, rest and weights must not require a gradient: the loss is differentiable in the student's logits")
     return _DistillFn.apply(student_logits, ops._distill_args(student_logits, top_values, top_ids, rest, weights, temperature))

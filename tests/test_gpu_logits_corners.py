@@ -88,3 +88,46 @@ def test_signalling_nan_in_a_students_row(pg, V):
     x = torch.cat([signalling(rows(2, V, torch.bfloat16, V)), x[2:]])
     check_distill(pg, x, v, i, r, 1.0, None)
     check_distill(pg, x, v, i, None, 1.0, torch.tensor([0.0, 1.0, 1.0, 2.0], device=DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("T,V", [(9, 30), (9, 64), (9, 700), (9, 20011), (1100, 9001)])
+def test_records_that_are_not_finite_give_nan(pg, dtype, tail, T, V):
+    """+inf among a row's values, +inf or NaN as its rest: no softmax, so NaN in the row's loss and gradient, whatever the sizes; the
+    other rows, rows of weight 0 among them, as ever."""
+    k = 6
+    x, v, i, r = record(pg, T, V, k, dtype, V, 2.0, True)
+    inf, nan = float("inf"), float("nan")
+    v[0, 0] = inf
+    v[1, :2] = inf
+    v[2, 3], i[2, 3] = inf, -1  # (an absent entry's value does not count)
+    v[3, 1] = nan               # (absent)
+    v[4, 0] = inf
+    r[5], r[6], r[7] = inf, nan, nan
+    w = torch.ones(T, device=DEV)
+    w[4] = w[7] = 0.0
+    bad = torch.zeros(T, dtype=torch.bool)
+    bad[[0, 1] + ([5, 6] if tail else [])] = True
+    rest = r if tail else None
+    leaf = x.detach().requires_grad_()
+    loss = pg.loss.distillation_loss(leaf, v, i, rest=rest, temperature=2.0, weights=w)
+    loss.sum().backward()
+    both = pg.ops.distill_loss_grad(x, v, i, rest=rest, temperature=2.0, weights=w)
+    for a, g in ((loss.detach(), leaf.grad), both):
+        assert torch.equal(a.isnan().cpu(), bad)
+        assert torch.equal(g.isnan().all(1).cpu(), bad) and torch.equal(g.isnan().any(1).cpu(), bad)
+        assert not a[4].any() and not g[4].any() and not a[7].any() and not g[7].any()
+    few = torch.tensor([2, 3, 4, 7, 8] + ([] if tail else [5, 6]), device=DEV)
+    check_distill(pg, x[few], v[few], i[few], None if rest is None else rest[few], 2.0, w[few])
+
+
+@pytest.mark.parametrize("V", [30, 700])
+def test_the_record_of_a_row_with_an_infinite_logit(pg, V):
+    """top_logits' own record of an overflowing teacher, inside the list and in the rest."""
+    x, t = rows(2, V, torch.float32, V), rows(2, V, torch.float32, V + 1)
+    t[0, 3] = t[1, 2] = t[1, 5] = float("inf")
+    v, i, r = pg.ops.top_logits(t, 1)
+    assert torch.isinf(v).all() and r[1] == float("inf") and torch.isfinite(r[0])
+    loss, grad = pg.ops.distill_loss_grad(x, v, i, rest=r)
+    assert loss.isnan().all() and grad.isnan().all()
