@@ -1091,19 +1091,20 @@ __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict
   bool sure = true;
   if (f.top_p < 1.f) {
     if (nk_in || nk == V) {
-      // the mass outside: fp32 sums of up to 2^7 terms per thread and a tree, their relative error below 2^-15
-      const double rest = nk_in ? 0.0 : left * MASS_ONE, err = rest * 0x1p-15;
-      const double need = fmax(1.0, ceil((double)f.top_p * ((double)l.mass[(nk_in ? keep : n) - 1] + rest)));
+      // the mass outside: fp32 sums of up to 2^7 terms per thread and a tree, their relative error below 2^-15, of masses that are
+      // not rounded to multiples of 2^-40 (each off by less than half a multiple, and by less than itself)
+      const double rest = nk_in ? 0.0 : left * MASS_ONE, err = rest * 0x1p-15 + fmin(rest, 0.5 * (V - n));
+      const double share = (double)f.top_p * ((double)l.mass[(nk_in ? keep : n) - 1] + rest), need = fmax(1.0, ceil(share));
       for (int i = a0; i < a1; ++i)
         if ((i == 0 || (double)l.mass[i - 1] < need) && (double)l.mass[i] >= need) l.cut = i;
       __syncthreads();
       const int at = l.cut;  // (n: beyond the list)
       const double before = at > 0 ? (double)l.mass[min(at, nv) - 1] : 0.0;
       if (at < nv) {
-        if (err > 0.0) sure = before < need - err && (double)l.mass[at] >= need + err;
+        if (err > 0.0) sure = before < fmax(1.0, share - err) && (double)l.mass[at] >= fmax(1.0, share + err);
         keep = min(keep, at + 1);
       } else if (!nk_in) {
-        sure = before < need - err;
+        sure = before < fmax(1.0, share - err);
       }
     } else {
       sure = false;  // (the mass of the first k is not known)
@@ -2044,10 +2045,10 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
   bool keep = v < V && x > -INFINITY && f.above_min_p(x, m);
   double total;
   if (f.top_p < 1.f && !greedy) {
-    // weights in the row's order, their running sum, and from it how many entries stay: an entry does while the mass before it is
-    // below the share of the first k's
+    // weights in the row's order, in multiples of 2^-40 as for wider vocabularies (by fixed()'s rounding; sums of 64 are exact), their
+    // running sum, and from it how many entries stay: an entry does while the mass before it is below the share of the first k's
     const int rank = rank_of<G>(keys + first, V, key);
-    weights[first + rank] = w;  // (lanes past V: key 0, w 0, ranks V.. by their lane)
+    weights[first + rank] = (w + 4096.0) - 4096.0;  // (lanes past V: key 0, w 0, ranks V.. by their lane)
     const int nk = f.top_k > 0 && f.top_k < V ? f.top_k : V;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const double mine = weights[threadIdx.x];

@@ -131,3 +131,26 @@ def test_the_record_of_a_row_with_an_infinite_logit(pg, V):
     assert torch.isinf(v).all() and r[1] == float("inf") and torch.isfinite(r[0])
     loss, grad = pg.ops.distill_loss_grad(x, v, i, rest=r)
     assert loss.isnan().all() and grad.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [5, 30, 32, 33, 64, 65, 700, 20000, 100003])
+def test_the_resolution_of_top_p_is_one_for_all_vocabularies(pg, dtype, V):
+    """Each entry's mass counts in multiples of 2^-40 of the largest's.  Two equal largest entries, top_p exactly 0.5: one stays where
+    every other mass rounds to 0, however many they are, both where one other weighs a multiple.  The second entry's draw wins
+    where it stays."""
+    ln2 = float(np.log(2.0))
+    x = torch.full((4, V), -60.0)
+    x[3] = -45 * ln2       # 1/32 multiples each: none
+    x[:, 1] = x[:, 3] = 0.0
+    x[1, 0] = -41.5 * ln2  # 0.35 multiples: none
+    x[2, 0] = -38.5 * ln2  # 2.8 multiples: three
+    x = x.to(dtype).to(DEV)
+    assert float(x[1, 0]) < -41.2 * ln2 and -38.7 * ln2 < float(x[2, 0]) < -38.2 * ln2 and float(x[3, 0]) < -44 * ln2
+    q = torch.ones(4, V, device=DEV)
+    q[:, 3] = 0.125
+    for T in (4, 300):
+        pred, conf = pg.ops.sample_filtered(x.repeat(T // 4, 1), q.repeat(T // 4, 1), top_p=0.5)
+        assert pred.tolist() == [1, 1, 3, 1] * (T // 4) and conf.tolist() == [1.0, 1.0, 0.5, 1.0] * (T // 4)
+    pred, conf = pg.ops.sample_filtered(x, q, top_p=0.5, top_k=min(V, 100))
+    assert pred.tolist() == [1, 1, 3, 1] and conf.tolist() == [1.0, 1.0, 0.5, 1.0]
