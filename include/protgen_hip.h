@@ -332,7 +332,7 @@ int pg_commit_topk(int64_t* ids, const int64_t* pred, const float* conf, int B, 
 int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k);
 int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, int V, int k, float temperature, void* values, int32_t* ids,
                   float* rest, void* workspace, int64_t workspace_bytes, void* stream);
-/* pg_sample_tokens over any vocabulary with truncation (generate.py / models.py:24-27 sample the whole softmax).  With
+/* pg_sample_tokens over any vocabulary below 2^24 with truncation (generate.py / models.py:24-27 sample the whole softmax).  With
  * w_v = exp((x_v - max) / temperature), the row keeps its first min(k, n_p, n_m) entries: n_p = those before which less than
  * top_p of the first k entries' mass lies, n_m = those with w >= min_p.  pred = argmax w_v / noise_v over them (ties: lowest
  * index; noise ~ Exp(1), row t at noise + t*ld_noise), conf = w_pred / their mass.  top_k 0, top_p 1, min_p 0 switch a filter

@@ -12,7 +12,7 @@
 namespace {
 
 constexpr int MAX_K = 1024;
-constexpr int MAX_VOCAB = 1 << 24;  // 2^24 weights of at most 2^40 each fit the 64-bit fixed-point sums
+constexpr int MAX_VOCAB = 1 << 24;  // sampling: one less, so that a row of weights of 2^40 each sums to less than 2^64
 constexpr float MIN_TAU = 1e-30f, MAX_TAU = 1e30f;
 constexpr double LOG2E = 1.4426950408889634074;
 constexpr double LN2 = 0.69314718055994530942;
@@ -2383,6 +2383,7 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
                                   int64_t workspace_bytes, void* stream) {
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
+  if (V == MAX_VOCAB) return PG_ERR_UNSUPPORTED;
   if (!noise || ld_noise < 0 || !pred || !conf || empty < -1) return PG_ERR_ARG;  // (below -1: rows still open between two launches)
   if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
       (!mins && !(min_p >= 0.f && min_p <= 1.f)))

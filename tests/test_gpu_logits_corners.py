@@ -154,3 +154,15 @@ def test_the_resolution_of_top_p_is_one_for_all_vocabularies(pg, dtype, V):
         assert pred.tolist() == [1, 1, 3, 1] * (T // 4) and conf.tolist() == [1.0, 1.0, 0.5, 1.0] * (T // 4)
     pred, conf = pg.ops.sample_filtered(x, q, top_p=0.5, top_k=min(V, 100))
     assert pred.tolist() == [1, 1, 3, 1] and conf.tolist() == [1.0, 1.0, 0.5, 1.0]
+
+
+def test_the_largest_sampled_vocabulary(pg):
+    """2^24 - 1 equal entries: 2^23 of them hold half the mass, in the order of their index."""
+    V = 2 ** 24 - 1
+    x = torch.full((1, V), 3.0, dtype=torch.bfloat16, device=DEV)
+    q = torch.empty(1, V, device=DEV).exponential_(1.0, generator=torch.Generator(DEV).manual_seed(1))
+    q[0, 2 ** 23:] *= 1e-6
+    pred, conf = pg.ops.sample_filtered(x, q, top_p=0.5)
+    assert int(pred) == int(q[0, :2 ** 23].argmin()) and float(conf) == 2.0 ** -23
+    pred, conf = pg.ops.sample_filtered(x, q)
+    assert int(pred) == int(q[0].argmin())
