@@ -402,9 +402,11 @@ def distill_fwd(logits, values, ids, rest=None, weights=None, temperature=1.0):
 
 def distill_bwd(logits, values, ids, stash, dloss, weights=None, temperature=1.0):
     """d sum(dloss * loss) / d logits, contiguous, in the logits' type.  `stash` from distill_fwd on the same arguments."""
-    call = _distill_args(logits, values, ids, None, weights, temperature)
     _same(logits, "dloss", dloss, torch.float32, logits.shape[:-1])
-    _same(logits, "stash", stash, torch.float32, (call[1] * _STASH,))
+    _same(logits, "stash", stash, torch.float32, (logits.shape[:-1].numel() * _STASH,))
+    if not stash.is_contiguous():
+        raise ValueError("stash must be contiguous, as distill_fwd returns it")
+    call = _distill_args(logits, values, ids, None, weights, temperature)
     return _distill_bwd(logits, call[:5] + call[9:], call[5], call[6], call[8], stash, dloss)
 
 

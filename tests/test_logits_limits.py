@@ -25,3 +25,11 @@ def test_sampling_refuses_a_vocabulary_whose_mass_would_wrap(pg):
     assert sample(lib, p, 1, 1 << 24) == UNSUPPORTED and sample(lib, p, 1, (1 << 24) + 1) == UNSUPPORTED
     assert sample(lib, p, 1, (1 << 24) - 1) == WORKSPACE
     assert lib.pg_distill_fwd(0, p, 1 << 24, 1, 1 << 24, p, p, 3, None, None, 1.0, p, p, None, 0, None) == WORKSPACE
+
+
+@pytest.mark.parametrize("stash", [torch.zeros(1).expand(32), torch.zeros(64)[::2], torch.zeros(31), torch.zeros(4, 8)])
+def test_distill_bwd_refuses_a_stash_of_another_layout(pg, stash):
+    """The kernel reads eight numbers a row one behind the other; an expanded or strided stash holds fewer in a row than that."""
+    x, v, i = torch.zeros(4, 10), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="stash"):
+        pg.ops.distill_bwd(x, v, i, stash, torch.ones(4))
