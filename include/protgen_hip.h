@@ -325,6 +325,8 @@ int pg_commit_topk(int64_t* ids, const int64_t* pred, const float* conf, int B, 
  * type.  Entries of a row are ordered by value, ties by the lower index; NaN counts as -inf, -0 as +0.  Workspaces: the
  * *_workspace_bytes functions (may be 0; then NULL will do); a workspace is 16-byte aligned and serves one
  * call at a time.  temperature lies in 1e-30 .. 1e30 (pg_sample_filtered: or is 0; finite ones outside count as the nearer end).
+ * A launch counts its threads in 32 bits: up to 2^23 - 9 rows always fit, from 2^23 to 2^27 by the vocabulary and the call (else
+ * PG_ERR_UNSUPPORTED, before a launch).
  *
  * pg_top_logits: a teacher's record of each row, for pg_distill_*: the first k <= min(V, 1024) entries (values [T][k] in the
  * activation type, ids [T][k], in order) and rest[t] = log sum over the other entries of exp(x / temperature) (-inf if there is

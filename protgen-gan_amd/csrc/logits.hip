@@ -2188,16 +2188,21 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const T* __restrict_
 
 int check_launch() { return hipGetLastError() == hipSuccess ? PG_OK : PG_ERR_LAUNCH; }
 
+// A launch counts its threads in 32 bits: no call with more rows than that leaves for so many threads a row (their number rounded up to
+// a workgroup's eight).
+bool fits(int rows, int threads) { return ((int64_t)rows + 8) * threads < 1ll << 32; }
+
 int check_rows(int dtype, const void* logits, int64_t ld, int T, int V) {
   if (!logits || T <= 0 || V <= 0 || ld < 0 || (dtype != PG_F32 && dtype != PG_BF16)) return PG_ERR_ARG;
-  return V > MAX_VOCAB ? PG_ERR_UNSUPPORTED : PG_OK;
+  return V > MAX_VOCAB || !fits(T, 32) ? PG_ERR_UNSUPPORTED : PG_OK;
 }
+bool small_rows(int V, int k) { return V <= 64 && k <= 64; }
 int check_distill(int dtype, const void* logits, int64_t ld, int T, int V, const void* values, const int32_t* ids, int k,
                   float tau) {
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
   if (!values || !ids || k <= 0 || !(tau >= MIN_TAU && tau <= MAX_TAU)) return PG_ERR_ARG;
-  return k > MAX_K ? PG_ERR_UNSUPPORTED : PG_OK;
+  return k > MAX_K || !fits(T, !small_rows(V, k) ? 256 : V <= 32 && k <= 32 ? 32 : 64) ? PG_ERR_UNSUPPORTED : PG_OK;
 }
 
 template <typename T>
@@ -2237,10 +2242,13 @@ Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
   if (!rows && !ends && !few_long_rows(T, V)) return {0, 0, 0, 0, false, 1};
   return cut_rows(dtype, T, V, sample_k(a.ks ? 0 : a.top_k));
 }
+// The segments' lists hold the first k of every row.
+bool settled(const Cut& cut, const SampleArgs& a) { return cut.nt && !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K; }
 // Parts of a row that the lists do not settle, 0: whole rows only.
 int split_parts(int dtype, int T, int V, const SampleArgs& a) {
-  const bool settled = !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K, both = !a.ks && a.top_k > MAX_SEG_K && a.top_k < V && !a.ps && a.top_p < 1.f;
-  if (settled || both || !few_long_rows(T, V) || sample_cut(dtype, T, V, a).nt == 0) return 0;
+  const bool both = !a.ks && a.top_k > MAX_SEG_K && a.top_k < V && !a.ps && a.top_p < 1.f;
+  const Cut cut = sample_cut(dtype, T, V, a);
+  if (settled(cut, a) || both || !few_long_rows(T, V) || cut.nt == 0) return 0;
   int parts = 1024 / T;
   if (parts > V / 8192) parts = V / 8192;
   return parts > 16 ? 16 : parts < 2 ? 2 : parts;
@@ -2275,8 +2283,7 @@ int sample_rows(const T* x, int64_t ld, const float* q, int64_t ldq, int n, int 
       hipLaunchKernelGGL((sample_part_kernel<T, 512>), dim3(n, parts), dim3(512), 0, s, x, ld, q, ldq, V, a, pred, conf, split);
       hipLaunchKernelGGL((sample_join_kernel<256>), dim3(n), dim3(256), 0, s, q, ldq, V, a, parts, pred, conf, split);
     }
-    const bool settled = cut.nt && !a.ks && a.top_k > 0 && a.top_k <= MAX_SEG_K;  // the lists hold the first k
-    if (!settled)
+    if (!settled(cut, a))
       hipLaunchKernelGGL((sample_row_kernel<T, 512>), dim3(n), dim3(512), 0, s, x, ld, q, ldq, V, a, cut.nt == 0, pred, conf);
   }
   return check_launch();
@@ -2293,7 +2300,6 @@ int distill_small(const T* x, int64_t ld, int n, int V, const DistillArgs& a, fl
                        up, grad, ldg);
   return check_launch();
 }
-bool small_rows(int V, int k) { return V <= 64 && k <= 64; }
 
 // Segments of a row: one where the rows fill the chip (four workgroups a CU), else as many as do, none below 1024 vectors; a
 // segment's membership bits fit MAX_MEMBER.
@@ -2364,7 +2370,7 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
   const int rc = check_rows(dtype, logits, ld, T, V);
   if (rc != PG_OK) return rc;
   if (!values || !ids || !rest || k <= 0 || k > V || !(temperature >= MIN_TAU && temperature <= MAX_TAU)) return PG_ERR_ARG;
-  if (k > MAX_K) return PG_ERR_UNSUPPORTED;
+  if (k > MAX_K || !fits(T, V <= 32 ? 32 : V <= 64 ? 64 : 256)) return PG_ERR_UNSUPPORTED;
   const int64_t need = pg_top_logits_workspace_bytes(dtype, T, V, k);
   if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
@@ -2388,10 +2394,11 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
   if ((!temps && !(temperature >= 0.f && temperature <= FLT_MAX)) || (!ks && top_k < 0) || (!ps && !(top_p > 0.f && top_p <= 1.f)) ||
       (!mins && !(min_p >= 0.f && min_p <= 1.f)))
     return PG_ERR_ARG;
+  const SampleArgs a = {temperature, top_p, min_p, top_k, empty, temps, ks, ps, mins};
+  if (!fits(T, V <= 32 ? 32 : V <= 64 ? 64 : settled(sample_cut(dtype, T, V, a), a) ? 256 : 512)) return PG_ERR_UNSUPPORTED;
   const int64_t need = pg_sample_filtered_workspace_bytes(dtype, T, V, ks ? 0 : top_k);
   if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;
-  const SampleArgs a = {temperature, top_p, min_p, top_k, empty, temps, ks, ps, mins};
   return dtype == PG_F32 ? sample_rows((const float*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream)
                          : sample_rows((const bf16_t*)logits, ld, noise, ld_noise, T, V, a, pred, conf, workspace, (hipStream_t)stream);
 }
@@ -2440,6 +2447,7 @@ extern "C" int pg_distill_loss_grad(int dtype, const void* logits, int64_t ld, i
   const int bad = check_distill(dtype, logits, ld, T, V, values, ids, k, temperature);
   if (bad != PG_OK) return bad;
   if (!loss || !dlogits || ld_dlogits < V) return PG_ERR_ARG;
+  if (V / (dtype == PG_F32 ? 4 : 8) > 256 * 16 && !fits(T, 512)) return PG_ERR_UNSUPPORTED;  // (rows in the registers of 512 threads)
   const int64_t need = pg_distill_workspace_bytes(dtype, T, V, k, 1);
   if (need && (!workspace || workspace_bytes < need)) return PG_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return PG_ERR_ALIGN;

@@ -223,6 +223,9 @@ def sample_tokens(logits, noise, temperature: float, pred=None, conf=None):
 
 
 # ----------------------------------------------------------------------------- rows of logits
+_INT_MAX = 2 ** 31 - 1
+
+
 def _rows(x, what="logits"):
     """x [..., V] as (T, V, ld): rows of unit stride at a common distance, without a copy."""
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -233,6 +236,8 @@ def _rows(x, what="logits"):
         except RuntimeError:
             raise ValueError(f"{what}: the leading dimensions of {tuple(x.shape)} have no common row stride; pass a contiguous tensor")
     T, V = x.shape
+    if max(T, V) > _INT_MAX:  # (the C ABI's int)
+        raise ValueError(f"{what}: {T} rows of {V} are more than a call takes")
     if V > 1 and x.stride(1) != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
     return T, V, (x.stride(0) if T > 1 else V)
@@ -337,7 +342,7 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError(f"top_p must lie in (0, 1], got {top_p}")
     if not 0.0 <= min_p <= 1.0:
         raise ValueError(f"min_p must lie in [0, 1], got {min_p}")
-    if empty < -1:
+    if not -1 <= empty <= _INT_MAX:
         raise ValueError(f"empty must be a token or -1, got {empty}")
     top_k = min(top_k, V)
     _need_cuda(logits)

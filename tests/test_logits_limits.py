@@ -33,3 +33,36 @@ def test_distill_bwd_refuses_a_stash_of_another_layout(pg, stash):
     x, v, i = torch.zeros(4, 10), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int32)
     with pytest.raises(ValueError, match="stash"):
         pg.ops.distill_bwd(x, v, i, stash, torch.ones(4))
+
+
+def test_rows_beyond_a_launch_are_refused(pg):
+    """A launch counts its threads in 32 bits: 32 or 64 threads a row up to 64 entries, 256 or 512 above."""
+    lib, p = pg._lib.lib, torch.zeros(64).data_ptr()
+    top = lambda T, V: lib.pg_top_logits(0, p, V, T, V, 3, 1.0, p, p, p, None, 0, None)  # noqa: E731
+    fwd = lambda T, V, k=3: lib.pg_distill_fwd(0, p, V, T, V, p, p, k, None, None, 1.0, p, p, None, 0, None)  # noqa: E731
+    bwd = lambda T, V, k=3: lib.pg_distill_bwd(0, p, V, T, V, p, p, k, None, 1.0, None, p, p, V, None)  # noqa: E731
+    both = lambda T, V, k=3: lib.pg_distill_loss_grad(0, p, V, T, V, p, p, k, None, None, 1.0, p, p, V, None, 0, None)  # noqa: E731
+    for call in (top, fwd, bwd, both, lambda T, V: sample(lib, p, T, V)):
+        assert call(2 ** 27, 30) == UNSUPPORTED and call(2 ** 26, 40) == UNSUPPORTED and call(2 ** 31 - 1, 4) == UNSUPPORTED
+        assert call(2 ** 24, 300) == UNSUPPORTED
+    for call in (fwd, bwd, both):  # (records of more than 64 entries, or 32, take the wider forms)
+        assert call(2 ** 24, 30, 100) == UNSUPPORTED and call(2 ** 26, 30, 40) == UNSUPPORTED
+    assert both(2 ** 23, 20000) == UNSUPPORTED
+    big = torch.zeros(1 << 20, dtype=torch.uint8)  # (a workspace, by its address and a size that is asked for only)
+    at = (big.data_ptr() + 15) // 16 * 16
+    assert lib.pg_sample_filtered(0, p, 300, p, 300, 2 ** 23, 300, 1.0, 0, 0.5, 0.0, None, None, None, None, -1, p, p, at, 2 ** 62, None) == UNSUPPORTED
+
+
+def test_sizes_beyond_the_int_of_the_c_abi_are_refused(pg):
+    """2^32 + 1 rows would arrive as one."""
+    one = torch.zeros(1)
+    for T, V in ((2 ** 32 + 1, 1), (2 ** 31, 1), (1, 2 ** 32 + 7)):
+        x = one.expand(T, V)
+        with pytest.raises(ValueError, match="more than a call takes"):
+            pg.ops.top_logits(x, 1)
+        with pytest.raises(ValueError, match="more than a call takes"):
+            pg.ops.sample_filtered(x, x)
+        with pytest.raises(ValueError, match="more than a call takes"):
+            pg.ops.distill_loss_grad(x, one.expand(T, 1), one.int().expand(T, 1))
+    with pytest.raises(ValueError, match="empty"):
+        pg.ops.sample_filtered(torch.zeros(2, 3), torch.ones(2, 3), empty=2 ** 32)
