@@ -2305,7 +2305,7 @@ int distill_small(const T* x, int64_t ld, int n, int V, const DistillArgs& a, fl
 // segment's membership bits fit MAX_MEMBER.
 int distill_segs(int dtype, int T, int V) {
   const int e = dtype == PG_F32 ? 4 : 8;
-  int nseg = (1024 + T - 1) / T;
+  int nseg = T < 1024 ? (1024 + T - 1) / T : 1;
   const int most = V / (1024 * e), least = (V + MAX_MEMBER - 1) / MAX_MEMBER;
   if (nseg > most) nseg = most;
   return nseg < least ? least : nseg < 1 ? 1 : nseg;
@@ -2361,6 +2361,7 @@ int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, flo
 }  // namespace
 
 extern "C" int64_t pg_top_logits_workspace_bytes(int dtype, int T, int V, int k) {
+  if (T <= 0 || V <= 0 || k <= 0) return 0;  // (sizes that the call refuses)
   const Cut cut = cut_rows(dtype, T, V, k);
   return cut.nseg > 1 ? (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8) : 0;
 }
@@ -2379,6 +2380,7 @@ extern "C" int pg_top_logits(int dtype, const void* logits, int64_t ld, int T, i
 }
 
 extern "C" int64_t pg_sample_filtered_workspace_bytes(int dtype, int T, int V, int top_k) {
+  if (T <= 0 || V <= 0 || top_k < 0) return 0;
   const Cut cut = cut_rows(dtype, T, V, sample_k(top_k));
   return (int64_t)T * cut.nseg * (sizeof(SegHead) + (int64_t)cut.cap * 8) + (few_long_rows(T, V) ? (int64_t)T * sizeof(SplitRow) : 0);
 }
@@ -2405,7 +2407,7 @@ extern "C" int pg_sample_filtered(int dtype, const void* logits, int64_t ld, con
 
 extern "C" int64_t pg_distill_stash_floats(void) { return STASH; }
 extern "C" int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k, int with_grad) {
-  if (small_rows(V, k)) return 0;
+  if (T <= 0 || V <= 0 || k <= 0 || small_rows(V, k)) return 0;
   const int64_t nseg = distill_segs(dtype, T, V);
   return nseg == 1 ? 0 : T * (nseg * 16 + (with_grad ? STASH * 4 : 0));
 }

@@ -66,3 +66,16 @@ def test_sizes_beyond_the_int_of_the_c_abi_are_refused(pg):
             pg.ops.distill_loss_grad(x, one.expand(T, 1), one.int().expand(T, 1))
     with pytest.raises(ValueError, match="empty"):
         pg.ops.sample_filtered(torch.zeros(2, 3), torch.ones(2, 3), empty=2 ** 32)
+
+
+@pytest.mark.parametrize("T,V", [(0, 1000), (0, 30), (-1, 1000), (-(2 ** 31), 100000), (4, 0), (4, -1), (0, 0)])
+def test_workspace_of_sizes_that_are_refused_is_nothing(pg, T, V):
+    """(Zero rows once divided by zero, which ends the process.)"""
+    lib, p = pg._lib.lib, torch.zeros(64).data_ptr()
+    for dt in (0, 1):
+        for k in (3, 100, 0, -1):
+            assert lib.pg_top_logits_workspace_bytes(dt, T, V, k) == 0 and lib.pg_sample_filtered_workspace_bytes(dt, T, V, k) == 0
+            assert lib.pg_distill_workspace_bytes(dt, T, V, k, 0) == 0 and lib.pg_distill_workspace_bytes(dt, T, V, k, 1) == 0
+            assert lib.pg_distill_loss_grad(dt, p, 8, T, V, p, p, k, None, None, 1.0, p, p, 8, None, 0, None) == ARG
+    for T in (1, 1023, 1024, 2 ** 22, 2 ** 31 - 1):  # (and of the largest counts no overflow)
+        assert lib.pg_distill_workspace_bytes(0, T, 100000, 3, 1) >= 0
