@@ -224,6 +224,7 @@ def sample_tokens(logits, noise, temperature: float, pred=None, conf=None):
 
 # ----------------------------------------------------------------------------- rows of logits
 _INT_MAX = 2 ** 31 - 1
+_FP32_LEAST = 2.0 ** -126
 
 
 def _rows(x, what="logits"):
@@ -344,7 +345,12 @@ def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError(f"min_p must lie in [0, 1], got {min_p}")
     if not -1 <= empty <= _INT_MAX:
         raise ValueError(f"empty must be a token or -1, got {empty}")
-    top_k = min(top_k, V)
+    # (numbers that fp32 does not hold arrive as the nearest that means the same, not as 0 or infinity)
+    top_k, top_p = min(top_k, V), max(top_p, _FP32_LEAST)
+    if temperature > 0.0:
+        temperature = min(max(temperature, 1e-30), 1e30)
+    if min_p > 0.0:
+        min_p = max(min_p, _FP32_LEAST)
     _need_cuda(logits)
     if pred is None:
         pred = torch.empty(T, dtype=torch.int64, device=dev)

@@ -166,3 +166,23 @@ def test_the_largest_sampled_vocabulary(pg):
     assert int(pred) == int(q[0, :2 ** 23].argmin()) and float(conf) == 2.0 ** -23
     pred, conf = pg.ops.sample_filtered(x, q)
     assert int(pred) == int(q[0].argmin())
+
+
+@pytest.mark.parametrize("V", [30, 700, 20000])
+def test_settings_that_fp32_does_not_hold(pg, V):
+    """Numbers within the documented ranges that fp32 rounds to 0 or infinity mean the nearest that it holds."""
+    x = rows(4, V, torch.float32, V)
+    for p in (1e-38, 1e-45, 1e-50, 1e-300):
+        check_sample(pg, x, top_p=p)
+    for least in (1e-45, 1e-50, 1e-300):
+        check_sample(pg, x, min_p=least)
+    x[:, V // 3] = x[:, V // 2] = 50.0
+    q = torch.ones(4, V, device=DEV)
+    q[:, V // 2] = 0.5
+    for temp in (1e-45, 1e-50, 1e-300):  # (above 0: the largest entries race)
+        pred, conf = pg.ops.sample_filtered(x, q, temperature=temp)
+        assert (pred == V // 2).all() and (conf == 0.5).all()
+    q[:, 1] = 0.25
+    for temp in (1e31, 1e39, 1e300):
+        pred, conf = pg.ops.sample_filtered(x, q, temperature=temp)
+        assert (pred == 1).all() and ((conf * V - 1).abs() < 1e-6).all()
