@@ -186,3 +186,68 @@ def test_settings_that_fp32_does_not_hold(pg, V):
     for temp in (1e31, 1e39, 1e300):
         pred, conf = pg.ops.sample_filtered(x, q, temperature=temp)
         assert (pred == 1).all() and ((conf * V - 1).abs() < 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V", [(12, 30), (12, 64), (12, 700), (300, 5001), (4, 40000)])
+def test_rows_with_many_infinite_logits(pg, dtype, T, V):
+    """Half of the entries, one in forty or all are +inf: they share the row."""
+    x = rows(T, V, dtype, V)
+    g = torch.Generator().manual_seed(V)
+    u = torch.rand(T, V, generator=g).to(DEV)
+    share = torch.tensor([0.5, 0.025, 2.0, 0.0], device=DEV).repeat(T)[:T].view(T, 1)
+    x[u < share] = float("inf")
+    check_top(pg, x, min(V, 50))
+    for n, f in enumerate([{}, {"top_k": 3}, {"top_p": 0.6}, {"min_p": 0.3}, {"temperature": 0.0}, {"top_k": V // 2, "top_p": 0.9},
+                           {"top_p": 0.3, "min_p": 1.0}]):
+        check_sample(pg, x, seed=n, **f)
+
+
+def test_the_largest_vocabulary_of_records_and_distillation(pg):
+    V, k, tau = 2 ** 24, 5, 2.0
+    x = torch.randn(2, V, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    v, i, r = pg.ops.top_logits(x, k, temperature=tau)
+    wv, wi = x.topk(k, dim=1)
+    assert torch.equal(v, wv) and torch.equal(i.long(), wi)
+    z = (x.double() / tau).scatter(1, wi, float("-inf"))
+    U = 2.0 ** -24
+    # (a thread adds V / 256 entries in a row, the workgroup joins 256 sums)
+    assert ((r.double() - torch.logsumexp(z, 1)).abs() <= (V // 256 + 48) * U).all()
+    student = (0.5 * x + torch.randn(2, V, device=DEV, generator=torch.Generator(DEV).manual_seed(2)))
+    loss, grad = pg.ops.distill_loss_grad(student, v, i, rest=r, temperature=tau)
+    wl, wg, ls, gs = spec.distill(student, v, i, r, tau, None)
+    a = (V // 256 + 48 + 64) * U
+    assert (np.abs(loss.double().cpu().numpy() - wl) <= a * ls).all()
+    assert (np.abs(grad.double().cpu().numpy() - wg) <= a * gs + U * np.abs(wg) * 1.01 + 1e-38).all()
+
+
+def test_captured_distillation_loss(pg):
+    """Forward and backward by autograd captured once and replayed on new inputs, with eager calls of the same between."""
+    cases = []
+    for T, V, dtype in ((64, 30, torch.float32), (4, 70001, torch.bfloat16), (3, 900, torch.float32)):
+        x, v, i, r = record(pg, T, V, 7, dtype, V, 2.0, True)
+        cases.append((x, v, i, r, torch.rand(T, device=DEV), torch.randn(T, device=DEV)))
+
+    def work():
+        out = []
+        for x, v, i, r, w, up in cases:
+            leaf = x.detach().requires_grad_()
+            loss = pg.loss.distillation_loss(leaf, v, i, rest=r, temperature=2.0, weights=w)
+            out += [loss.detach(), torch.autograd.grad(loss, leaf, up)[0]]
+        return out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for n in range(4):
+        for x, v, i, r, w, up in cases:
+            x.add_((0.37 * torch.randn(x.shape, generator=torch.Generator().manual_seed(n))).to(x.dtype).to(DEV))
+        graph.replay()
+        eager = work()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
