@@ -355,7 +355,7 @@ int pg_sample_filtered(int dtype, const void* logits, int64_t ld, const float* n
  * An id that occurs twice counts as two entries and once in the set that s_rest leaves out.  weights [T] (NULL = 1): a row with
  * weight 0 is not read and gives loss 0 and gradient 0, and so does a row with no entry or with no logit above -inf.
  * pg_distill_fwd leaves pg_distill_stash_floats() floats per row (16-byte aligned) for pg_distill_bwd, which writes
- * dlogits = dloss[t] d loss[t] / d logits (activation type, every entry of every row; dloss NULL = 1);
+ * dlogits = dloss[t] d loss[t] / d logits (activation type, every entry of every row, no overlap with logits; dloss NULL = 1);
  * pg_distill_loss_grad is both in one call, for updates that know the weights beforehand. */
 int64_t pg_distill_stash_floats(void);
 int64_t pg_distill_workspace_bytes(int dtype, int T, int V, int k, int with_grad /* 1: for pg_distill_loss_grad */);

@@ -219,7 +219,8 @@ struct FixedSum {
   }
   __device__ __forceinline__ ExpSum end() const { return {m, s * __builtin_amdgcn_exp2f(-fmaf(m, c, -mc))}; }
 };
-// 16 bytes of a row that is read once: past the caches (6.4 TB/s against 5.6 of ordinary loads, 256 MB).
+// 16 bytes of a row that is read once: past the caches (1024 x 131072 bf16, k 64: 91 us against 95 with ordinary loads; loss and
+// gradient of 4096 x 32768 bf16: 133 against 144).
 __device__ __forceinline__ uint4 load_once(const void* p) {
   typedef __attribute__((ext_vector_type(4))) uint32_t u4;
   const u4 v = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
@@ -617,9 +618,10 @@ __device__ __forceinline__ void top_finish(uint64_t* list, int n, int K, float t
     *rest_out = rest.m == INFINITY ? INFINITY : rest.s > 0.f ? (float)((double)rest.m / tau + log((double)rest.s)) : -INFINITY;
 }
 
-// 1024 rows of 131072 bf16, k 64: 88-92 us (268 MB; reading alone 45), whole rows by one workgroup of 256, four a CU.  A segment's load, the
+// 1024 rows of 131072 bf16, k 64: 91 us (268 MB; reading alone 45), whole rows by one workgroup of 256, four a CU.  A segment's load, the
 // rounds that count for the bound, and the sum follow one another, and four workgroups overlap them only in part; a fifth does
-// not fit beside 128 registers a thread.  16 rows of 50021 fp32, k 100, in 13 segments each: 8.9 us.
+// not fit beside 128 registers a thread (the next segment's loads straight into LDS, which would take none, were not tried).  16 rows
+// of 50021 fp32, k 100, in 13 segments each: 8.8 us.
 template <typename T, int NT, int VPT, bool MANY>
 __global__ __launch_bounds__(NT, 4) void top_segment_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, int cap, int count, float tau,
                                                          T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest_out,
@@ -753,7 +755,8 @@ struct MergeLds {
 };
 
 // One workgroup a row, bound by latency: the lists' lengths, their keys, the bound and the sort wait for memory and LDS one after
-// the other.  16 rows of 13 lists, k 100: 19 us; 1000 rows of 4 lists, k 512: 60 us.
+// the other, and the bound's eight rounds read the keys from scratch memory (160 bytes a lane: loops over RowKeys::k end at a run-time
+// count).  16 rows of 13 lists, k 100: 19 us; 1000 rows of 4 lists, k 512: 58 us.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void top_merge_kernel(int nseg, int K, int cap, float tau, T* __restrict__ values,
                                                        int32_t* __restrict__ ids, float* __restrict__ rest_out,
@@ -775,6 +778,8 @@ Cut cut_rows(int dtype, int T, int V, int K) {
   if (K > MAX_SEG_K || V <= 64) return none;
   const bool many = K > 128;
   const int vecs = V / (dtype == PG_F32 ? 4 : 8);
+  // (64 threads leave 64 maxima: for K above that there is no bound, all entries are listed, and rows of more than `cap` of them go
+  // by digits; 4096 x 1000 bf16: k 32 14 us, k 100 34)
   const int shapes[3][2] = {{64, 4}, {256, 4}, {256, 16}};
   for (int i = many ? 1 : 0; i < 3; ++i) {
     const int per = shapes[i][0] * shapes[i][1], nseg = vecs <= per ? 1 : (vecs + per - 1) / per;
@@ -1012,8 +1017,8 @@ __device__ __forceinline__ void finish(const Race& race, double kept_mass, uint3
 }
 
 // From the segments' lists, if the end of the kept entries lies within them.  A row where it does not is left to
-// sample_row_kernel: pred = -2 - (index of its largest entry), conf = that entry.  Bound by latency as the merge: 13 us a row, 19 us
-// for 256 rows of 4 lists.
+// sample_row_kernel: pred = -2 - (index of its largest entry), conf = that entry.  Bound as the merge, its keys in scratch memory too
+// (1024 rows write 39 MiB of it): 13 us a row, 19 us for 256 rows of 4 lists.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void sample_list_kernel(const float* __restrict__ noise, int64_t ld_noise, int V, SampleArgs args,
                                                          int nseg, int cap, const SegHead* __restrict__ heads,
@@ -1211,8 +1216,8 @@ __device__ __forceinline__ void sweep(const T* p, int n, int i0, const float* q,
 }
 
 // From the whole row: every row (all), or those sample_list_kernel left.  The border of top-k, then of top-p among those, then
-// the race.  One workgroup a row, bound by the 64-bit exponentials of its CU: 1024 rows of 32768 bf16 without a filter 141 us, with
-// a nucleus that the lists do not hold 196 us.
+// the race.  One workgroup a row, bound by the 64-bit exponentials of its CU, one for every entry: 1024 rows of 32768 bf16 (normal
+// logits) without a filter 135 us, at top_p 0.95, which the lists do not hold, 220 us.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__ logits, int64_t ld, const float* __restrict__ noise,
                                                         int64_t ld_noise, int V, SampleArgs args, bool all, int64_t* __restrict__ pred,
@@ -1279,7 +1284,9 @@ __global__ __launch_bounds__(NT, 2) void sample_row_kernel(const T* __restrict__
 // The rows sample_list_kernel left, where there are few rows: each cut into parts for several CUs, in three launches (bins of the
 // parts added up; the race of the parts, the border's entries listed; the border and the race joined).  For rows with one border or
 // none; a row with both filters open, or with more entries in the border's bin than the list holds, stays for sample_row_kernel.
-// 256 rows of 32768 bf16, normal logits, top_p 0.95: bins 16 us, race 44, join 9; one row: 5, 11-17, 7.
+// The parts are counted from all rows of the call: where the lists leave only a few, most workgroups return at once and as few CUs
+// work.  256 rows of 32768 bf16, normal logits, top_p 0.95 (all left): bins 15 us, race 49, join 10; one row: 5, 19, 8; 256 of 131072
+// of which the lists leave about one in twenty: 40, 45, 24.
 struct SplitPart { double best, total; uint64_t at; float x; int pad; };
 struct SplitRow {  // one per row, in the workspace
   uint64_t mass[BINS], list[POOL];
@@ -1432,7 +1439,7 @@ __global__ __launch_bounds__(NT, 4) void sample_segment_kernel(const T* __restri
 
 // ------------------------------------------------------------------ top entries, any k and vocabulary
 // For k above MAX_SEG_K, and where lists of k do not fit one merge: the row three to four times through the caches.  1024 rows of
-// 131072 bf16, k 1024: 255 us.
+// 131072 bf16, k 1024: 276 us for normal logits, 342 with a few entries far above the rest.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void top_kernel(const T* __restrict__ logits, int64_t ld, int V, int K, float tau,
                                                  T* __restrict__ values, int32_t* __restrict__ ids, float* __restrict__ rest) {
@@ -1761,7 +1768,7 @@ __device__ __forceinline__ void distill_grad(const T* row, int V, const Span<T>&
 }
 
 // LOSS: loss and, without GRAD, the stash; GRAD: the gradient, from this pass's numbers or (not LOSS) the stash.  LOSS takes whole
-// rows (grid n x 1), GRAD alone may have them cut (grid n x nseg).  Bound by memory: 2048 rows of 131072 bf16, k 64, loss 96-165 us
+// rows (grid n x 1), GRAD alone may have them cut (grid n x nseg).  Bound by memory: 2048 rows of 131072 bf16, k 64, loss 129-165 us
 // (537 MB), gradient 178 us (1074 MB, 6.0 TB/s).
 template <typename T, int NT, bool LOSS, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
@@ -1799,7 +1806,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ logit
 
 // Loss and gradient with the row in registers, read once: NT * 16 vectors of 16 bytes.  4096 x 32768 bf16, k 32: 130 us, against the
 // 105 of reading and writing it once at the rate of a copy; two passes, the second from the memory-side cache, took 168.  2048 x 65536
-// by 512 threads: 141 us.
+// by 512 threads: 134 us; 4096 rows of 1000, where most of the 16 vectors a thread are empty: 50.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT, 4) void distill_resident_kernel(const T* __restrict__ logits, int64_t ld, int V, DistillArgs a,
                                                                   float* __restrict__ loss, T* __restrict__ grad, int64_t ld_grad) {
@@ -2232,7 +2239,7 @@ int top_rows(const T* x, int64_t ld, int n, int V, int k, float tau, T* values, 
 
 // The entries the segments look for: k itself where it is one number up to 512, else 128, the end of most nucleus and min-p
 // sets.  No segments where they could not end the kept set: no filter at all, or a larger k that only top_p or nothing can undercut.
-bool few_long_rows(int T, int V) { return T <= 256 && V >= 16384; }  // (more rows fill the chip whole)
+bool few_long_rows(int T, int V) { return T <= 256 && V >= 16384; }  // (more rows: each that the lists leave by one workgroup)
 int sample_k(int top_k) { return top_k > 0 && top_k <= MAX_SEG_K ? (top_k < 16 ? 16 : top_k) : 128; }
 Cut sample_cut(int dtype, int T, int V, const SampleArgs& a) {
   const bool rows = a.temps || a.ks || a.ps || a.mins;
@@ -2348,7 +2355,7 @@ int distill_both(const T* x, int64_t ld, int n, int V, const DistillArgs& a, flo
       hipLaunchKernelGGL((distill_resident_kernel<T, 256>), dim3(n), dim3(256), lds, s, x, ld, V, a, loss, grad, ldg);
     else if (vecs <= 512 * 16)
       hipLaunchKernelGGL((distill_resident_kernel<T, 512>), dim3(n), dim3(512), lds, s, x, ld, V, a, loss, grad, ldg);
-    else  // (a workgroup of 1024 holds 131072 bf16 entries, alone on its CU: 408 us for 2048 rows, two passes 350)
+    else  // (a workgroup of 1024 holds 131072 bf16 entries, alone on its CU: 354 us for 2048 rows, two passes 312)
       hipLaunchKernelGGL((distill_kernel<T, 256, true, true>), dim3(n), dim3(256), member_bytes(V, 1, a.rest != nullptr), s, x, ld, V, a,
                          loss, (float*)nullptr, (const float*)nullptr, grad, ldg);
     return check_launch();

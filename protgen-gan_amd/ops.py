@@ -311,12 +311,14 @@ TOP_LOGITS_MAX = 1024  # entries of a teacher's record
 
 
 def sample_filtered(logits, noise, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, empty=-1, pred=None, conf=None):
-    """One token per row of logits [T, V] (fp32 or bf16, any V) from the softmax at `temperature`, cut to the first `top_k`
+    """One token per row of logits [T, V] (fp32 or bf16, V below 2^24) from the softmax at `temperature`, cut to the first `top_k`
     entries (0: all), of those to the smallest leading set that holds `top_p` of their mass, and to the entries of at least
     `min_p` times the largest probability.  `noise` fp32 [T, V] ~ Exp(1): the token is the argmax of p / noise, as in
-    sample_tokens; only the kept entries' noise is read.  Every setting is a number or a tensor [T] on the device (fp32; top_k:
-    int32), read per row without a check.  temperature 0: the largest entry; 1e-30 is the least above it.  Returns (pred int64 [T], conf fp32 [T]), conf the
-    token's probability among the kept entries; a row with nothing above -inf gives (`empty`, 0)."""
+    sample_tokens; only the kept entries' noise counts.  temperature 0: the largest entry; 1e-30 is the least above it.  Every
+    setting is a number or a tensor [T] on the device (fp32; top_k: int32), read per row without a check: there a temperature <= 0
+    or NaN is 0, top_k <= 0, top_p >= 1 or NaN and min_p <= 0 or NaN are off, top_p <= 0 keeps the first entry.  Returns (pred
+    int64 [T], conf fp32 [T]), conf the token's probability among the kept entries; a row with nothing above -inf gives
+    (`empty`, 0)."""
     if logits.dim() != 2:
         raise ValueError(f"logits: expected [T, V], got {tuple(logits.shape)}")
     dt = dt_code(logits.dtype)
