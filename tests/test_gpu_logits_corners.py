@@ -251,3 +251,23 @@ def test_captured_distillation_loss(pg):
         eager = work()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V", [(5, 30), (5, 64), (5, 700), (5, 5001), (5, 40000), (1030, 9001)])
+def test_rows_of_subnormal_logits(pg, dtype, T, V):
+    """Values below the least normal number are ordered as any others."""
+    x = (3e-39 * torch.randn(T, V, generator=torch.Generator().manual_seed(V))).to(dtype).to(DEV)
+    assert 0 < float(x.abs().float().median()) < 2.0 ** -126
+    few = torch.tensor([0, 1, T // 2, T - 1], device=DEV)
+    k = min(V, 20)
+    v, i, _ = pg.ops.top_logits(x, k)
+    wv, wi, _ = spec.top_logits(x[few], k, 1.0)
+    assert np.array_equal(i[few].cpu().numpy(), wi) and np.array_equal(v[few].double().cpu().numpy(), wv)
+    q = torch.empty(T, V, device=DEV).exponential_(1.0, generator=torch.Generator(DEV).manual_seed(V))
+    for f in ({"temperature": 0.0}, {"top_k": 3}, {"top_k": k, "top_p": 0.5}, {"min_p": 1.0}):
+        full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+        full.update(f)
+        pred, _ = pg.ops.sample_filtered(x, q, **full)
+        want, _ = spec.sample(x[few], q[few], full["temperature"], full["top_k"], full["top_p"], full["min_p"])
+        assert np.array_equal(pred[few].cpu().numpy(), want)
