@@ -271,3 +271,14 @@ def test_rows_of_subnormal_logits(pg, dtype, T, V):
         pred, _ = pg.ops.sample_filtered(x, q, **full)
         want, _ = spec.sample(x[few], q[few], full["temperature"], full["top_k"], full["top_p"], full["min_p"])
         assert np.array_equal(pred[few].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [0, 3])
+def test_signalling_nan_in_whole_row_passes(pg, dtype, shift):
+    """Records of more than 512 entries, and rows that no list settles, read in passes over the row."""
+    x = signalling(rows(300, 5003, dtype, 7, pad=2, shift=shift))[:6]
+    check_top(pg, x, 700)
+    check_top(pg, x, 1024, tau=2.0)
+    for n, f in enumerate([{}, {"top_k": 900}, {"top_p": 0.99, "temperature": 8.0}, {"top_k": 2000, "top_p": 0.9, "temperature": 8.0}]):
+        check_sample(pg, x, seed=n, **f)
